@@ -22,7 +22,15 @@ EXPORTS = (
     "arcq_dense_weight_gemm_unpack", "arcq_dense_weight_gemm_unpack_room", "arcq_unpack_beside_gemm", "arcq_dense_weight_gemm_gelu_quant",
     "arcq_dense_weight_gemm_gelu_quant_applies", "arcq_packed_linear_small", "arcq_packed_linear_small_applies",
     "arcq_packed_linear_small_applies_captured",
+    "arcq_kv_cache_write", "arcq_kv_cache_read", "arcq_paged_attention", "arcq_cross_attention",
 )
+
+
+class KvCache(ctypes.Structure):
+    """``arcq_kv_cache`` of the header."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "k_stats", "v_stats", "codebooks")] + [
+        (n, ctypes.c_int64) for n in ("pages", "heads", "page_size")] + [("bits", ctypes.c_int), ("dtype", ctypes.c_int)]
+
 
 _lib = None
 
@@ -75,6 +83,11 @@ def load() -> ctypes.CDLL:
     lib.arcq_packed_linear_small_applies_captured.argtypes = [i64, i64, i64]
     lib.arcq_packed_linear_small.argtypes = [ci, vp, ci, i64, vp, vp, ci, vp, vp, vp, ci, vp]
     lib.arcq_dense_weight_gemm_gelu_quant.argtypes = [vp, vp, vp, i64, i64, i64, vp, vp, ci, ci, vp, vp, ci, vp]
+    cache, strides = ctypes.POINTER(KvCache), ctypes.POINTER(i64)
+    lib.arcq_kv_cache_write.argtypes = [cache, vp, vp, vp, ci, i64, strides, strides, vp, vp]
+    lib.arcq_kv_cache_read.argtypes = [cache, vp, i64, vp, vp, ci, vp]
+    lib.arcq_paged_attention.argtypes = [cache, vp, ci, i64, strides, i64, i64, vp, i64, vp, vp, i64, ci, ctypes.c_float, vp, vp]
+    lib.arcq_cross_attention.argtypes = [vp, vp, vp, ci, i64, i64, i64, i64, i64, strides, strides, strides, vp, vp, i64, ctypes.c_float, vp, vp]
     for name in EXPORTS:
         getattr(lib, name)  # AttributeError here means header and library disagree
     _lib = lib

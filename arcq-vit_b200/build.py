@@ -1,8 +1,8 @@
 """Build recipe for the CUDA shared library (sm_100a only) and the host extension, in-tree.
 
-``python arcq-vit_b200/build.py`` or ``build_library()``: one nvcc call that compiles ``csrc/arcq_b200.cu`` into
-``libarcq_b200.so`` and one g++ call that compiles ``csrc/host_ext.cpp`` (torch tensors in, library calls out) into
-``_arcq_host.so``, both next to this file.  nvcc cross-compiles, so no GPU is needed to build.
+``python arcq-vit_b200/build.py`` or ``build_library()``: nvcc compiles the ``csrc/*.cu`` side by side and links them into
+``libarcq_b200.so``, g++ compiles ``csrc/host_ext.cpp`` (torch tensors in, library calls out) into ``_arcq_host.so``, both next to
+this file.  nvcc cross-compiles, so no GPU is needed to build.
 """
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -21,7 +22,7 @@ HOST_PATH = PKG_DIR / "_arcq_host.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -32,8 +33,12 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; set NVCC or put /usr/local/cuda/bin on PATH")
 
 
+def units():
+    return sorted(CSRC.glob("*.cu"))
+
+
 def sources():
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [PKG_DIR.parent / "include" / "arcq_b200.h"]
+    return units() + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [PKG_DIR.parent / "include" / "arcq_b200.h"]
 
 
 def _older(target: Path, srcs) -> bool:
@@ -64,10 +69,22 @@ def _host_command():
             f"-L{PKG_DIR}", "-larcq_b200", "-Wl,-rpath,$ORIGIN"]
 
 
+def _compile(unit: Path, force: bool, verbose: bool) -> Path:
+    """The unit's object, compiled anew where a file that went into it (nvcc's list beside it) is newer."""
+    obj, used = unit.with_suffix(".o"), unit.with_suffix(".d")
+    names = used.read_text().replace("\\\n", " ").split(":", 1)[-1].split() if used.exists() else []
+    files = [Path(n) for n in names]
+    if force or not files or not all(f.exists() for f in files) or _older(obj, files):
+        _run([_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-c", "-MD", "-MF", str(used), "-o", str(obj), str(unit)], verbose)
+    return obj
+
+
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     """Compile what is missing or older than its sources."""
     if force or _older(LIB_PATH, sources()):
-        _run([_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-o", str(LIB_PATH), str(CSRC / "arcq_b200.cu")], verbose)
+        with ThreadPoolExecutor() as pool:
+            objects = list(pool.map(lambda unit: _compile(unit, force, verbose), units()))
+        _run([_nvcc(), *NVCC_FLAGS, "--shared", "-o", str(LIB_PATH), *map(str, objects)])
     if force or _older(HOST_PATH, [HOST_SOURCE, PKG_DIR.parent / "include" / "arcq_b200.h"]):
         _run(_host_command())
     return LIB_PATH

@@ -1,5 +1,5 @@
 // C ABI of the B200 back end: argument checks, launch configuration, error reporting.
-// The kernels live in the .cuh files included below; this is the only translation unit.
+// The kernels live in the .cuh files included below; those of the key/value cache and its attention are in cache_attention.cu.
 #include <cuda_runtime.h>
 #include <cmath>
 #include <mutex>
@@ -27,6 +27,7 @@
 #include "attention.cuh"
 #include "small_linear.cuh"
 #include "patch_embed.cuh"
+#include "launch.h"
 #include <cudaTypedefs.h>
 
 namespace {
@@ -854,6 +855,16 @@ bool choose_small_linear(long long M, long long N, long long K, SmallLinearConfi
 }
 
 }  // namespace
+
+namespace arcq_host {
+int fail(int code, const char* text) { return ::fail(code, "%s", text); }
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int* status_ptr() { return ::status_ptr(); }
+int sm_count() { return ::sm_count(); }
+bool dependent_launches() { return opt(O_PDL) != 0; }
+uint32_t poll_limit() { return static_cast<uint32_t>(opt(O_POLL_LIMIT)); }
+int launch_regs() { return opt(O_LAUNCH_REGS); }
+}  // namespace arcq_host
 
 extern "C" {
 

@@ -1,0 +1,305 @@
+// C ABI of the key/value cache, attention over it and attention to an encoder's states: argument checks and launches.
+#include <cuda_runtime.h>
+#include <cuda_fp16.h>
+#include <cuda_bf16.h>
+#include <stdint.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <math.h>
+
+#include "../../include/arcq_b200.h"
+#include "launch.h"
+#include "kv_cache.cuh"
+#include "split_attention.cuh"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char text[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(text, sizeof(text), fmt, ap);
+  va_end(ap);
+  return arcq_host::fail(code, text);
+}
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// As a programmatic dependent of the kernel before it (see arcq_b200.cu), `cluster` blocks of the x dimension to a cluster.
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = dim3(threads);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (arcq_host::dependent_launches()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  lc.attrs = attr;
+  lc.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, kernel, static_cast<KArgs>(args)...);
+  const cudaError_t left = cudaGetLastError();
+  return e != cudaSuccess ? e : left;
+}
+
+int log2_of(int64_t v) {
+  int s = 0;
+  while ((1ll << s) < v) ++s;
+  return s;
+}
+
+int check_cache(const arcq_kv_cache* c) {
+  if (c == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (c->bits != 2 && c->bits != 3 && c->bits != 4 && c->bits != 16) return fail(ARCQ_E_BAD_ARG, "bits must be 2, 3, 4 or 16, got %d", c->bits);
+  if (c->heads <= 0 || c->heads > 65535 || c->pages < 0 || c->pages > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad cache: pages=%lld heads=%lld", (long long)c->pages, (long long)c->heads);
+  if (c->page_size < 16 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(ARCQ_E_UNSUPPORTED, "page size %lld: a power of two of at least 16 tokens", (long long)c->page_size);
+  if (c->pages == 0) return ARCQ_OK;
+  if (c->k_pages == nullptr || c->v_pages == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16)) return fail(ARCQ_E_ALIGN, "pages must be 16-byte aligned");
+  if (c->bits == 16) {
+    if (c->dtype != ARCQ_DT_F16 && c->dtype != ARCQ_DT_BF16) return fail(ARCQ_E_BAD_ARG, "pages in 16 bits are fp16 or bf16");
+    return ARCQ_OK;
+  }
+  if (c->k_stats == nullptr || c->v_stats == nullptr || c->codebooks == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (!aligned(c->k_stats, 16) || !aligned(c->v_stats, 16) || !aligned(c->codebooks, 4)) return fail(ARCQ_E_ALIGN, "statistics must be 16-byte aligned");
+  return ARCQ_OK;
+}
+
+arcq::KvCacheParams cache_params(const arcq_kv_cache* c, const int64_t* slots, int64_t tokens) {
+  arcq::KvCacheParams p = {};
+  p.slots = reinterpret_cast<const long long*>(slots);
+  p.tokens = tokens;
+  p.slot_count = c->pages * c->page_size;
+  p.heads = static_cast<int>(c->heads);
+  p.page_shift = log2_of(c->page_size);
+  const int levels = c->bits == 16 ? 0 : 1 << c->bits;
+  for (int i = 0; i < 2; ++i) {
+    p.kv[i].pages = static_cast<uint8_t*>(i ? c->v_pages : c->k_pages);
+    p.kv[i].stats = static_cast<__half2*>(i ? c->v_stats : c->k_stats);
+    p.kv[i].levels = c->codebooks + i * levels;
+  }
+  return p;
+}
+
+int blocks_for(long long items, int per_block, int per_sm) {
+  const long long need = (items + per_block - 1) / per_block, cap = static_cast<long long>(arcq_host::sm_count()) * per_sm;
+  return static_cast<int>(need < 1 ? 1 : need < cap ? need : cap);
+}
+
+template <typename T> cudaError_t write_packed(const arcq::KvCacheParams& p, int bits, cudaStream_t st) {
+  const dim3 grid(blocks_for(p.tokens * p.heads, 32, 4), 2);
+  switch (bits) {
+    case 4: return launch(arcq::kv_write_kernel<T, 4>, grid, 256, 0, 1, st, p);
+    case 3: return launch(arcq::kv_write_kernel<T, 3>, grid, 256, 0, 1, st, p);
+    default: return launch(arcq::kv_write_kernel<T, 2>, grid, 256, 0, 1, st, p);
+  }
+}
+template <typename O> cudaError_t read_cache(const arcq::KvCacheParams& p, int bits, int dtype, cudaStream_t st) {
+  const dim3 grid(blocks_for(p.tokens * p.heads * 8, 256, 4), 2);
+  switch (bits) {
+    case 16:
+      if (dtype == ARCQ_DT_F16) return launch(arcq::kv_read_kernel<__half, 16, O>, grid, 256, 0, 1, st, p);
+      return launch(arcq::kv_read_kernel<__nv_bfloat16, 16, O>, grid, 256, 0, 1, st, p);
+    case 4: return launch(arcq::kv_read_kernel<__half, 4, O>, grid, 256, 0, 1, st, p);
+    case 3: return launch(arcq::kv_read_kernel<__half, 3, O>, grid, 256, 0, 1, st, p);
+    default: return launch(arcq::kv_read_kernel<__half, 2, O>, grid, 256, 0, 1, st, p);
+  }
+}
+
+template <int BITS, typename E> int launch_split(arcq::AttendParams& p, cudaStream_t st) {
+  auto k = arcq::split_attention_kernel<BITS, E>;
+  constexpr size_t smem = 2 * arcq::kPairTableBytes;      // also room for the warps' accumulators
+  static_assert(smem >= arcq::kSplitWarps * arcq::kSplitRows * 64 * 4, "");
+  static thread_local int done_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (done_dev != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return arcq_host::cuda_fail(e, "split attention set-up");
+    done_dev = dev;
+  }
+  p.tiles = static_cast<int>((static_cast<long long>(p.max_new) * p.group + arcq::kSplitRows - 1) / arcq::kSplitRows);
+  const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.tiles;
+  const long long steps = (p.max_keys + arcq::KeyBlock<BITS>::kKeys * arcq::kSplitWarps - 1) / (arcq::KeyBlock<BITS>::kKeys * arcq::kSplitWarps);
+  int splits = 1;
+  while (splits < arcq::kSplitMaxBlocks && splits < steps && units * splits < arcq_host::sm_count()) splits *= 2;
+  p.splits = splits;
+  if (units * splits > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
+  const cudaError_t e = launch(k, dim3(static_cast<unsigned>(units * splits)), arcq::kSplitThreads, smem, splits, st, p);
+  return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
+}
+
+int run_attention(arcq::AttendParams& p, int bits, int dtype, cudaStream_t st) {
+  switch (bits) {
+    case 4: return launch_split<4, __half>(p, st);
+    case 3: return launch_split<3, __half>(p, st);
+    case 2: return launch_split<2, __half>(p, st);
+    default: return dtype == ARCQ_DT_BF16 ? launch_split<16, __nv_bfloat16>(p, st) : launch_split<16, __half>(p, st);
+  }
+}
+
+int check_query(const void* q, int dtype, const void* out, int64_t heads, int64_t kv_heads, float scale) {
+  if (q == nullptr || out == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (dtype != ARCQ_DT_F16 && dtype != ARCQ_DT_BF16) return fail(ARCQ_E_BAD_ARG, "queries are fp16 or bf16");
+  if (heads <= 0 || kv_heads <= 0 || heads > 65535 || heads % kv_heads != 0)
+    return fail(ARCQ_E_BAD_SHAPE, "%lld heads over %lld key heads", (long long)heads, (long long)kv_heads);
+  if (!(scale > 0.0f) || !isfinite(scale)) return fail(ARCQ_E_BAD_ARG, "scale must be positive and finite");
+  if (!aligned(q, 16) || !aligned(out, 16)) return fail(ARCQ_E_ALIGN, "queries and out must be 16-byte aligned");
+  return ARCQ_OK;
+}
+bool strides_ok(const int64_t* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] % 8 != 0) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int arcq_kv_cache_write(const arcq_kv_cache* cache, const float* thresholds, const void* k, const void* v, int x_dtype, int64_t tokens,
+                        const int64_t* k_strides, const int64_t* v_strides, const int64_t* slots, void* stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (tokens < 0 || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
+  if (tokens == 0 || cache->pages == 0) return ARCQ_OK;
+  if (k == nullptr || v == nullptr || slots == nullptr || k_strides == nullptr || v_strides == nullptr || (cache->bits != 16 && thresholds == nullptr))
+    return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (x_dtype != ARCQ_DT_F32 && x_dtype != ARCQ_DT_F16 && x_dtype != ARCQ_DT_BF16) return fail(ARCQ_E_BAD_ARG, "bad element type %d", x_dtype);
+  if (cache->bits == 16 && x_dtype != cache->dtype) return fail(ARCQ_E_BAD_ARG, "keys and values must have the type of the pages");
+  if (!aligned(k, 16) || !aligned(v, 16) || !strides_ok(k_strides, 2) || !strides_ok(v_strides, 2))
+    return fail(ARCQ_E_ALIGN, "keys and values must be 16-byte aligned, their strides multiples of 8 values");
+  arcq::KvCacheParams p = cache_params(cache, slots, tokens);
+  const int levels = cache->bits == 16 ? 0 : (1 << cache->bits) - 1;
+  for (int i = 0; i < 2; ++i) {
+    p.kv[i].x = i ? v : k;
+    p.kv[i].token_stride = (i ? v_strides : k_strides)[0];
+    p.kv[i].head_stride = (i ? v_strides : k_strides)[1];
+    p.kv[i].thresholds = thresholds != nullptr ? thresholds + i * levels : nullptr;
+  }
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (cache->bits == 16) e = launch(arcq::kv_write_copy_kernel, dim3(blocks_for(tokens * cache->heads * 8, 256, 4), 2), 256, 0, 1, st, p);
+  else if (x_dtype == ARCQ_DT_F32) e = write_packed<float>(p, cache->bits, st);
+  else if (x_dtype == ARCQ_DT_F16) e = write_packed<__half>(p, cache->bits, st);
+  else e = write_packed<__nv_bfloat16>(p, cache->bits, st);
+  return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "cache write launch");
+}
+
+int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int out_dtype, void* stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (tokens < 0 || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
+  if (tokens == 0) return ARCQ_OK;
+  if (k_out == nullptr || v_out == nullptr || slots == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16)) return fail(ARCQ_E_ALIGN, "outputs must be 16-byte aligned");
+  arcq::KvCacheParams p = cache_params(cache, slots, tokens);
+  p.kv[0].out = k_out;
+  p.kv[1].out = v_out;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (out_dtype == ARCQ_DT_F32) e = read_cache<float>(p, cache->bits, cache->dtype, st);
+  else if (out_dtype == ARCQ_DT_F16) e = read_cache<__half>(p, cache->bits, cache->dtype, st);
+  else if (out_dtype == ARCQ_DT_BF16) e = read_cache<__nv_bfloat16>(p, cache->bits, cache->dtype, st);
+  else return fail(ARCQ_E_BAD_ARG, "bad element type %d", out_dtype);
+  return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "cache read launch");
+}
+
+int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype, int64_t q_rows, const int64_t* q_strides, int64_t heads,
+                         int64_t batch, const int32_t* page_table, int64_t table_width, const int32_t* lengths, const int32_t* starts,
+                         int64_t max_new, int causal, float scale, void* out, void* stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (batch < 0 || table_width < 0 || max_new < 0 || q_rows < 0 || q_rows > 0x7fffffffLL || batch > 0x7fffffffLL || max_new > 0x7fffffffLL)
+    return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld table=%lld new=%lld rows=%lld", (long long)batch, (long long)table_width, (long long)max_new, (long long)q_rows);
+  if (starts == nullptr && batch * max_new != q_rows) return fail(ARCQ_E_BAD_SHAPE, "%lld queries for %lld sequences of %lld", (long long)q_rows, (long long)batch, (long long)max_new);
+  if (table_width * cache->page_size > 0x7fffffffLL - 64) return fail(ARCQ_E_TOO_LARGE, "contexts of more than 2^31 tokens");
+  if (batch == 0 || q_rows == 0 || max_new == 0) return ARCQ_OK;
+  if (lengths == nullptr || (page_table == nullptr && table_width > 0) || q_strides == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (const int rc = check_query(q, q_dtype, out, heads, cache->heads, scale)) return rc;
+  if (cache->bits == 16 && q_dtype != cache->dtype) return fail(ARCQ_E_BAD_ARG, "queries must have the type of the pages");
+  if (!strides_ok(q_strides, 2)) return fail(ARCQ_E_ALIGN, "strides of the queries must be multiples of 8 values");
+  arcq::AttendParams p = {};
+  const int row = cache->bits == 16 ? 128 : 8 * cache->bits;
+  for (int i = 0; i < 2; ++i) {
+    arcq::AttendView& a = i ? p.v : p.k;
+    a.rows = static_cast<const uint8_t*>(i ? cache->v_pages : cache->k_pages);
+    a.stats = static_cast<const __half2*>(i ? cache->v_stats : cache->k_stats);
+    a.token_stride = row;
+    a.head_stride = cache->page_size * row;
+    a.block_stride = cache->heads * a.head_stride;
+  }
+  p.codebooks = cache->codebooks;
+  p.table = page_table;
+  p.table_width = static_cast<int>(table_width);
+  p.page_shift = log2_of(cache->page_size);
+  p.pages = static_cast<int>(cache->pages);
+  p.lengths = lengths;
+  p.max_keys = static_cast<int>(table_width * cache->page_size);
+  p.q = q;
+  p.q_token = q_strides[0];
+  p.q_head = q_strides[1];
+  p.q_batch = max_new * q_strides[0];
+  p.q_rows = q_rows;
+  p.starts = starts;
+  p.max_new = static_cast<int>(max_new);
+  p.causal = causal != 0;
+  p.q_bf16 = q_dtype == ARCQ_DT_BF16;
+  p.scale_log2 = scale * 1.44269504088896340736f;
+  p.out = out;
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(cache->heads);
+  p.group = p.heads / p.kv_heads;
+  p.batch = static_cast<int>(batch);
+  return run_attention(p, cache->bits, cache->dtype, static_cast<cudaStream_t>(stream));
+}
+
+int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
+                         int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
+                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* stream) {
+  if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > 0x7fffffffLL - 64)
+    return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld queries=%lld states=%lld", (long long)batch, (long long)queries, (long long)states);
+  if (batch == 0 || queries == 0) return ARCQ_OK;
+  if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || (states > 0 && (k == nullptr || v == nullptr)))
+    return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (const int rc = check_query(q, dtype, out, heads, kv_heads, scale)) return rc;
+  if (lengths != nullptr && mask != nullptr) return fail(ARCQ_E_BAD_ARG, "lengths or a mask, not both");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(ARCQ_E_ALIGN, "keys and values must be 16-byte aligned");
+  if (!strides_ok(q_strides, 3) || !strides_ok(k_strides, 3) || !strides_ok(v_strides, 3)) return fail(ARCQ_E_ALIGN, "strides must be multiples of 8 values");
+  arcq::AttendParams p = {};
+  for (int i = 0; i < 2; ++i) {
+    arcq::AttendView& a = i ? p.v : p.k;
+    const int64_t* const s = i ? v_strides : k_strides;
+    a.rows = static_cast<const uint8_t*>(i ? v : k);
+    a.block_stride = 2 * s[0];
+    a.token_stride = 2 * s[1];
+    a.head_stride = 2 * s[2];
+  }
+  p.lengths = lengths;
+  p.mask = mask;
+  p.mask_stride = mask_stride;
+  p.max_keys = static_cast<int>(states);
+  p.q = q;
+  p.q_batch = q_strides[0];
+  p.q_token = q_strides[1];
+  p.q_head = q_strides[2];
+  p.q_rows = batch * queries;
+  p.max_new = static_cast<int>(queries);
+  p.q_bf16 = dtype == ARCQ_DT_BF16;
+  p.scale_log2 = scale * 1.44269504088896340736f;
+  p.out = out;
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = p.heads / p.kv_heads;
+  p.batch = static_cast<int>(batch);
+  return run_attention(p, 16, dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t load_codes8(const uint8_t* __restrict__ row,
   }
 }
 
-__global__ void unpack_codes_kernel(const uint8_t* __restrict__ packed, long long rows, long long length,
+static __global__ void unpack_codes_kernel(const uint8_t* __restrict__ packed, long long rows, long long length,
                                     long long packed_cols, int bits, uint8_t* __restrict__ out) {
   const long long total = rows * length;
   const unsigned mask = (1u << bits) - 1u;
@@ -52,7 +52,7 @@ __global__ void unpack_codes_kernel(const uint8_t* __restrict__ packed, long lon
 }
 
 // One thread per output byte: gathers the (at most 5) codes that overlap it.
-__global__ void pack_codes_kernel(const uint8_t* __restrict__ codes, long long rows, long long length,
+static __global__ void pack_codes_kernel(const uint8_t* __restrict__ codes, long long rows, long long length,
                                   long long packed_cols, int bits, uint8_t* __restrict__ out) {
   const long long total = rows * packed_cols;
   const unsigned mask = (1u << bits) - 1u;
@@ -73,7 +73,7 @@ __global__ void pack_codes_kernel(const uint8_t* __restrict__ codes, long long r
 
 // out[r, k] = mu + sigma * (cb[c] - codesum/gs); one thread per chunk of 8 codes.  Any group size, any alignment of the output.
 template <int BITS, typename OUT>
-__global__ void dequant_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
+static __global__ void dequant_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
                                const float* __restrict__ sigma, const float* __restrict__ codesum,
                                const float* __restrict__ codebook, long long rows, int K, int gs,
                                OUT* __restrict__ out) {
@@ -105,7 +105,7 @@ __global__ void dequant_kernel(const uint8_t* __restrict__ packed, const float* 
 // number / 8 and nothing is divided.  Two chunks a thread, their loads issued together.  From 4-bit codes to fp16 [12608, 384] 3.6 us, [25216,
 // 3072] 45 us (4.8 TB/s); 11.4 and 170 us when every chunk was found by a 64-bit division and stored a value at a time.
 template <int BITS, typename OUT>
-__global__ void __launch_bounds__(256) dequant64_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
+static __global__ void __launch_bounds__(256) dequant64_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
                                                         const float* __restrict__ sigma, const float* __restrict__ codesum,
                                                         const float* __restrict__ codebook, long long total, OUT* __restrict__ out) {
   pdl_launch_dependents();
@@ -273,13 +273,13 @@ __device__ __forceinline__ void unpack_jobs_block(const UnpackJobs& u) {
 }
 
 // The jobs on their own.
-__global__ void __launch_bounds__(256) unpack_jobs_kernel(const __grid_constant__ UnpackJobs jobs) {
+static __global__ void __launch_bounds__(256) unpack_jobs_kernel(const __grid_constant__ UnpackJobs jobs) {
   pdl_launch_dependents();
   unpack_jobs_block(jobs);
 }
 
 template <int BITS>
-__global__ void unpack_weight_f16_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
+static __global__ void unpack_weight_f16_kernel(const uint8_t* __restrict__ packed, const float* __restrict__ mu,
                                          const float* __restrict__ sigma, const float* __restrict__ codesum,
                                          const float* __restrict__ codebook, long long rows, int K,
                                          __half* __restrict__ out) {

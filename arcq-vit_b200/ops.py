@@ -9,6 +9,7 @@ Bad arguments raise ``RuntimeError`` like the reference's ``TORCH_CHECK``s.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 
 import torch
@@ -290,6 +291,209 @@ def attention(qkv: torch.Tensor, batch: int, tokens: int, heads: int, thresholds
         else:
             _check(lib.arcq_attention_act_quant(q2.data_ptr(), batch, tokens, heads, 64, thresholds.data_ptr(), codebook.data_ptr(), bits,
                                                 group_size, out.data_ptr(), _stream()), "arcq_attention_act_quant")
+    return out
+
+
+# ---------------------------------------------------------------- key/value cache, attention over it and to an encoder's states
+def _no_gradient(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or with detached tensors")
+
+
+def _plain(t, name: str, dtype, device, shape=None) -> torch.Tensor:
+    """A contiguous CUDA tensor as it is: what the call writes, or what is too large to be copied for it."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    return t
+
+
+def _heads_of_64(t, name: str, dims: int, device=None, dtypes=(torch.float16, torch.bfloat16)) -> torch.Tensor:
+    """[..., heads, 64] as the kernels read it: any strides that keep the 64 values together and 16-byte accesses possible; else a copy."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} must be one of {dtypes}, got {t.dtype}")
+    if t.dim() != dims or t.shape[-1] != 64:
+        raise RuntimeError(f"{name} must have {dims} dimensions, the last of 64 values (the head), got {tuple(t.shape)}")
+    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+        t = t.contiguous()
+        t = t.clone() if t.data_ptr() % 16 else t
+    return t
+
+
+def _strides(t: torch.Tensor):
+    n = t.dim() - 1
+    return (ctypes.c_int64 * n)(*t.stride()[:-1])
+
+
+def _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks, device=None):
+    """The C view of a cache, and the tensors that it holds besides the pages."""
+    if not isinstance(k_pages, torch.Tensor) or not k_pages.is_cuda or k_pages.dim() != 4:
+        raise RuntimeError("k_pages must be a CUDA tensor [pages, heads, page_size, row]")
+    device = k_pages.device if device is None else device
+    pages, heads, size, row = k_pages.shape
+    c = _cabi.KvCache(pages=pages, heads=heads, page_size=size)
+    held = None
+    if k_pages.dtype == torch.uint8:
+        if row not in (16, 24, 32):
+            raise RuntimeError(f"a row of packed codes has 16, 24 or 32 bytes (2, 3 or 4 bits for 64 values), got {row}")
+        c.bits = row // 8
+        if k_stats is None or v_stats is None or codebooks is None:
+            raise RuntimeError("pages of packed codes need k_stats, v_stats and codebooks")
+        for t, name in ((k_stats, "k_stats"), (v_stats, "v_stats")):
+            _plain(t, name, torch.float16, device, (pages, heads, size, 2))
+        held = _const(codebooks, "codebooks", torch.float32)
+        if tuple(held.shape) != (2, 2 ** c.bits) or held.device != device:
+            raise RuntimeError(f"codebooks must be [2, {2 ** c.bits}] on {device}, got {tuple(held.shape)} on {held.device}")
+        c.k_stats, c.v_stats, c.codebooks = k_stats.data_ptr(), v_stats.data_ptr(), held.data_ptr()
+    elif k_pages.dtype in (torch.float16, torch.bfloat16) and row == 64:
+        if k_stats is not None or v_stats is not None or codebooks is not None:
+            raise RuntimeError("pages in 16 bits have no statistics and no codebooks")
+        c.bits, c.dtype = 16, _DT[k_pages.dtype]
+    else:
+        raise RuntimeError(f"pages are packed codes (uint8) or 64 values in fp16 or bf16 a row, got {k_pages.dtype} and {row}")
+    _plain(k_pages, "k_pages", None, device)
+    _plain(v_pages, "v_pages", k_pages.dtype, device, k_pages.shape)
+    c.k_pages, c.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    return c, held
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_stats=None,
+                   v_stats=None, thresholds=None, codebooks=None) -> None:
+    """Write keys and values [tokens, heads, 64] of new tokens into a paged cache, quantised on the way where its pages are packed codes.
+
+    A page holds ``page_size`` tokens (a power of two, 16 or more) of every head: ``k_pages`` / ``v_pages`` are [pages, heads, page_size, 64]
+    in fp16 or bf16, or [pages, heads, page_size, 8 * bits] uint8 with bits 2, 3 or 4.  Packed, a head's 64 values are one quantizer
+    group: the codes are those of ``quantize_activation``, and ``k_stats`` / ``v_stats`` [pages, heads, page_size, 2] fp16 hold
+    (mean - scale * code_sum / 64, scale).  ``codebooks`` [2, 2^bits] and ``thresholds`` [2, 2^bits - 1], fp32: the keys' and the values'.
+
+    ``slots`` int64 [tokens]: page * page_size + place in the page.  Tokens with a negative slot, or one beyond the cache, are left out.
+    As with ``index_put_``, of tokens with the same slot any may be found there afterwards, or parts of several."""
+    lib = _cabi.load()
+    k = _heads_of_64(k, "k", 3, None, tuple(_DT))
+    v = _heads_of_64(v, "v", 3, k.device, (k.dtype,))
+    _no_gradient(k, v)
+    c, _held = _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks, k.device)
+    if v.shape != k.shape or k.shape[1] != c.heads:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache of {c.heads} heads")
+    if not isinstance(slots, torch.Tensor) or slots.dim() != 1 or slots.shape[0] != k.shape[0]:
+        raise RuntimeError("slots must be one int64 for each token")
+    slots = _dev(slots, "slots", torch.int64)
+    if slots.device != k.device:
+        raise RuntimeError(f"slots is on {slots.device}, expected {k.device}")
+    th = None
+    if c.bits != 16:
+        th = _const(thresholds, "thresholds", torch.float32)
+        if tuple(th.shape) != (2, 2 ** c.bits - 1) or th.device != k.device:
+            raise RuntimeError(f"thresholds must be [2, {2 ** c.bits - 1}] on {k.device}, got {tuple(th.shape)} on {th.device}")
+    elif c.dtype != _DT[k.dtype]:
+        raise RuntimeError(f"keys and values must have the type of the pages, {k_pages.dtype}, got {k.dtype}")
+    with torch.cuda.device(k.device):
+        _check(lib.arcq_kv_cache_write(ctypes.byref(c), th.data_ptr() if th is not None else None, k.data_ptr(), v.data_ptr(), _DT[k.dtype],
+                                       k.shape[0], _strides(k), _strides(v), slots.data_ptr(), _stream()), "arcq_kv_cache_write")
+
+
+def kv_cache_read(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_stats=None, v_stats=None, codebooks=None,
+                  out_dtype: torch.dtype = torch.float16):
+    """The keys and values in the given slots (see ``kv_cache_write``): two tensors [len(slots), heads, 64], each value rounded once to
+    ``out_dtype``.  Zeros where a slot is negative or beyond the cache."""
+    lib = _cabi.load()
+    c, _held = _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks)
+    if out_dtype not in _DT:
+        raise RuntimeError("out_dtype must be float32, float16 or bfloat16")
+    if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
+        raise RuntimeError("slots must be int64 [tokens]")
+    slots = _dev(slots, "slots", torch.int64)
+    if slots.device != k_pages.device:
+        raise RuntimeError(f"slots is on {slots.device}, expected {k_pages.device}")
+    k, v = (torch.empty((slots.shape[0], c.heads, 64), dtype=out_dtype, device=k_pages.device) for _ in range(2))
+    with torch.cuda.device(k_pages.device):
+        _check(lib.arcq_kv_cache_read(ctypes.byref(c), slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(), _DT[out_dtype], _stream()),
+               "arcq_kv_cache_read")
+    return k, v
+
+
+def _attention_out(out, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _plain(out, "out", q.dtype, q.device, q.shape)
+    if out.data_ptr() % 16:
+        raise RuntimeError("out must be 16-byte aligned")
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    starts=None, max_new: int = 1, k_stats=None, v_stats=None, codebooks=None, causal: bool = True, scale=None, out=None) -> torch.Tensor:
+    """Attention of the newest tokens of each sequence over its cached keys and values, the new tokens' own among them (write them first).
+
+    ``q`` [tokens, heads, 64], fp16 or bf16: the new tokens of all sequences one after the other, sequence b in rows ``starts[b]`` to
+    ``starts[b + 1] - 1`` (int32 [batch + 1]), at most ``max_new`` of them; without ``starts``, ``max_new`` rows each.  ``page_table`` int32
+    [batch, width] and ``lengths`` int32 [batch]: where a sequence's tokens are in the cache (see ``kv_cache_write``) and how many there
+    are.  All three stay on the device: a captured call takes new lengths on every replay.  Causal: the last token of a sequence sees all of
+    it, the one before one less.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
+
+    Returns [tokens, heads, 64] (``out`` where given): zeros for a token that sees nothing.  Rows of no sequence are not written."""
+    lib = _cabi.load()
+    q = _heads_of_64(q, "q", 3)
+    _no_gradient(q)
+    c, _held = _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks, q.device)
+    page_table = _plain(page_table, "page_table", torch.int32, q.device)
+    if page_table.dim() != 2:
+        raise RuntimeError(f"page_table must be [batch, width], got {tuple(page_table.shape)}")
+    batch, width = page_table.shape
+    _plain(lengths, "lengths", torch.int32, q.device, (batch,))
+    if starts is not None:
+        _plain(starts, "starts", torch.int32, q.device, (batch + 1,))
+    if c.bits == 16 and c.dtype != _DT[q.dtype]:
+        raise RuntimeError(f"q must have the type of the pages, {k_pages.dtype}, got {q.dtype}")
+    out = _attention_out(out, q)
+    with torch.cuda.device(q.device):
+        _check(lib.arcq_paged_attention(ctypes.byref(c), q.data_ptr(), _DT[q.dtype], q.shape[0], _strides(q), q.shape[1], batch, page_table.data_ptr(),
+                                        width, lengths.data_ptr(), starts.data_ptr() if starts is not None else None, max_new, int(causal),
+                                        0.125 if scale is None else float(scale), out.data_ptr(), _stream()), "arcq_paged_attention")
+    return out
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths=None, mask=None, scale=None, out=None) -> torch.Tensor:
+    """Attention of ``q`` [batch, queries, heads, 64] to an encoder's states, ``k`` and ``v`` [batch, states, kv_heads, 64], all fp16 or all
+    bf16 (views of a projection's output are read where they are).  ``lengths`` int32 [batch]: the first of the states are seen; or ``mask`` bool
+    [batch, states]: those that are True; or neither.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
+
+    Returns [batch, queries, heads, 64] (``out`` where given): zeros where nothing is seen."""
+    lib = _cabi.load()
+    q = _heads_of_64(q, "q", 4)
+    k, v = (_heads_of_64(t, n, 4, q.device, (q.dtype,)) for t, n in ((k, "k"), (v, "v")))
+    _no_gradient(q, k, v)
+    batch, queries, heads, _ = q.shape
+    if k.shape != v.shape or k.shape[0] != batch:
+        raise RuntimeError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    states, kv_heads = k.shape[1:3]
+    stride = 0
+    if lengths is not None and mask is not None:
+        raise RuntimeError("lengths or a mask, not both")
+    if lengths is not None:
+        _plain(lengths, "lengths", torch.int32, q.device, (batch,))
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or tuple(mask.shape) != (batch, states) or mask.device != q.device:
+            raise RuntimeError(f"mask must be bool [{batch}, {states}] on {q.device}")
+        mask = mask if states <= 1 or mask.stride(1) == 1 else mask.contiguous()
+        stride = mask.stride(0)
+    out = _attention_out(out, q)
+    with torch.cuda.device(q.device):
+        _check(lib.arcq_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[q.dtype], batch, queries, states, heads, kv_heads,
+                                        _strides(q), _strides(k), _strides(v), lengths.data_ptr() if lengths is not None else None,
+                                        mask.data_ptr() if mask is not None else None, stride, 0.125 if scale is None else float(scale),
+                                        out.data_ptr(), _stream()), "arcq_cross_attention")
     return out
 
 

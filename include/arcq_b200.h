@@ -398,6 +398,63 @@ int arcq_dense_weight_gemm_prefetch(const void* xhat, const void* w16, const flo
                                     const float* next_codebook, int next_bits, int next_group_size,
                                     int64_t next_rows, int64_t next_K, void* next_out, void* stream);
 
+/*
+ * A key/value cache in pages, for the decoder beside a packed encoder (captions, text in images, questions about them).  The reference
+ * has no counterpart: its models have no decoder.  Keys and values apart, [pages, heads, page_size, row], heads of 64:
+ *   bits 16      row = 64 values of `dtype` (fp16 or bf16); stats and codebooks are not used
+ *   bits 2, 3, 4 row = 8 * bits bytes: the codes of one quantizer group, as arcq_act_quant packs them, bit for bit;
+ *                stats fp16 [pages, heads, page_size, 2] = (mean - scale * code_sum / 64, scale) rounded to fp16 (and held to its
+ *                range); codebooks fp32 [2, 2^bits], keys' and values'.  A value is stats[0] + stats[1] * codebook[code].
+ * page_size: a power of two, 16 or more.  Buffers contiguous, 16-byte aligned.
+ */
+typedef struct arcq_kv_cache {
+  void *k_pages, *v_pages;
+  void *k_stats, *v_stats;
+  const float* codebooks;
+  int64_t pages, heads, page_size;
+  int bits, dtype;
+} arcq_kv_cache;
+
+/*
+ * Writes `tokens` keys and values [tokens, heads, 64] into the cache, quantised on the way (thresholds fp32 [2, 2^bits - 1]; not used in
+ * 16 bits, where x_dtype is the pages').  strides: of a token and of a head, in values, multiples of 8; the 64 values of a head lie side by side.
+ * slots int64 [tokens]: page * page_size + place; a token whose slot is negative or beyond the cache is left out.  Of two tokens with
+ * the same slot either may be found there afterwards, or parts of both.
+ */
+int arcq_kv_cache_write(const arcq_kv_cache* cache, const float* thresholds, const void* k, const void* v, int x_dtype, int64_t tokens,
+                        const int64_t* k_strides, const int64_t* v_strides, const int64_t* slots, void* stream);
+
+/* Reads tokens back: k_out, v_out [tokens, heads, 64] of out_dtype, each value rounded once; zeros where the slot is negative or beyond
+ * the cache. */
+int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int out_dtype, void* stream);
+
+/*
+ * Attention of the newest tokens of each sequence over its cached keys and values (the new tokens' own among them):
+ *   q     [q_rows, heads, 64] fp16 or bf16 (the pages' type in 16 bits), strides of a token and a head in values, multiples of 8;
+ *         the queries of sequence b are rows starts[b] .. starts[b+1] - 1 (starts int32 [batch + 1]), or, with starts NULL, max_new rows
+ *         each (q_rows = batch * max_new).  max_new bounds the queries of a sequence; what is beyond is left out.
+ *   page_table int32 [batch, table_width]: page of tokens 0 .. page_size - 1 of the sequence, and so on.  Keys on a page that does
+ *         not exist (negative, or not below cache.pages) are not seen.
+ *   lengths int32 [batch]: tokens of the sequence in the cache, at most table_width * page_size
+ *   causal 1: query i of n sees the first lengths[b] - n + i + 1 tokens; 0: all of them
+ *   out   [q_rows, heads, 64] of q's type: softmax(scale q k^T) v, zeros for a query that sees nothing; rows of no sequence stay as they are.
+ * heads is a multiple of cache.heads: query head h reads key head h / (heads / cache.heads).  Packed keys and values are rebuilt in
+ * fp16, one half-precision fma each, so |center| + 3 scale has to stay within fp16's range; products accumulate in fp32, probabilities are rounded
+ * to 16 bits for the second one.  NaN and infinities in keys and values that are not seen have no effect.
+ */
+int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype, int64_t q_rows, const int64_t* q_strides, int64_t heads,
+                         int64_t batch, const int32_t* page_table, int64_t table_width, const int32_t* lengths, const int32_t* starts,
+                         int64_t max_new, int causal, float scale, void* out, void* stream);
+
+/*
+ * Attention of queries [batch, queries, heads, 64] to an encoder's states, keys and values [batch, states, kv_heads, 64], all fp16 or all
+ * bf16; strides of a sequence, a token and a head in values, multiples of 8.  lengths int32 [batch] (the first of the states are seen)
+ * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64]; otherwise as above.
+ */
+int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
+                         int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
+                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -278,6 +278,206 @@ PyObject* dequant(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// ---------------------------------------------------------------- key/value cache and the attentions of a decoder
+bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+// [..., heads, 64] on a CUDA device as the kernels read it, with the strides of the dimensions before the last
+const at::Tensor* heads_tensor(PyObject* o, int dims, int64_t* strides) {
+  const at::Tensor* t = tensor_of(o);
+  if (t == nullptr || !t->is_cuda() || t->dim() != dims || t->size(dims - 1) != 64 || t->stride(dims - 1) != 1 || t->numel() == 0 ||
+      !aligned16(t->const_data_ptr()))
+    return nullptr;
+  for (int i = 0; i + 1 < dims; ++i)
+    if ((strides[i] = t->stride(i)) % 8 != 0) return nullptr;
+  return t;
+}
+const at::Tensor* plain_tensor(PyObject* o, at::ScalarType t, const c10::Device& dev) {
+  const at::Tensor* v = tensor_of(o);
+  return v != nullptr && v->scalar_type() == t && v->device() == dev && v->is_contiguous() ? v : nullptr;
+}
+// args: k_pages, v_pages, k_stats, v_stats, codebooks
+bool read_kv_cache(PyObject* const* args, arcq_kv_cache* c) {
+  const at::Tensor *k = tensor_of(args[0]), *v = tensor_of(args[1]);
+  if (k == nullptr || v == nullptr || !k->is_cuda() || k->dim() != 4 || !k->is_contiguous() || !v->is_contiguous() || v->sizes() != k->sizes() ||
+      v->scalar_type() != k->scalar_type() || v->device() != k->device())
+    return false;
+  c->pages = k->size(0);
+  c->heads = k->size(1);
+  c->page_size = k->size(2);
+  const int64_t row = k->size(3);
+  c->k_pages = k->mutable_data_ptr();
+  c->v_pages = v->mutable_data_ptr();
+  c->dtype = 0;
+  c->k_stats = c->v_stats = nullptr;
+  c->codebooks = nullptr;
+  if (k->scalar_type() != at::kByte) {
+    c->bits = 16;
+    c->dtype = dtype_code(k->scalar_type());
+    return row == 64 && (c->dtype == ARCQ_DT_F16 || c->dtype == ARCQ_DT_BF16) && args[2] == Py_None && args[3] == Py_None && args[4] == Py_None;
+  }
+  if (row != 16 && row != 24 && row != 32) return false;
+  c->bits = static_cast<int>(row / 8);
+  const at::Tensor *ks = plain_tensor(args[2], at::kHalf, k->device()), *vs = plain_tensor(args[3], at::kHalf, k->device()),
+                   *cb = plain_tensor(args[4], at::kFloat, k->device());
+  if (ks == nullptr || vs == nullptr || cb == nullptr || cb->dim() != 2 || cb->size(0) != 2 || cb->size(1) != 1 << c->bits) return false;
+  for (const at::Tensor* t : {ks, vs})
+    if (t->dim() != 4 || t->size(0) != c->pages || t->size(1) != c->heads || t->size(2) != c->page_size || t->size(3) != 2) return false;
+  c->k_stats = ks->mutable_data_ptr();
+  c->v_stats = vs->mutable_data_ptr();
+  c->codebooks = cb->const_data_ptr<float>();
+  return true;
+}
+const at::Tensor* slots_tensor(PyObject* o, const c10::Device& dev) {
+  const at::Tensor* t = plain_tensor(o, at::kLong, dev);
+  return t != nullptr && t->dim() == 1 ? t : nullptr;
+}
+// out: None, or a tensor to write
+bool read_out(PyObject* o, const at::Tensor& q, at::Tensor* out) {
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain_tensor(o, q.scalar_type(), q.device());
+  if (t == nullptr || t->sizes() != q.sizes() || !aligned16(t->const_data_ptr())) return false;
+  *out = *t;
+  return true;
+}
+bool read_scale(PyObject* o, float* scale) {
+  *scale = 0.125f;
+  if (o == Py_None) return true;
+  if (!PyFloat_CheckExact(o)) return false;
+  *scale = static_cast<float>(PyFloat_AS_DOUBLE(o));
+  return true;
+}
+
+// kv_cache_write(k, v, slots, thresholds, k_pages, v_pages, k_stats, v_stats, codebooks) -> True or None
+PyObject* kv_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) Py_RETURN_NONE;
+  int64_t ks[2], vs[2];
+  const at::Tensor *k = heads_tensor(args[0], 3, ks), *v = heads_tensor(args[1], 3, vs);
+  arcq_kv_cache c;
+  if (k == nullptr || v == nullptr || !read_kv_cache(args + 4, &c)) Py_RETURN_NONE;
+  const c10::Device dev = k->device();
+  const at::Tensor *slots = slots_tensor(args[2], dev), *pages = tensor_of(args[4]);
+  const int xt = dtype_code(k->scalar_type());
+  if (slots == nullptr || pages->device() != dev || v->device() != dev || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() ||
+      k->size(1) != c.heads || slots->size(0) != k->size(0) || xt < 0 || (c.bits == 16 && xt != c.dtype) || wants_gradient({k, v}))
+    Py_RETURN_NONE;
+  const at::Tensor* th = nullptr;
+  if (c.bits != 16) {
+    th = plain_tensor(args[3], at::kFloat, dev);
+    if (th == nullptr || th->dim() != 2 || th->size(0) != 2 || th->size(1) != (1 << c.bits) - 1) Py_RETURN_NONE;
+  }
+  without_gil([&] {
+    const c10::cuda::CUDAGuard guard(dev);
+    check(arcq_kv_cache_write(&c, th != nullptr ? th->const_data_ptr<float>() : nullptr, k->const_data_ptr(), v->const_data_ptr(), xt, k->size(0), ks,
+                              vs, slots->const_data_ptr<int64_t>(), c10::cuda::getCurrentCUDAStream().stream()),
+          "arcq_kv_cache_write");
+  });
+  Py_RETURN_TRUE;
+}
+
+// kv_cache_read(slots, k_pages, v_pages, k_stats, v_stats, codebooks, output type code) -> (k, v) or None
+PyObject* kv_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  arcq_kv_cache c;
+  if (n != 7 || !read_kv_cache(args + 1, &c)) Py_RETURN_NONE;
+  const c10::Device dev = tensor_of(args[1])->device();
+  const at::Tensor* slots = slots_tensor(args[0], dev);
+  const long ot = int_of(args[6]);
+  if (slots == nullptr || ot < 0 || ot > 2) Py_RETURN_NONE;
+  const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
+  at::Tensor k, v;
+  without_gil([&] {
+    const c10::cuda::CUDAGuard guard(dev);
+    k = empty_cuda({slots->size(0), c.heads, 64}, types[ot], dev);
+    v = empty_cuda({slots->size(0), c.heads, 64}, types[ot], dev);
+    check(arcq_kv_cache_read(&c, slots->const_data_ptr<int64_t>(), slots->size(0), k.mutable_data_ptr(), v.mutable_data_ptr(), static_cast<int>(ot),
+                             c10::cuda::getCurrentCUDAStream().stream()),
+          "arcq_kv_cache_read");
+  });
+  PyObject* out = PyTuple_New(2);
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(v)));
+  return out;
+}
+
+// paged_attention(q, page_table, lengths, starts, max_new, causal, scale, out, k_pages, v_pages, k_stats, v_stats, codebooks) -> out or None
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 13 || !all_bools(args, {5})) Py_RETURN_NONE;
+  int64_t qs[2];
+  const at::Tensor* q = heads_tensor(args[0], 3, qs);
+  arcq_kv_cache c;
+  if (q == nullptr || !read_kv_cache(args + 8, &c)) Py_RETURN_NONE;
+  const c10::Device dev = q->device();
+  const at::Tensor *table = plain_tensor(args[1], at::kInt, dev), *lengths = plain_tensor(args[2], at::kInt, dev), *starts = nullptr;
+  const long max_new = int_of(args[4]);
+  const int qt = dtype_code(q->scalar_type());
+  float scale;
+  at::Tensor out;
+  if (table == nullptr || lengths == nullptr || table->dim() != 2 || lengths->dim() != 1 || lengths->size(0) != table->size(0) || max_new < 0 ||
+      (qt != ARCQ_DT_F16 && qt != ARCQ_DT_BF16) || (c.bits == 16 && qt != c.dtype) || tensor_of(args[8])->device() != dev || wants_gradient({q}) ||
+      !read_scale(args[6], &scale) || !read_out(args[7], *q, &out))
+    Py_RETURN_NONE;
+  if (args[3] != Py_None) {
+    starts = plain_tensor(args[3], at::kInt, dev);
+    if (starts == nullptr || starts->dim() != 1 || starts->size(0) != table->size(0) + 1) Py_RETURN_NONE;
+  }
+  without_gil([&] {
+    const c10::cuda::CUDAGuard guard(dev);
+    if (!out.defined()) out = empty_cuda(q->sizes(), q->scalar_type(), dev);
+    check(arcq_paged_attention(&c, q->const_data_ptr(), qt, q->size(0), qs, q->size(1), table->size(0), table->const_data_ptr<int>(), table->size(1),
+                               lengths->const_data_ptr<int>(), starts != nullptr ? starts->const_data_ptr<int>() : nullptr, max_new,
+                               args[5] == Py_True, scale, out.mutable_data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
+          "arcq_paged_attention");
+  });
+  if (args[7] != Py_None) {
+    Py_INCREF(args[7]);
+    return args[7];
+  }
+  return THPVariable_Wrap(std::move(out));
+}
+
+// cross_attention(q, k, v, lengths, mask, scale, out) -> out or None
+PyObject* cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  int64_t qs[3], ks[3], vs[3];
+  const at::Tensor *q = heads_tensor(args[0], 4, qs), *k = heads_tensor(args[1], 4, ks), *v = heads_tensor(args[2], 4, vs);
+  if (q == nullptr || k == nullptr || v == nullptr) Py_RETURN_NONE;
+  const c10::Device dev = q->device();
+  const int qt = dtype_code(q->scalar_type());
+  for (const at::Tensor* t : {k, v})
+    if (t->device() != dev || t->scalar_type() != q->scalar_type() || t->sizes() != k->sizes() || t->size(0) != q->size(0)) Py_RETURN_NONE;
+  float scale;
+  at::Tensor out;
+  if ((qt != ARCQ_DT_F16 && qt != ARCQ_DT_BF16) || wants_gradient({q, k, v}) || !read_scale(args[5], &scale) || !read_out(args[6], *q, &out)) Py_RETURN_NONE;
+  const at::Tensor *lengths = nullptr, *mask = nullptr;
+  if (args[3] != Py_None) {
+    lengths = plain_tensor(args[3], at::kInt, dev);
+    if (lengths == nullptr || args[4] != Py_None || lengths->dim() != 1 || lengths->size(0) != q->size(0)) Py_RETURN_NONE;
+  }
+  if (args[4] != Py_None) {
+    mask = tensor_of(args[4]);
+    if (mask == nullptr || mask->scalar_type() != at::kBool || mask->device() != dev || mask->dim() != 2 || mask->size(0) != q->size(0) ||
+        mask->size(1) != k->size(1) || mask->stride(1) != 1)
+      Py_RETURN_NONE;
+  }
+  without_gil([&] {
+    const c10::cuda::CUDAGuard guard(dev);
+    if (!out.defined()) out = empty_cuda(q->sizes(), q->scalar_type(), dev);
+    check(arcq_cross_attention(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), qt, q->size(0), q->size(1), k->size(1), q->size(2),
+                               k->size(2), qs, ks, vs, lengths != nullptr ? lengths->const_data_ptr<int>() : nullptr,
+                               mask != nullptr ? static_cast<const uint8_t*>(mask->const_data_ptr()) : nullptr,
+                               mask != nullptr ? mask->stride(0) : 0, scale, out.mutable_data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
+          "arcq_cross_attention");
+  });
+  if (args[6] != Py_None) {
+    Py_INCREF(args[6]);
+    return args[6];
+  }
+  return THPVariable_Wrap(std::move(out));
+}
+
 // ---------------------------------------------------------------- the library's attention
 // Whether nothing was chosen about it: all back ends allowed, in the order that the framework settles on.  It does so when it is first
 // asked for a back end, whatever the order was until then; after that, the order that it starts with is a choice like any other.  So
@@ -613,7 +813,8 @@ PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   }
 }
 #define ARCQ_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<f>)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {ARCQ_METHOD(linear), ARCQ_METHOD(quantize_activation), ARCQ_METHOD(dequant), ARCQ_METHOD(vit_plan),
+PyMethodDef g_methods[] = {ARCQ_METHOD(linear), ARCQ_METHOD(quantize_activation), ARCQ_METHOD(dequant), ARCQ_METHOD(kv_cache_write),
+                           ARCQ_METHOD(kv_cache_read), ARCQ_METHOD(paged_attention), ARCQ_METHOD(cross_attention), ARCQ_METHOD(vit_plan),
                            ARCQ_METHOD(vit_forward), ARCQ_METHOD(attention_back_ends_as_they_come), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_arcq_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

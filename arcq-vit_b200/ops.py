@@ -379,6 +379,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_page
 
     ``slots`` int64 [tokens]: page * page_size + place in the page.  Tokens with a negative slot, or one beyond the cache, are left out.
     As with ``index_put_``, of tokens with the same slot any may be found there afterwards, or parts of several."""
+    if _cabi.host().kv_cache_write(k, v, slots, thresholds, k_pages, v_pages, k_stats, v_stats, codebooks):
+        return
     lib = _cabi.load()
     k = _heads_of_64(k, "k", 3, None, tuple(_DT))
     v = _heads_of_64(v, "v", 3, k.device, (k.dtype,))
@@ -407,6 +409,9 @@ def kv_cache_read(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
                   out_dtype: torch.dtype = torch.float16):
     """The keys and values in the given slots (see ``kv_cache_write``): two tensors [len(slots), heads, 64], each value rounded once to
     ``out_dtype``.  Zeros where a slot is negative or beyond the cache."""
+    got = _cabi.host().kv_cache_read(slots, k_pages, v_pages, k_stats, v_stats, codebooks, _DT.get(out_dtype))
+    if got is not None:
+        return got
     lib = _cabi.load()
     c, _held = _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks)
     if out_dtype not in _DT:
@@ -443,6 +448,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     it, the one before one less.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
 
     Returns [tokens, heads, 64] (``out`` where given): zeros for a token that sees nothing.  Rows of no sequence are not written."""
+    got = _cabi.host().paged_attention(q, page_table, lengths, starts, max_new, causal, scale, out, k_pages, v_pages, k_stats, v_stats, codebooks)
+    if got is not None:
+        return got
     lib = _cabi.load()
     q = _heads_of_64(q, "q", 3)
     _no_gradient(q)
@@ -470,6 +478,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths=N
     [batch, states]: those that are True; or neither.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
 
     Returns [batch, queries, heads, 64] (``out`` where given): zeros where nothing is seen."""
+    got = _cabi.host().cross_attention(q, k, v, lengths, mask, scale, out)
+    if got is not None:
+        return got
     lib = _cabi.load()
     q = _heads_of_64(q, "q", 4)
     k, v = (_heads_of_64(t, n, 4, q.device, (q.dtype,)) for t, n in ((k, "k"), (v, "v")))

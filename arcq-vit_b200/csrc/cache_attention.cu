@@ -11,6 +11,7 @@
 #include "launch.h"
 #include "kv_cache.cuh"
 #include "split_attention.cuh"
+#include "tile_attention.cuh"
 
 namespace {
 
@@ -139,12 +140,57 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, cudaStre
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 
+// Blocks of a row tile, 1 to 8: the cluster size for which the rounds of blocks over the SMs take the fewest tiles of keys, a block's set-up and
+// the joining of results counted as tiles.
+template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStream_t st) {
+  auto k = arcq::tile_attention_kernel<BITS, E>;
+  constexpr size_t smem = arcq::tile_smem_layout(BITS != 16).total;
+  static thread_local int done_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (done_dev != dev) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaFuncAttributes a = {};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, k);
+    if (e != cudaSuccess) return arcq_host::cuda_fail(e, "attention set-up");
+    const int got = arcq_host::launch_regs() > 0 ? arcq_host::launch_regs() : a.numRegs;
+    if (got < arcq::kTileLaunchRegs)             // the warp groups' hand-over would wait for good
+      return fail(ARCQ_E_CUDA, "attention: compiled for %d registers a thread, its warp groups share out %d", got, arcq::kTileLaunchRegs);
+    done_dev = dev;
+  }
+  const long long all_rows = static_cast<long long>(p.max_new) * p.group;
+  p.tiles = static_cast<int>((all_rows + 2 * arcq::kTileRows - 1) / (2 * arcq::kTileRows));
+  const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.tiles;
+  const double key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys, each = all_rows > arcq::kTileRows ? 1.0 : 0.5;
+  int splits = 1;
+  double best = 1e30;
+  for (int s = 1; s <= 8 && (s == 1 || s <= key_tiles); ++s) {
+    const int room = arcq_host::sm_count() / s - (s > 2 ? 2 : 0);             // clusters at a time: some SMs of a group are left over
+    const double rounds = ceil(static_cast<double>(units) / (room > 0 ? room : 1));
+    const double cost = rounds * (ceil(key_tiles / s) * each + 3.0 + (s > 1 ? 1.0 : 0.0));
+    if (cost < best) {
+      best = cost;
+      splits = s;
+    }
+  }
+  p.splits = splits;
+  p.poll_limit = arcq_host::poll_limit();
+  p.status = arcq_host::status_ptr();
+  if (units * splits > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
+  const cudaError_t e = launch(k, dim3(static_cast<unsigned>(units * splits)), arcq::kTileThreads, smem, splits, st, p);
+  return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
+}
+
+template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, cudaStream_t st) {
+  return static_cast<long long>(p.max_new) * p.group > 2 * arcq::kSplitRows ? launch_tile<BITS, E>(p, st) : launch_split<BITS, E>(p, st);
+}
+
 int run_attention(arcq::AttendParams& p, int bits, int dtype, cudaStream_t st) {
   switch (bits) {
-    case 4: return launch_split<4, __half>(p, st);
-    case 3: return launch_split<3, __half>(p, st);
-    case 2: return launch_split<2, __half>(p, st);
-    default: return dtype == ARCQ_DT_BF16 ? launch_split<16, __nv_bfloat16>(p, st) : launch_split<16, __half>(p, st);
+    case 4: return launch_attention<4, __half>(p, st);
+    case 3: return launch_attention<3, __half>(p, st);
+    case 2: return launch_attention<2, __half>(p, st);
+    default: return dtype == ARCQ_DT_BF16 ? launch_attention<16, __nv_bfloat16>(p, st) : launch_attention<16, __half>(p, st);
   }
 }
 

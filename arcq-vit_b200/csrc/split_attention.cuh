@@ -17,6 +17,7 @@
 #include <stdint.h>
 #include "ptx.cuh"
 #include "f32x2.cuh"
+#include "attention.cuh"
 #include "kv_cache.cuh"
 
 namespace arcq {
@@ -45,6 +46,8 @@ struct AttendParams {
   float scale_log2;                     // scale / ln 2
   void* out;                            // [tokens, heads, 64]
   int heads, kv_heads, group, tiles, splits, batch;
+  uint32_t poll_limit;                  // tile_attention.cuh
+  int* status;
 };
 
 // What a block has to know of its sequence
@@ -87,10 +90,25 @@ __device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t b, uint32_t c
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float d;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
-  return d;
+// A row of bf16 queries (or a lane's part of it, with `top` the whole row's largest magnitude) as fp16: times the power of two that brings
+// the largest value to 2^13..2^14, so that fp16 holds all that counts exactly.  Returns the factor that undoes it.
+__device__ __forceinline__ float bf16_top(const uint32_t* w, int n) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < n; ++j) {
+    float x, y;
+    unpack2(sixteen_to_pair<__nv_bfloat16>(w[j]), x, y);
+    top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+  }
+  return top;
+}
+__device__ __forceinline__ float bf16_to_half(uint32_t* w, int n, float top) {
+  const int e = (__float_as_int(top) >> 23) - 127;
+  const int up = top > 0.0f && e < 128 ? min(max(13 - e, -100), 100) : 0;
+  const float f = __int_as_float((up + 127) << 23);
+#pragma unroll
+  for (int j = 0; j < n; ++j) w[j] = pair_to_sixteen<__half>(mul2(sixteen_to_pair<__nv_bfloat16>(w[j]), pack2(f, f)));
+  return __int_as_float((127 - up) << 23);
 }
 
 constexpr int kSplitWarps = 8, kSplitThreads = kSplitWarps * 32, kSplitRows = 16;
@@ -112,6 +130,27 @@ __device__ __forceinline__ void pair_levels(uint32_t table, uint32_t w, uint32_t
   pairs[1] = lds_const_u32(table + ((w >> 1) & 0x7F80u));
   pairs[2] = lds_const_u32(table + ((w >> 9) & 0x7F80u));
   pairs[3] = lds_const_u32(table + ((w >> 17) & 0x7F80u));
+}
+
+// The same in fp32, for values: [byte][lane & 15], `table` with the lane's column.  Rounded to fp16 a level is off by the same amount in every
+// key that has its code, which adds up over a long context; one rounding of center + scale * level does not.
+__device__ __forceinline__ void fill_pair_table_f32(uint32_t table, const float* levels, int count, int tid, int threads) {
+  for (int i = tid; i < 256 * 8; i += threads) {
+    const int byte = i >> 3;
+    const uint32_t lo = __float_as_uint(__ldg(levels + min(byte & 15, count - 1))), hi = __float_as_uint(__ldg(levels + min(byte >> 4, count - 1)));
+    sts128(table + byte * 128 + (i & 7) * 16, lo, hi, lo, hi);
+  }
+}
+__device__ __forceinline__ f32x2 lds_const_pair(uint32_t addr) {
+  f32x2 v;
+  asm("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void pair_levels_f32(uint32_t table, uint32_t w, f32x2 (&pairs)[4]) {
+  pairs[0] = lds_const_pair(table + ((w << 7) & 0x7F80u));
+  pairs[1] = lds_const_pair(table + ((w >> 1) & 0x7F80u));
+  pairs[2] = lds_const_pair(table + ((w >> 9) & 0x7F80u));
+  pairs[3] = lds_const_pair(table + ((w >> 17) & 0x7F80u));
 }
 
 // The rows of one block of keys that a lane holds.  Lane 4g + c: of keys 8n + g the 16 values from 16c, of values 2c, 2c + 1 (+ 8 n) the 8 from 8g.
@@ -136,10 +175,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
   const int tile = unit % p.tiles, kvh = unit / p.tiles % p.kv_heads, b = unit / p.tiles / p.kv_heads;
-  const uint32_t k_table = smem_u32(smem) + lane * 4, v_table = k_table + kPairTableBytes;
+  const uint32_t k_table = smem_u32(smem) + lane * 4, v_table = smem_u32(smem) + kPairTableBytes + (lane & 15) * 8;
   if constexpr (PACKED) {
     fill_pair_table(smem_u32(smem), p.codebooks, 1 << BITS, tid, kSplitThreads);
-    fill_pair_table(smem_u32(smem) + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, tid, kSplitThreads);
+    fill_pair_table_f32(smem_u32(smem) + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, tid, kSplitThreads);
   }
   pdl_wait();
   __syncthreads();
@@ -171,24 +210,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
       w[0] = u0.x; w[1] = u0.y; w[2] = u0.z; w[3] = u0.w; w[4] = u1.x; w[5] = u1.y; w[6] = u1.z; w[7] = u1.w;
     }
     if (PACKED && p.q_bf16) {
-      float top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float x, y;
-        unpack2(sixteen_to_pair<__nv_bfloat16>(w[j]), x, y);
-        top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
-      }
+      float top = bf16_top(w, 8);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (__float_as_int(top) >> 23) - 127;
-      const int up = top > 0.0f && e < 128 ? min(max(13 - e, -100), 100) : 0;
-      const float f = __int_as_float((up + 127) << 23);
-      row_scale[h] *= __int_as_float((127 - up) << 23);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const f32x2 x = mul2(sixteen_to_pair<__nv_bfloat16>(w[j]), pack2(f, f));
-        w[j] = pair_to_sixteen<__half>(x);
-      }
+      row_scale[h] *= bf16_to_half(w, 8, top);
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -331,7 +356,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
     if (__any_sync(0xffffffffu, m[0] > top[0] || m[1] > top[1])) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float f = m[h] == ninf ? 1.0f : exp2_fast(top[h] - m[h]);
+        const float f = m[h] == ninf ? 1.0f : exp2_approx(top[h] - m[h]);
         top[h] = m[h];
         sum[h] *= f;
 #pragma unroll
@@ -347,7 +372,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float x = exp2_fast(fmaf(s[n][2 * h], row_scale[h], nm[h])), y = exp2_fast(fmaf(s[n][2 * h + 1], row_scale[h], nm[h]));
+        const float x = exp2_approx(fmaf(s[n][2 * h], row_scale[h], nm[h])), y = exp2_approx(fmaf(s[n][2 * h + 1], row_scale[h], nm[h]));
         sum[h] += x + y;
         pa[n][h] = pair_to_sixteen<E>(pack2(x, y));            // probabilities of at most 1, rounded for the second product
       }
@@ -360,15 +385,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
         const int n = 2 * u + e;
         if constexpr (PACKED) {
           const uint32_t w0 = spread_codes<BITS>(blk.v[n][0]), w1 = spread_codes<BITS>(blk.v[n][1]);
-          uint32_t even[4], odd[4];
-          pair_levels(v_table, (w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), even);
-          pair_levels(v_table, ((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), odd);
-          const uint32_t center = __byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x5410);
-          const uint32_t scale = __byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x7632);
+          f32x2 even[4], odd[4];
+          pair_levels_f32(v_table, (w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), even);
+          pair_levels_f32(v_table, ((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), odd);
+          const f32x2 center = sixteen_to_pair<__half>(__byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x5410));
+          const f32x2 scale = sixteen_to_pair<__half>(__byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x7632));
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            vb[e][2 * j] = half2_fma(scale, even[j], center);
-            vb[e][2 * j + 1] = half2_fma(scale, odd[j], center);
+            vb[e][2 * j] = pair_to_sixteen<__half>(fma2(scale, even[j], center));
+            vb[e][2 * j + 1] = pair_to_sixteen<__half>(fma2(scale, odd[j], center));
           }
         } else {
           const uint4 a = blk.v[n][0], d = blk.v[n][1];
@@ -422,8 +447,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
     whole_max[h] = m;
     const float base = m == ninf ? 0.0f : m;
 #pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) whole_sum[h] += s_sum[w][g + 8 * h] * exp2_fast(s_max[w][g + 8 * h] - base);
-    const float f = exp2_fast(top[h] - base);
+    for (int w = 0; w < kSplitWarps; ++w) whole_sum[h] += s_sum[w][g + 8 * h] * exp2_approx(s_max[w][g + 8 * h] - base);
+    const float f = exp2_approx(top[h] - base);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float4* const dst = reinterpret_cast<float4*>(s_out + (warp * kSplitRows + g + 8 * h) * 64 + 16 * c + 8 * j);
@@ -467,7 +492,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const
       const float base = m == ninf ? 0.0f : m;
       x = l = 0.0f;
       for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2_fast(remote(smem_u32(s_block_max + r), s) - base);
+        const float f = exp2_approx(remote(smem_u32(s_block_max + r), s) - base);
         l += f * remote(smem_u32(s_block_sum + r), s);
         x += f * remote(smem_u32(s_out + i), s);
       }

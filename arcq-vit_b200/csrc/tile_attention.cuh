@@ -1,0 +1,552 @@
+// Attention of many queries a key head on the fifth-generation tensor cores: pieces of prompts over a cache, texts over an encoder's states.
+// Same operator as split_attention.cuh; keys and values are staged in shared memory (packed ones rebuilt in fp16 there, once a block).
+//
+// A block takes up to 256 rows, (query, head) pairs that share a key head, in two streams of 128 with scores and output of their own in tensor
+// memory, a softmax thread a row:
+//   more than 128 rows   the streams are the two halves of the rows; both use every tile of 128 keys
+//   up to 128 rows       both streams have the same rows, one takes the even tiles of keys, the other the odd ones
+// so that one stream's exponentials run while the other's products do.  The keys of a row tile are also split over the blocks of a
+// cluster where there are too few row tiles for the SMs.  Partial results are joined in shared memory of the cluster, in a fixed order.
+//
+// Running maximum: a row's exponents are taken against a maximum that is renewed only when a score passes it by 2^8 (then the output in
+// tensor memory is scaled): probabilities reach 256 instead of 1 at most, and sums and products are as exact either way.
+//
+// Warps: 0-3 softmax of stream 0, 4-7 of stream 1 (a tensor-memory lane quarter each), 8-11 keys and values, 12 and 13 products of the
+// streams; 14 and 15 only keep step (registers are handed over by groups of four warps).
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_bf16.h>
+#include <stdint.h>
+#include "ptx.cuh"
+#include "f32x2.cuh"
+#include "attention.cuh"
+#include "split_attention.cuh"
+
+namespace arcq {
+
+constexpr int kStatusTileAttentionTimeout = 0x502;
+constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128, kTileSlots = 3;
+constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 192, kTileLoadRegs = 88, kTileIssueRegs = 40;
+static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
+constexpr uint32_t kTileBytes = 128 * 128;                        // 128 rows of 64 16-bit values
+constexpr uint32_t kTileTmemCols = 512;
+// tensor memory of stream t: scores, probabilities (pairs), output
+__host__ __device__ constexpr uint32_t tile_s_col(int t) { return 128u * t; }
+__host__ __device__ constexpr uint32_t tile_p_col(int t) { return 256u + 64u * t; }
+__host__ __device__ constexpr uint32_t tile_o_col(int t) { return 384u + 64u * t; }
+
+struct TileSmem {
+  uint32_t q, k, v, tables, seen, max, sum, bars, total;
+};
+__host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
+  TileSmem s = {};
+  s.q = 0;
+  s.k = s.q + 2 * kTileBytes;
+  s.v = s.k + kTileSlots * kTileBytes;
+  s.tables = s.v + kTileSlots * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
+  s.seen = s.tables + (packed ? 2 * kPairTableBytes : 0);
+  s.max = s.seen + kTileSlots * 16;
+  s.sum = s.max + 2 * kTileRows * 4;
+  s.bars = s.sum + 2 * kTileRows * 4;
+  s.total = s.bars + 32 * 8 + 1024;                               // and alignment
+  return s;
+}
+
+template <typename E> __device__ __forceinline__ uint32_t tile_idesc(int M, int N) {
+  return umma_idesc_f16(M, N) | (sizeof(E) == 2 && std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool is) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 "
+      "[%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ float lds_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 lds128_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int BITS, typename E>
+__global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const __grid_constant__ AttendParams p) {
+  constexpr bool PACKED = BITS != 16;
+  extern __shared__ uint8_t tile_smem_raw[];
+  uint8_t* const smem = tile_smem_raw + ((1024u - (smem_u32(tile_smem_raw) & 1023u)) & 1023u);
+  constexpr TileSmem L = tile_smem_layout(PACKED);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L.bars);
+  uint64_t *const k_full = bars, *const k_free = bars + 3, *const v_full = bars + 6, *const v_free = bars + 9;     // [slot]
+  uint64_t *const q_full = bars + 12, *const s_full = bars + 14, *const s_read = bars + 16, *const p_full = bars + 18, *const o_done = bars + 20;   // [stream]
+  uint64_t* const stopped = bars + 22;
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 24);
+  uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [slot][warp]
+  float* const s_max = reinterpret_cast<float*>(smem + L.max);                    // [stream][row]
+  float* const s_sum = reinterpret_cast<float*>(smem + L.sum);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t polls = p.poll_limit;
+
+  const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
+  const int tile = p.tiles - 1 - unit / (p.kv_heads * p.batch);                   // long rows of causal keys first
+  const int kvh = unit % p.kv_heads, b = unit / p.kv_heads % p.batch;
+
+  if constexpr (PACKED) {
+    fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, tid, kTileThreads);
+    fill_pair_table_f32(smem_u32(smem) + L.tables + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, tid, kTileThreads);
+  }
+  pdl_wait();
+  const AttendSequence seq = attend_sequence(p, b);
+  const int all_rows = seq.queries * p.group;
+  const bool halves = all_rows > kTileRows;                                       // the streams are halves of the rows
+  const int row0 = tile * 2 * kTileRows, rows = min(all_rows - row0, 2 * kTileRows);
+  // Tiles of rows that are not there: the whole cluster leaves.
+  if (rows <= 0) {
+    pdl_launch_dependents();
+    return;
+  }
+  if (tid == 0) {
+    const int users = halves ? 2 : 1;                                             // streams that read a tile of keys
+    for (int i = 0; i < kTileSlots; ++i) {
+      mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
+      mbar_init(k_free + i, users); mbar_init(v_free + i, users);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full + t, 4); mbar_init(s_read + t, 4); mbar_init(p_full + t, 4);
+      mbar_init(s_full + t, 1); mbar_init(o_done + t, 1);
+    }
+    mbar_init(stopped, 2);
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(s_tmem, kTileTmemCols);
+    tmem_relinquish();
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  tc_fence_after_sync();
+  const uint32_t tmem = *s_tmem;
+  // keys that the last row sees, the block's share of their tiles
+  int keys = seq.keys;
+  if (p.causal) keys = min(keys, max(seq.keys - seq.all_queries + (row0 + rows - 1) / p.group + 1, 0));
+  const int all_tiles = (keys + kTileKeys - 1) / kTileKeys, per = (all_tiles + p.splits - 1) / p.splits;
+  const int first = min(split * per, all_tiles), count = min(first + per, all_tiles) - first;
+  // tile j of the block is tile i of stream t: halves: j = i for both; else j = 2 i + t
+  bool ok = true;
+
+  if (warp >= 12) {
+    // ------------------------------------------------------------------ products: warps 12 and 13, a stream each
+    fewer_registers<kTileIssueRegs>();
+    const int t = warp - 12;
+    const int mine = t > 1 ? 0 : halves ? count : (count + 1 - t) / 2;
+    if (t < 2 && mine > 0) {
+      const uint32_t idesc_s = tile_idesc<E>(kTileRows, kTileKeys);
+      const uint32_t idesc_o = tile_idesc<E>(kTileRows, 64) | (1u << 16);         // B with its rows (keys) along K
+      auto desc_lo = [&](uint32_t off) { return ((smem_u32(smem + off) & 0x3FFFFu) >> 4) | (1u << 16); };
+      const uint32_t q = desc_lo(L.q + (halves ? t : 0) * kTileBytes), k0 = desc_lo(L.k), v0 = desc_lo(L.v);
+      auto at = [&](int i) { return halves ? i : 2 * i + t; };
+      for (int i = 0; i <= mine; ++i) {
+        if (i < mine) {
+          const int j = at(i), slot = j % kTileSlots;
+          ok = ok && (i > 0 || mbar_wait(q_full + (halves ? t : 0), 0, polls)) && mbar_wait(k_full + slot, (j / kTileSlots) & 1, polls) &&
+               (i == 0 || mbar_wait(s_read + t, (i - 1) & 1, polls));
+          tc_fence_after_sync();
+          if (elect_one() && ok) {
+            umma_f16_x4(tmem + tile_s_col(t), q, k0 + slot * (kTileBytes >> 4), idesc_s);
+            umma_commit(s_full + t);
+            umma_commit(k_free + slot);
+          }
+          __syncwarp();
+        }
+        if (i > 0) {
+          const int j = at(i - 1), slot = j % kTileSlots;
+          ok = ok && mbar_wait(v_full + slot, (j / kTileSlots) & 1, polls) && mbar_wait(p_full + t, (i - 1) & 1, polls);
+          tc_fence_after_sync();
+          if (elect_one() && ok) {
+#pragma unroll
+            for (int k = 0; k < kTileKeys; k += 16)
+              umma_f16_tmem_a_lo(tmem + tile_o_col(t), tmem + tile_p_col(t) + (k >> 1), v0 + slot * (kTileBytes >> 4) + 8 * k, idesc_o,
+                                 i > 1 || k > 0 ? 1u : 0u);
+            umma_commit(o_done + t);
+            umma_commit(v_free + slot);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------------ keys and values: a warp 32 keys of a tile
+    fewer_registers<kTileLoadRegs>();
+    const int w = warp - 8;
+    const uint32_t k_smem = smem_u32(smem) + L.k + w * 4096, v_smem = smem_u32(smem) + L.v + w * 4096;
+    // where the two sixteens of keys of the warp lie (in one page each), and which keys are seen
+    struct Place {
+      long long k[2], v[2], st[2];
+      uint32_t seen;
+    };
+    auto place = [&](int j) {
+      Place pl;
+      const int base = (first + j) * kTileKeys + 32 * w;
+      bool there[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = base + 16 * u;
+        int block = b, in = key;
+        there[u] = key < keys;
+        if (p.table != nullptr && there[u]) {
+          block = p.table[static_cast<long long>(b) * p.table_width + (key >> p.page_shift)];
+          in = key & ((1 << p.page_shift) - 1);
+          there[u] = block >= 0 && block < p.pages;
+        }
+        pl.k[u] = block * p.k.block_stride + kvh * p.k.head_stride + in * p.k.token_stride;
+        pl.v[u] = block * p.v.block_stride + kvh * p.v.head_stride + in * p.v.token_stride;
+        pl.st[u] = PACKED ? ((static_cast<long long>(block) * p.kv_heads + kvh) << p.page_shift) + in : 0;
+      }
+      bool is = base + lane < keys && (lane < 16 ? there[0] : there[1]);
+      if (is && p.mask != nullptr) is = p.mask[b * p.mask_stride + base + lane] != 0;
+      pl.seen = __ballot_sync(0xffffffffu, is);
+      return pl;
+    };
+    auto free_slot = [&](uint64_t* bar, int j) {
+      if (j >= kTileSlots) ok = mbar_wait(bar + j % kTileSlots, (j / kTileSlots - 1) & 1, polls) && ok;
+    };
+    if constexpr (!PACKED) {
+      // 16 bits: eight lanes a row, asynchronous copies.  A tile is handed over before a slot is waited for: the slot may be freed by a product
+      // that is issued behind one with that tile.
+      auto copy = [&](const AttendView& a, const long long (&at)[2], uint32_t seen, uint32_t dst) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = 4 * r + (lane >> 3), c = lane & 7;
+          const bool is = (seen >> row) & 1;
+          cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), a.rows + (is ? at[r >> 2] + (row & 15) * a.token_stride + 16 * c : 0), is);
+        }
+        cp_async_commit();
+      };
+      auto hand_over = [&](uint64_t* bar) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      };
+      for (int j = 0; j < count; ++j) {
+        const Place pl = place(j);
+        const int slot = j % kTileSlots, before = (j + kTileSlots - 1) % kTileSlots;
+        if (j > 0) {
+          cp_async_wait<1>();
+          hand_over(k_full + before);
+        }
+        free_slot(k_free, j);
+        copy(p.k, pl.k, pl.seen, k_smem + slot * kTileBytes);
+        if (j > 0) {
+          cp_async_wait<1>();
+          hand_over(v_full + before);
+        }
+        free_slot(v_free, j);
+        copy(p.v, pl.v, pl.seen, v_smem + slot * kTileBytes);
+        if (lane == 0) s_seen[slot * 4 + w] = pl.seen;
+      }
+      if (count > 0) {
+        cp_async_wait<1>();
+        hand_over(k_full + (count - 1) % kTileSlots);
+        cp_async_wait<0>();
+        hand_over(v_full + (count - 1) % kTileSlots);
+      }
+    } else {
+      // packed: a lane has a key's row, eight values of it at a time
+      const uint32_t k_table = smem_u32(smem) + L.tables + lane * 4, v_table = smem_u32(smem) + L.tables + kPairTableBytes + (lane & 15) * 8;
+      const uint32_t row = lane * 128, x7 = lane & 7;
+      struct Row {
+        uint32_t w[2 * BITS], stats;
+      };
+      auto load_row = [&](const AttendView& a, long long at, long long st, bool is, Row& r) {
+        const uint32_t* const src = reinterpret_cast<const uint32_t*>(a.rows + at);
+#pragma unroll
+        for (int i = 0; i < 2 * BITS; i += 2) {
+          const uint2 u = is ? *reinterpret_cast<const uint2*>(src + i) : make_uint2(0, 0);
+          r.w[i] = u.x; r.w[i + 1] = u.y;
+        }
+        r.stats = is ? *reinterpret_cast<const uint32_t*>(a.stats + st) : 0;
+      };
+      // the codes of values 8c .. 8c + 7, one per nibble
+      auto codes = [](const Row& r, int c) {
+        if (BITS == 4) return r.w[c];
+        if (BITS == 2) return spread_codes<2>((c & 1) ? r.w[c >> 1] >> 16 : r.w[c >> 1] & 0xFFFFu);
+        const uint32_t* const w = r.w + 3 * (c >> 2);                             // 24 bits each, four of them in three words
+        switch (c & 3) {
+          case 0: return spread_codes<3>(w[0] & 0xFFFFFFu);
+          case 1: return spread_codes<3>(__funnelshift_r(w[0], w[1], 24) & 0xFFFFFFu);
+          case 2: return spread_codes<3>(__funnelshift_r(w[1], w[2], 16) & 0xFFFFFFu);
+          default: return spread_codes<3>(w[2] >> 8);
+        }
+      };
+      auto write_keys = [&](uint32_t dst, const Row& r) {
+        const uint32_t center = __byte_perm(r.stats, 0, 0x1010), scale = __byte_perm(r.stats, 0, 0x3232);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t l[4];
+          pair_levels(k_table, codes(r, c), l);
+          sts128(dst + ((static_cast<uint32_t>(c) ^ x7) << 4), half2_fma(scale, l[0], center), half2_fma(scale, l[1], center),
+                 half2_fma(scale, l[2], center), half2_fma(scale, l[3], center));
+        }
+      };
+      auto write_values = [&](uint32_t dst, const Row& r) {
+        const f32x2 center = sixteen_to_pair<__half>(__byte_perm(r.stats, 0, 0x1010)), scale = sixteen_to_pair<__half>(__byte_perm(r.stats, 0, 0x3232));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          f32x2 l[4];
+          pair_levels_f32(v_table, codes(r, c), l);
+          uint32_t w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) w[n] = pair_to_sixteen<__half>(fma2(scale, l[n], center));
+          sts128(dst + ((static_cast<uint32_t>(c) ^ x7) << 4), w[0], w[1], w[2], w[3]);
+        }
+      };
+      Row kr, vr;
+      uint32_t seen = 0;
+      auto fetch = [&](int j) {
+        const Place pl = place(j);
+        const int u = lane >> 4;
+        const bool is = (pl.seen >> lane) & 1;
+        load_row(p.k, pl.k[u] + (lane & 15) * p.k.token_stride, pl.st[u] + (lane & 15), is, kr);
+        load_row(p.v, pl.v[u] + (lane & 15) * p.v.token_stride, pl.st[u] + (lane & 15), is, vr);
+        seen = pl.seen;
+      };
+      if (count > 0) fetch(0);
+      for (int j = 0; j < count; ++j) {
+        const int slot = j % kTileSlots;
+        const Row k = kr, v = vr;
+        const uint32_t now = seen;
+        if (j + 1 < count) fetch(j + 1);
+        free_slot(k_free, j);
+        write_keys(k_smem + slot * kTileBytes + row, k);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full + slot);
+        free_slot(v_free, j);
+        write_values(v_smem + slot * kTileBytes + row, v);
+        if (lane == 0) s_seen[slot * 4 + w] = now;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full + slot);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: a thread a row
+    more_registers<kTileSoftmaxRegs>();
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int at = row0 + (halves ? t * kTileRows : 0) + r;                       // of the sequence's rows
+    const bool live = at < row0 + rows;
+    const int i_query = at / p.group, head = kvh * p.group + at % p.group;
+    const int limit = !live ? 0 : p.causal ? min(seq.keys, max(seq.keys - seq.all_queries + i_query + 1, 0)) : seq.keys;
+    float scale = p.scale_log2;
+    // ---- the row of queries; without halves the second stream's are the first's
+    if (halves || t == 0) {
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (live) u = reinterpret_cast<const uint4*>(attend_query(p, seq, b, i_query, head))[c];
+        w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
+      }
+      if (PACKED && p.q_bf16) scale *= bf16_to_half(w, 32, bf16_top(w, 32));
+      const uint32_t dst = smem_u32(smem) + L.q + t * kTileBytes + r * 128;
+      row_store<1>(w, dst, r & 7);
+      fence_proxy_async_smem();
+      if (!halves) s_max[r] = scale;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + t);
+    }
+    if (!halves) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      scale = s_max[r];
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    const int mine = halves ? count : (count + 1 - t) / 2;
+    const float ninf = __int_as_float(0xff800000);
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_at = tmem + tile_s_col(t) + lanes, p_at = tmem + tile_p_col(t) + lanes, o_at = tmem + tile_o_col(t) + lanes;
+    const bool rows_here = __any_sync(0xffffffffu, live);
+    float top = ninf;                                                             // in units of the exponent
+    f32x2 sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
+    for (int i = 0; i < mine; ++i) {
+      const int j = halves ? i : 2 * i + t, slot = j % kTileSlots;
+      ok = ok && mbar_wait_warp(s_full + t, i & 1, polls);
+      tc_fence_after_sync();
+      if (rows_here && ok) {
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read + t);
+        // ---- what is not seen
+        ok = ok && mbar_wait_warp(v_full + slot, (j / kTileSlots) & 1, polls);
+        const uint4 seen = lds128(smem_u32(s_seen + slot * 4));
+        const int base = (first + j) * kTileKeys;
+        if (!__all_sync(0xffffffffu, (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && base + kTileKeys <= limit)) {
+          const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int left = limit - base - 32 * c;                               // keys of the 32 that the row may see
+            const uint32_t word = words[c] & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+#pragma unroll
+            for (int n = 0; n < 32; ++n) s[c][n] = (word >> n) & 1 ? s[c][n] : 0xff800000u;
+          }
+        }
+        // ---- maximum
+        float m0 = ninf, m1 = ninf, m2 = ninf, m3 = ninf;
+#pragma unroll
+        for (int n = 0; n < 32; n += 2) {
+          m0 = max3(m0, __uint_as_float(s[0][n]), __uint_as_float(s[0][n + 1]));
+          m1 = max3(m1, __uint_as_float(s[1][n]), __uint_as_float(s[1][n + 1]));
+          m2 = max3(m2, __uint_as_float(s[2][n]), __uint_as_float(s[2][n + 1]));
+          m3 = max3(m3, __uint_as_float(s[3][n]), __uint_as_float(s[3][n + 1]));
+        }
+        const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale;
+        // the probabilities' columns are free, and the output may be scaled, once the last product has ended
+        if (i > 0) ok = ok && mbar_wait_warp(o_done + t, (i - 1) & 1, polls);
+        tc_fence_after_sync();
+        const bool renew = m > top + 8.0f || (top == ninf && m > ninf);
+        if (__any_sync(0xffffffffu, renew) && ok) {
+          const float next = renew ? m : top;
+          const float f = renew ? exp2_approx(top - next) : 1.0f;
+          top = next;
+          const f32x2 f2 = pack2(f, f);
+          sum0 = mul2(sum0, f2);
+          sum1 = mul2(sum1, f2);
+          if (i > 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_at + 32 * h, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
+              tmem_st_32x32(o_at + 32 * h, o);
+            }
+          }
+        }
+        const float nm = top == ninf ? 0.0f : -top;
+        const f32x2 scale2 = pack2(scale, scale), nm2 = pack2(nm, nm);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            float x, y;
+            unpack2(fma2(pack2(__uint_as_float(s[c][2 * n]), __uint_as_float(s[c][2 * n + 1])), scale2, nm2), x, y);
+            const f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
+            if (n & 1) sum1 = add2(sum1, e); else sum0 = add2(sum0, e);
+            w[n] = pair_to_sixteen<E>(e);
+          }
+          tmem_st_32x16(p_at + 16 * c, w);
+        }
+        tmem_st_wait();
+      } else {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read + t);
+        if (i > 0 && ok) ok = mbar_wait_warp(o_done + t, (i - 1) & 1, polls);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + t);
+    }
+    // ---- the stream's part: maximum, sum and output, as they are
+    if (mine > 0) ok = ok && mbar_wait_warp(o_done + t, (mine - 1) & 1, polls);
+    tc_fence_after_sync();
+    float x, y;
+    unpack2(add2(sum0, sum1), x, y);
+    s_max[t * kTileRows + r] = top;
+    s_sum[t * kTileRows + r] = x + y;
+  }
+  // ---------------------------------------------------------------------- join and write
+  // All copies into the key and value slots have landed (their products have ended) or nobody waits for them any more.
+  tc_fence_before_sync();
+  const bool gave_up = __syncthreads_or(!ok) != 0;
+  tc_fence_after_sync();
+  if (gave_up && tid == 12 * 32) atomicExch(p.status, kStatusTileAttentionTimeout);
+  float* const part = reinterpret_cast<float*>(smem + L.k);                       // [stream][row][64], over the slots, 16-byte chunks swizzled by row
+  if (warp < 8) {
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int mine = halves ? count : (count + 1 - t) / 2;
+    const uint32_t o_at = tmem + tile_o_col(t) + (static_cast<uint32_t>(quarter * 32) << 16);
+    const bool none = s_max[t * kTileRows + r] == __int_as_float(0xff800000);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t o[32];
+      if (mine > 0 && !gave_up) {
+        tmem_ld_32x32(o_at + 32 * h, o);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int n = 0; n < 32; n += 4) {
+        uint4 u = make_uint4(o[n], o[n + 1], o[n + 2], o[n + 3]);
+        if (mine <= 0 || gave_up || none) u = make_uint4(0, 0, 0, 0);
+        sts128(smem_u32(part) + (t * kTileRows + r) * 256 + (((h * 8 + (n >> 2)) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  const bool many = p.splits > 1;
+  __syncthreads();
+  tc_fence_after_sync();
+  if (gave_up && (warp == 12 || warp == 13)) {                                    // products that nobody waited for end before their memory is given back
+    if (elect_one()) umma_commit(stopped);
+    __syncwarp();
+    mbar_wait(stopped, 0);
+    __syncwarp();
+  }
+  if (warp == 12) tmem_dealloc(tmem, kTileTmemCols);
+  if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  // four values a thread; the rows are shared out over the blocks of the cluster
+  {
+    const int share = (rows + p.splits - 1) / p.splits, from = split * share, to = min(rows, from + share);
+    const int parts = (halves ? 1 : 2) * p.splits;
+    for (int e = from * 16 + tid; e < to * 16; e += kTileThreads) {
+      const int r = e >> 4, c = e & 15;
+      float m = __int_as_float(0xff800000), l = 0.0f;
+      float4 o = make_float4(0, 0, 0, 0);
+      auto address = [&](int q, uint32_t offset, int stream_bytes) {
+        const int rank = halves ? q : q >> 1, t = halves ? r >> 7 : q & 1;
+        uint32_t a = smem_u32(smem) + offset + t * stream_bytes, d;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(rank));
+        return d;
+      };
+      const int rr = r & 127;
+      for (int q = 0; q < parts; ++q) m = fmaxf(m, lds_cluster(address(q, L.max, kTileRows * 4) + rr * 4));
+      const float base = m == __int_as_float(0xff800000) ? 0.0f : m;
+      for (int q = 0; q < parts; ++q) {
+        const float f = exp2_approx(lds_cluster(address(q, L.max, kTileRows * 4) + rr * 4) - base);
+        l += f * lds_cluster(address(q, L.sum, kTileRows * 4) + rr * 4);
+        const float4 v = lds128_cluster(address(q, L.k, kTileRows * 256) + rr * 256 + ((c ^ (rr & 7)) << 4));
+        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+      }
+      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);             // a query that sees no key: zeros; NaN stays NaN
+      const int at = row0 + r;
+      const long long token = seq.first_row + at / p.group;
+      const long long dst = (token * p.heads + kvh * p.group + at % p.group) * 64 + 4 * c;
+      const f32x2 lo = pack2(o.x * inv, o.y * inv), hi = pack2(o.z * inv, o.w * inv);
+      const uint2 u = p.q_bf16 ? make_uint2(pair_to_sixteen<__nv_bfloat16>(lo), pair_to_sixteen<__nv_bfloat16>(hi))
+                               : make_uint2(pair_to_sixteen<__half>(lo), pair_to_sixteen<__half>(hi));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + dst) = u;
+    }
+  }
+  __syncwarp();
+  if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+}  // namespace arcq

@@ -220,6 +220,15 @@ def test_new_tokens_in_pieces(pkg, cuda_device, bits, dtype, heads, kv_heads, pa
     _paged_check(pkg, cuda_device, bits, dtype, heads, kv_heads, page, lengths, new, seed=4, causal=False, scale=0.3, strided=True)
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("new", [3, 40, 140])
+def test_more_sequences_than_multiprocessors(pkg, cuda_device, bits, new):
+    """Every block then has all keys of its rows, a ring of tiles deep."""
+    lengths = [200 + (37 * i) % 900 for i in range(170)]
+    _paged_check(pkg, cuda_device, bits, torch.float16, 1, 1, 64, lengths, [min(new, 1 + (11 * i) % (new + 9)) for i in range(170)], seed=14)
+    _cross_check(pkg, cuda_device, torch.bfloat16, 170, new, 900, 1, 1, "mask", seed=15)
+
+
 @pytest.mark.parametrize("bits,dtype", [(4, torch.float16), (16, torch.bfloat16)])
 def test_long_contexts(pkg, cuda_device, bits, dtype):
     _paged_check(pkg, cuda_device, bits, dtype, 3, 3, 64, [20011, 4097], [1, 1], seed=5)

@@ -23,6 +23,7 @@ EXPORTS = (
     "arcq_dense_weight_gemm_gelu_quant_applies", "arcq_packed_linear_small", "arcq_packed_linear_small_applies",
     "arcq_packed_linear_small_applies_captured",
     "arcq_kv_cache_write", "arcq_kv_cache_read", "arcq_paged_attention", "arcq_cross_attention",
+    "arcq_attention_workspace",
 )
 
 
@@ -86,8 +87,9 @@ def load() -> ctypes.CDLL:
     cache, strides = ctypes.POINTER(KvCache), ctypes.POINTER(i64)
     lib.arcq_kv_cache_write.argtypes = [cache, vp, vp, vp, ci, i64, strides, strides, vp, vp]
     lib.arcq_kv_cache_read.argtypes = [cache, vp, i64, vp, vp, ci, vp]
-    lib.arcq_paged_attention.argtypes = [cache, vp, ci, i64, strides, i64, i64, vp, i64, vp, vp, i64, ci, ctypes.c_float, vp, vp]
-    lib.arcq_cross_attention.argtypes = [vp, vp, vp, ci, i64, i64, i64, i64, i64, strides, strides, strides, vp, vp, i64, ctypes.c_float, vp, vp]
+    lib.arcq_paged_attention.argtypes = [cache, vp, ci, i64, strides, i64, i64, vp, i64, vp, vp, i64, ci, ctypes.c_float, vp, vp, i64, vp]
+    lib.arcq_cross_attention.argtypes = [vp, vp, vp, ci, i64, i64, i64, i64, i64, strides, strides, strides, vp, vp, i64, ctypes.c_float, vp, vp, i64, vp]
+    lib.arcq_attention_workspace.argtypes, lib.arcq_attention_workspace.restype = [i64] * 4, i64
     for name in EXPORTS:
         getattr(lib, name)  # AttributeError here means header and library disagree
     _lib = lib

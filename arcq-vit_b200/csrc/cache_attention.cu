@@ -64,6 +64,7 @@ int check_cache(const arcq_kv_cache* c) {
   if (c->heads <= 0 || c->heads > 65535 || c->pages < 0 || c->pages > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad cache: pages=%lld heads=%lld", (long long)c->pages, (long long)c->heads);
   if (c->page_size < 16 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)) != 0)
     return fail(ARCQ_E_UNSUPPORTED, "page size %lld: a power of two of at least 16 tokens", (long long)c->page_size);
+  if (c->bits != 16 && (c->codebooks == nullptr || !aligned(c->codebooks, 4))) return fail(ARCQ_E_BAD_ARG, "packed pages need codebooks");
   if (c->pages == 0) return ARCQ_OK;
   if (c->k_pages == nullptr || c->v_pages == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16)) return fail(ARCQ_E_ALIGN, "pages must be 16-byte aligned");
@@ -71,8 +72,8 @@ int check_cache(const arcq_kv_cache* c) {
     if (c->dtype != ARCQ_DT_F16 && c->dtype != ARCQ_DT_BF16) return fail(ARCQ_E_BAD_ARG, "pages in 16 bits are fp16 or bf16");
     return ARCQ_OK;
   }
-  if (c->k_stats == nullptr || c->v_stats == nullptr || c->codebooks == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
-  if (!aligned(c->k_stats, 16) || !aligned(c->v_stats, 16) || !aligned(c->codebooks, 4)) return fail(ARCQ_E_ALIGN, "statistics must be 16-byte aligned");
+  if (c->k_stats == nullptr || c->v_stats == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
+  if (!aligned(c->k_stats, 16) || !aligned(c->v_stats, 16)) return fail(ARCQ_E_ALIGN, "statistics must be 16-byte aligned");
   return ARCQ_OK;
 }
 
@@ -117,26 +118,40 @@ template <typename O> cudaError_t read_cache(const arcq::KvCacheParams& p, int b
   }
 }
 
-template <int BITS, typename E> int launch_split(arcq::AttendParams& p, cudaStream_t st) {
+// ---- few rows: the steps of all units cut evenly, parts joined behind
+void split_shape(arcq::AttendParams& p) {
+  const long long rows = static_cast<long long>(p.max_new) * p.group;
+  p.tiles = static_cast<int>((rows + arcq::kSplitRows - 1) / arcq::kSplitRows);
+  p.part_rows = static_cast<int>(rows < arcq::kSplitRows ? rows : arcq::kSplitRows);
+}
+bool few_rows(const arcq::AttendParams& p) { return static_cast<long long>(p.max_new) * p.group <= 2 * arcq::kSplitRows; }
+
+template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
-  constexpr size_t smem = 2 * arcq::kPairTableBytes;      // also room for the warps' accumulators
-  static_assert(smem >= arcq::kSplitWarps * arcq::kSplitRows * 64 * 4, "");
+  auto join = arcq::join_attention_kernel<arcq::SplitStep<BITS>::kKeys>;
+  constexpr size_t smem = arcq::split_smem<BITS>();
   static thread_local int done_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
   if (done_dev != dev) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return arcq_host::cuda_fail(e, "split attention set-up");
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaFuncAttributes a = {};
+    int reserved = 0;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, k);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev);
+    if (e != cudaSuccess) return arcq_host::cuda_fail(e, "attention set-up");
+    if (BITS != 16 && a.sharedSizeBytes + reserved + 128 > arcq::kSplitBase)       // the rings are laid out around the table
+      return fail(ARCQ_E_CUDA, "attention: %lld bytes of shared memory before the rings, %lld are provided for", (long long)(a.sharedSizeBytes + reserved), (long long)arcq::kSplitBase);
     done_dev = dev;
   }
-  p.tiles = static_cast<int>((static_cast<long long>(p.max_new) * p.group + arcq::kSplitRows - 1) / arcq::kSplitRows);
-  const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.tiles;
-  const long long steps = (p.max_keys + arcq::KeyBlock<BITS>::kKeys * arcq::kSplitWarps - 1) / (arcq::KeyBlock<BITS>::kKeys * arcq::kSplitWarps);
-  int splits = 1;
-  while (splits < arcq::kSplitMaxBlocks && splits < steps && units * splits < arcq_host::sm_count()) splits *= 2;
-  p.splits = splits;
-  if (units * splits > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
-  const cudaError_t e = launch(k, dim3(static_cast<unsigned>(units * splits)), arcq::kSplitThreads, smem, splits, st, p);
+  split_shape(p);
+  const int sms = arcq_host::sm_count();
+  if (p.workspace == nullptr || workspace_bytes < arcq::split_workspace(p, sms))
+    return fail(ARCQ_E_BAD_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)arcq::split_workspace(p, sms));
+  const long long units = arcq::split_units(p), steps = units * (p.max_keys / arcq::SplitStep<BITS>::kKeys + 1);
+  if (units > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
+  cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
+  if (e == cudaSuccess) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 
@@ -181,16 +196,18 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 
-template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, cudaStream_t st) {
-  return static_cast<long long>(p.max_new) * p.group > 2 * arcq::kSplitRows ? launch_tile<BITS, E>(p, st) : launch_split<BITS, E>(p, st);
+template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
+  return few_rows(p) ? launch_split<BITS, E>(p, workspace_bytes, st) : launch_tile<BITS, E>(p, st);
 }
 
-int run_attention(arcq::AttendParams& p, int bits, int dtype, cudaStream_t st) {
+int run_attention(arcq::AttendParams& p, int bits, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+  p.workspace = workspace;
+  if (!aligned(workspace, 16)) return fail(ARCQ_E_ALIGN, "the workspace must be 16-byte aligned");
   switch (bits) {
-    case 4: return launch_attention<4, __half>(p, st);
-    case 3: return launch_attention<3, __half>(p, st);
-    case 2: return launch_attention<2, __half>(p, st);
-    default: return dtype == ARCQ_DT_BF16 ? launch_attention<16, __nv_bfloat16>(p, st) : launch_attention<16, __half>(p, st);
+    case 4: return launch_attention<4, __half>(p, workspace_bytes, st);
+    case 3: return launch_attention<3, __half>(p, workspace_bytes, st);
+    case 2: return launch_attention<2, __half>(p, workspace_bytes, st);
+    default: return dtype == ARCQ_DT_BF16 ? launch_attention<16, __nv_bfloat16>(p, workspace_bytes, st) : launch_attention<16, __half>(p, workspace_bytes, st);
   }
 }
 
@@ -259,9 +276,21 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "cache read launch");
 }
 
+int64_t arcq_attention_workspace(int64_t batch, int64_t max_new, int64_t heads, int64_t kv_heads) {
+  if (batch <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || batch > 0x7fffffffLL || max_new > 0x7fffffffLL || heads > 65535 || heads % kv_heads != 0) return 0;
+  arcq::AttendParams p = {};
+  p.batch = static_cast<int>(batch);
+  p.max_new = static_cast<int>(max_new);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = static_cast<int>(heads / kv_heads);
+  if (!few_rows(p)) return 0;
+  split_shape(p);
+  return arcq::split_workspace(p, arcq_host::sm_count());
+}
+
 int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype, int64_t q_rows, const int64_t* q_strides, int64_t heads,
                          int64_t batch, const int32_t* page_table, int64_t table_width, const int32_t* lengths, const int32_t* starts,
-                         int64_t max_new, int causal, float scale, void* out, void* stream) {
+                         int64_t max_new, int causal, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check_cache(cache)) return rc;
   if (batch < 0 || table_width < 0 || max_new < 0 || q_rows < 0 || q_rows > 0x7fffffffLL || batch > 0x7fffffffLL || max_new > 0x7fffffffLL)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld table=%lld new=%lld rows=%lld", (long long)batch, (long long)table_width, (long long)max_new, (long long)q_rows);
@@ -304,12 +333,12 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
   p.kv_heads = static_cast<int>(cache->heads);
   p.group = p.heads / p.kv_heads;
   p.batch = static_cast<int>(batch);
-  return run_attention(p, cache->bits, cache->dtype, static_cast<cudaStream_t>(stream));
+  return run_attention(p, cache->bits, cache->dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
-                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* stream) {
+                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > 0x7fffffffLL - 64)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld queries=%lld states=%lld", (long long)batch, (long long)queries, (long long)states);
   if (batch == 0 || queries == 0) return ARCQ_OK;
@@ -345,7 +374,7 @@ int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype,
   p.kv_heads = static_cast<int>(kv_heads);
   p.group = p.heads / p.kv_heads;
   p.batch = static_cast<int>(batch);
-  return run_attention(p, 16, dtype, static_cast<cudaStream_t>(stream));
+  return run_attention(p, 16, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

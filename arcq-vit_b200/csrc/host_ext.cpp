@@ -402,6 +402,11 @@ PyObject* kv_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return out;
 }
 
+at::Tensor attention_workspace(int64_t batch, int64_t max_new, int64_t heads, int64_t kv_heads, c10::Device dev) {
+  const int64_t bytes = arcq_attention_workspace(batch, max_new, heads, kv_heads);
+  return bytes > 0 ? empty_cuda({bytes}, at::kByte, dev) : at::Tensor();
+}
+
 // paged_attention(q, page_table, lengths, starts, max_new, causal, scale, out, k_pages, v_pages, k_stats, v_stats, codebooks) -> out or None
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 13 || !all_bools(args, {5})) Py_RETURN_NONE;
@@ -426,9 +431,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   without_gil([&] {
     const c10::cuda::CUDAGuard guard(dev);
     if (!out.defined()) out = empty_cuda(q->sizes(), q->scalar_type(), dev);
+    const at::Tensor work = attention_workspace(table->size(0), max_new, q->size(1), c.heads, dev);
     check(arcq_paged_attention(&c, q->const_data_ptr(), qt, q->size(0), qs, q->size(1), table->size(0), table->const_data_ptr<int>(), table->size(1),
                                lengths->const_data_ptr<int>(), starts != nullptr ? starts->const_data_ptr<int>() : nullptr, max_new,
-                               args[5] == Py_True, scale, out.mutable_data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
+                               args[5] == Py_True, scale, out.mutable_data_ptr(), work.defined() ? work.mutable_data_ptr() : nullptr,
+                               work.defined() ? work.numel() : 0, c10::cuda::getCurrentCUDAStream().stream()),
           "arcq_paged_attention");
   });
   if (args[7] != Py_None) {
@@ -465,10 +472,12 @@ PyObject* cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   without_gil([&] {
     const c10::cuda::CUDAGuard guard(dev);
     if (!out.defined()) out = empty_cuda(q->sizes(), q->scalar_type(), dev);
+    const at::Tensor work = attention_workspace(q->size(0), q->size(1), q->size(2), k->size(2), dev);
     check(arcq_cross_attention(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), qt, q->size(0), q->size(1), k->size(1), q->size(2),
                                k->size(2), qs, ks, vs, lengths != nullptr ? lengths->const_data_ptr<int>() : nullptr,
                                mask != nullptr ? static_cast<const uint8_t*>(mask->const_data_ptr()) : nullptr,
-                               mask != nullptr ? mask->stride(0) : 0, scale, out.mutable_data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
+                               mask != nullptr ? mask->stride(0) : 0, scale, out.mutable_data_ptr(), work.defined() ? work.mutable_data_ptr() : nullptr,
+                               work.defined() ? work.numel() : 0, c10::cuda::getCurrentCUDAStream().stream()),
           "arcq_cross_attention");
   });
   if (args[6] != Py_None) {

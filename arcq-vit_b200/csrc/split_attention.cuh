@@ -1,16 +1,22 @@
 // Attention of few queries a key head over long keys: one new token of a sequence over its cache, or of an image's text over the
-// encoder's states.  Keys and values are read once and never staged: registers straight from global memory to the tensor instructions.
+// encoder's states.
 //
 //   s_ij = scale * q_i . k_j over the keys j that query i sees,   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
 //
-// The rows of a tile are 16 (query, head) pairs that share a key head.  Its keys are split over the blocks of a cluster, and a block's
-// over its warps, blocks of 16 or 32 keys in turn; each warp keeps a running maximum, sum and 16 x 64 accumulator, joined in shared
-// memory of the block and then of the cluster.  No workspace, no second launch, a fixed order of every sum.
+// A unit is a tile of up to 16 (query, head) rows of a sequence that share a key head, with all the keys they see, in steps of 32 keys (16
+// in 16 bits).  The steps of all units lie on one line that is cut into equal pieces, one a warp, whatever the lengths are: no warp waits
+// for another, and long sequences are spread over the GPU as evenly as many short ones.  A warp keeps the running maximum and sum and the
+// 16 x 64 accumulator in registers; it writes a unit that lies in its piece whole, and of one that does not (at most the first and the last)
+// its part, which the join kernel behind it adds up in the order of the keys.
 //
-// Packed keys and values become fp16 in registers: a byte of two codes is an index into a table of pairs of levels (a copy a lane, so
-// that a read has no bank conflicts), one half-precision fma makes center + scale * level.  Keys are paired along a head's values, which
-// the packed byte already is; values along the keys, two bytes interleaved.  The order of a head's values within a product is free, so
-// each lane takes 16 (keys) or 8 (values) that lie next to each other.
+// Each warp has a ring of steps in shared memory of its own, filled by asynchronous copies two steps ahead (no barriers).  Packed rows are
+// copied as they are and become fp16 on the way into the tensor instructions: a byte of two codes is moved into bits 8-15 of a table
+// address by one byte permute (the table lies on a 64 KB boundary, with a copy a lane or half warp, so reads have no bank conflicts), and one
+// fma makes center + scale * level.  Keys: levels in fp16, a half-precision fma of two values.  Values: levels and fma in fp32 and one
+// rounding, because the rounding of a level is the same in every key that has its code and adds up over a long context (error against
+// 64 bits over 65 521 keys of 3 bits, relative to the output: 3.9e-4 with fp16 levels, 2.1e-4 so, which is the output's own rounding).
+// Pairs of keys' values are a byte as it is stored; of values, which have to be paired along the keys, nibbles of two keys are interleaved.  The
+// order of a head's values in a product is free, and so is that of keys: each lane takes values that lie side by side.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -46,6 +52,8 @@ struct AttendParams {
   float scale_log2;                     // scale / ln 2
   void* out;                            // [tokens, heads, 64]
   int heads, kv_heads, group, tiles, splits, batch;
+  void* workspace;                      // split_attention_kernel
+  int part_rows;                        // of a part: 16, or all rows that there can be
   uint32_t poll_limit;                  // tile_attention.cuh
   int* status;
 };
@@ -111,8 +119,7 @@ __device__ __forceinline__ float bf16_to_half(uint32_t* w, int n, float top) {
   return __int_as_float((127 - up) << 23);
 }
 
-constexpr int kSplitWarps = 8, kSplitThreads = kSplitWarps * 32, kSplitRows = 16;
-constexpr int kSplitMaxBlocks = 8;                                  // of a cluster: the portable size
+constexpr int kSplitWarps = 16, kSplitThreads = kSplitWarps * 32, kSplitRows = 16, kSplitStages = 3;
 constexpr uint32_t kPairTableBytes = 256 * 32 * 4;                  // [byte][lane]
 
 // [byte][lane]: the levels of the byte's two codes, low nibble first
@@ -153,361 +160,586 @@ __device__ __forceinline__ void pair_levels_f32(uint32_t table, uint32_t w, f32x
   pairs[3] = lds_const_pair(table + ((w >> 17) & 0x7F80u));
 }
 
-// The rows of one block of keys that a lane holds.  Lane 4g + c: of keys 8n + g the 16 values from 16c, of values 2c, 2c + 1 (+ 8 n) the 8 from 8g.
-template <int BITS> struct KeyBlock;
-template <int BITS> struct KeyBlock {
-  static constexpr int kKeys = 32;
-  uint32_t k[4][BITS == 4 ? 2 : BITS == 3 ? 2 : 1], v[4][2], k_stats[4], v_stats[4][2];
+// ---------------------------------------------------------------- shared memory of split_attention_kernel
+// Packed: the tables at shared address 64 KB, 256 bytes a byte of codes: 32 copies of its pair of fp16 levels (keys), 16 of fp32 levels
+// (values); the warps' rings below and above.
+constexpr uint32_t kSplitTable = 0x10000, kSplitTableEnd = 0x20000;
+template <int BITS> struct SplitStep {
+  static constexpr int kKeys = BITS == 16 ? 16 : 32;
+  static constexpr uint32_t kRow = BITS == 16 ? 128 : 8 * BITS;
+  static constexpr uint32_t kRows = kKeys * kRow;                                 // keys, or values
+  static constexpr uint32_t kStats = BITS == 16 ? 0 : 4 * kKeys;                  // likewise
+  static constexpr uint32_t kBytes = 2 * (kRows + kStats) + 16;      // and which keys are seen
+  static constexpr uint32_t kRing = kSplitStages * kBytes;
 };
-template <> struct KeyBlock<16> {
-  static constexpr int kKeys = 16;
-  uint4 k[2][2], v[2][2];
+// `base`: where the block's shared memory starts; rings of warps that do not fit below the table lie above it
+template <int BITS> __host__ __device__ constexpr uint32_t split_ring(uint32_t base, int warp) {
+  const uint32_t ring = SplitStep<BITS>::kRing;
+  if (BITS == 16) return base + warp * ring;
+  const int below = static_cast<int>((kSplitTable - base) / ring);
+  return warp < below ? base + warp * ring : kSplitTableEnd + (warp - below) * ring;
+}
+// dynamic shared memory for a base of at most kSplitBase
+constexpr uint32_t kSplitBase = 8192;
+template <int BITS> constexpr uint32_t split_smem() {
+  return BITS == 16 ? kSplitWarps * SplitStep<16>::kRing + 128 : split_ring<BITS>(kSplitBase, kSplitWarps);
+}
+
+// ---------------------------------------------------------------- units and their line
+struct SplitUnit {
+  int b, kvh, tile;
+  AttendSequence seq;
+  int rows, keys, steps;
 };
+__device__ __forceinline__ int split_tiles(const AttendParams& p, const AttendSequence& s) {
+  return static_cast<int>((static_cast<long long>(s.queries) * p.group + kSplitRows - 1) / kSplitRows);
+}
+template <int KEYS> __device__ __forceinline__ void split_tile(const AttendParams& p, SplitUnit& u) {
+  u.rows = static_cast<int>(min(static_cast<long long>(u.seq.queries) * p.group - static_cast<long long>(u.tile) * kSplitRows, static_cast<long long>(kSplitRows)));
+  u.keys = u.seq.keys;
+  if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * kSplitRows + u.rows - 1) / p.group + 1, 0));
+  u.steps = max((u.keys + KEYS - 1) / KEYS, 1);                                   // a unit without keys has a step, in which nothing is seen
+}
+// steps of all units of a sequence
+template <int KEYS> __device__ __forceinline__ long long split_sequence_steps(const AttendParams& p, int b) {
+  SplitUnit u;
+  u.seq = attend_sequence(p, b);
+  const int tiles = split_tiles(p, u.seq);
+  long long n = 0;
+  for (u.tile = 0; u.tile < tiles; ++u.tile) {
+    split_tile<KEYS>(p, u);
+    n += u.steps;
+  }
+  return n * p.kv_heads;
+}
+// Behind the last unit: b = batch.
+template <int KEYS> __device__ __forceinline__ void split_next(const AttendParams& p, SplitUnit& u) {
+  if (++u.tile >= split_tiles(p, u.seq)) {
+    u.tile = 0;
+    if (++u.kvh == p.kv_heads) {
+      u.kvh = 0;
+      while (++u.b < p.batch) {
+        u.seq = attend_sequence(p, u.b);
+        if (u.seq.queries > 0) break;
+      }
+      if (u.b >= p.batch) return;
+    }
+  }
+  split_tile<KEYS>(p, u);
+}
+
+// Workspace: a header, a record for each unit, and two parts a warp (of a unit that began before the warp's piece, and of one that goes on
+// behind it); a part is a row of 64 outputs, maximum and sum for each of its rows.
+struct SplitHeader {
+  long long piece, unused;
+};
+struct SplitRecord {
+  long long start;
+  int steps, whole;
+};
+constexpr int kSplitPartRow = 68;
+__host__ __device__ inline long long split_units(const AttendParams& p) { return static_cast<long long>(p.batch) * p.kv_heads * p.tiles; }
+__host__ __device__ inline long long split_workspace(const AttendParams& p, int blocks) {
+  return static_cast<long long>(sizeof(SplitHeader)) + split_units(p) * sizeof(SplitRecord) +
+         2ll * blocks * kSplitWarps * p.part_rows * kSplitPartRow * 4;
+}
+__device__ __forceinline__ SplitRecord* split_records(const AttendParams& p) {
+  return reinterpret_cast<SplitRecord*>(static_cast<uint8_t*>(p.workspace) + sizeof(SplitHeader));
+}
+__device__ __forceinline__ float* split_part(const AttendParams& p, long long slot) {
+  return reinterpret_cast<float*>(split_records(p) + split_units(p)) + slot * p.part_rows * kSplitPartRow;
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool is) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// byte i of w into bits 8-15 of a table address
+template <int I> __device__ __forceinline__ uint32_t table_address(uint32_t w, uint32_t column) { return __byte_perm(w, column, 0x7604 | (I << 4)); }
 
 template <int BITS, typename E>
-__global__ void __launch_bounds__(kSplitThreads, 2) split_attention_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const __grid_constant__ AttendParams p) {
   pdl_launch_dependents();
   constexpr bool PACKED = BITS != 16;
-  constexpr int KEYS = KeyBlock<BITS>::kKeys, NT = KEYS / 8;
-  extern __shared__ __align__(128) uint8_t smem[];                  // tables of levels (keys, values), then accumulators over them
-  __shared__ float s_max[kSplitWarps][kSplitRows], s_sum[kSplitWarps][kSplitRows];
-  __shared__ float s_block_max[kSplitRows], s_block_sum[kSplitRows];
+  using Step = SplitStep<BITS>;
+  constexpr int KEYS = Step::kKeys, NT = KEYS / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_scan[kSplitThreads / 32], s_line[kSplitThreads];         // steps before each share of the sequences
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int tile = unit % p.tiles, kvh = unit / p.tiles % p.kv_heads, b = unit / p.tiles / p.kv_heads;
-  const uint32_t k_table = smem_u32(smem) + lane * 4, v_table = smem_u32(smem) + kPairTableBytes + (lane & 15) * 8;
   if constexpr (PACKED) {
-    fill_pair_table(smem_u32(smem), p.codebooks, 1 << BITS, tid, kSplitThreads);
-    fill_pair_table_f32(smem_u32(smem) + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, tid, kSplitThreads);
+    // 16-byte columns of the table: 8 of keys, 8 of values
+    const float *kl = p.codebooks, *vl = p.codebooks + (1 << BITS);
+    for (int i = tid; i < 256 * 16; i += kSplitThreads) {
+      const int byte = i >> 4, a = min(byte & 15, (1 << BITS) - 1), b = min(byte >> 4, (1 << BITS) - 1);
+      const uint32_t dst = kSplitTable + byte * 256 + (i & 15) * 16;
+      if ((i & 8) == 0) {
+        const uint32_t w = pair_to_sixteen<__half>(pack2(__ldg(kl + a), __ldg(kl + b)));
+        sts128(dst, w, w, w, w);
+      } else {
+        const uint32_t lo = __float_as_uint(__ldg(vl + a)), hi = __float_as_uint(__ldg(vl + b));
+        sts128(dst, lo, hi, lo, hi);
+      }
+    }
   }
   pdl_wait();
+
+  // ---- the line of steps: each thread a share of the sequences, a scan over the block
+  const int share = (p.batch + kSplitThreads - 1) / kSplitThreads;
+  long long mine = 0;
+  for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_sequence_steps<KEYS>(p, b);
+  long long before = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31) s_scan[warp] = before;
   __syncthreads();
-  const AttendSequence seq = attend_sequence(p, b);
-  const int rows = min(seq.queries * p.group - tile * kSplitRows, kSplitRows);     // <= 0: an empty tile
-  // keys that some row of the tile sees
-  int limit[2], keys = 0;
-  const uint16_t* q_row[2];
+  long long total = 0, base_of_warp = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = min(g + 8 * h, max(rows, 1) - 1), at = tile * kSplitRows + r, i = at / p.group, head = kvh * p.group + at % p.group;
-    limit[h] = p.causal ? min(seq.keys, max(seq.keys - seq.all_queries + i + 1, 0)) : seq.keys;
-    q_row[h] = attend_query(p, seq, b, i, head);
+  for (int w = 0; w < kSplitWarps; ++w) {
+    if (w < warp) base_of_warp += s_scan[w];
+    total += s_scan[w];
   }
-  if (rows > 0) {
-    const int i = (tile * kSplitRows + rows - 1) / p.group;
-    keys = p.causal ? min(seq.keys, max(seq.keys - seq.all_queries + i + 1, 0)) : seq.keys;
+  s_line[tid] = base_of_warp + before - mine;
+  __syncthreads();
+  const long long warps = static_cast<long long>(gridDim.x) * kSplitWarps;
+  const long long piece = max((total + warps - 1) / warps, 1ll);
+  const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;      // small jobs: a warp a multiprocessor
+  if (blockIdx.x == 0 && tid == 0) static_cast<SplitHeader*>(p.workspace)->piece = piece;
+  const long long start = me * piece, end = min(start + piece, total);
+  if (start >= end) return;
+
+  // ---- the unit that the piece starts in
+  SplitUnit u;
+  long long at;                                                                    // first step of the unit
+  {
+    int lo = 0, hi = kSplitThreads - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_line[mid] <= start) lo = mid; else hi = mid - 1;
+    }
+    at = s_line[lo];
+    int b = lo * share;
+    for (;; ++b) {
+      const long long n = split_sequence_steps<KEYS>(p, b);
+      if (at + n > start) break;
+      at += n;
+    }
+    u.b = b;
+    u.seq = attend_sequence(p, b);
+    const int tiles = split_tiles(p, u.seq);
+    long long n = 0;
+    for (u.tile = 0; u.tile < tiles; ++u.tile) {
+      split_tile<KEYS>(p, u);
+      n += u.steps;
+    }
+    u.kvh = static_cast<int>((start - at) / n);
+    at += u.kvh * n;
+    u.tile = 0;
+    for (;; ++u.tile) {
+      split_tile<KEYS>(p, u);
+      if (at + u.steps > start) break;
+      at += u.steps;
+    }
   }
 
-  // ---- queries: fragments of the four steps of 16 values; bf16 against fp16 keys: a power of two makes the row's largest value 2^13..2^14
-  uint32_t qa[4][4];
-  float row_scale[2] = {p.scale_log2, p.scale_log2};
+  const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
+  // ---- copies, ahead of the computation
+  SplitUnit f = u;                                                                 // where the next step to be copied is
+  int f_step = static_cast<int>(start - at);
+  long long f_left = end - start;
+  int page[KEYS / 16], f_slot = 0;                                                 // pages of its sixteens of keys; < 0: none
+  bool f_masked = true;
+  auto look_up = [&]() {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t w[8] = {};
-    if (g + 8 * h < rows) {
-      const uint4* const src = reinterpret_cast<const uint4*>(q_row[h] + 16 * c);
-      const uint4 u0 = src[0], u1 = src[1];
-      w[0] = u0.x; w[1] = u0.y; w[2] = u0.z; w[3] = u0.w; w[4] = u1.x; w[5] = u1.y; w[6] = u1.z; w[7] = u1.w;
+    for (int h = 0; h < KEYS / 16; ++h) {
+      const int key = f_step * KEYS + 16 * h;
+      page[h] = key < f.keys ? f.b : -1;
+      if (p.table != nullptr && key < f.keys) page[h] = p.table[static_cast<long long>(f.b) * p.table_width + (key >> p.page_shift)];
     }
-    if (PACKED && p.q_bf16) {
-      float top = bf16_top(w, 8);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      row_scale[h] *= bf16_to_half(w, 8, top);
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      qa[s][h] = w[2 * s];
-      qa[s][2 + h] = w[2 * s + 1];
-    }
-  }
-
-  const float ninf = __int_as_float(0xff800000);
-  float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {};
-
-  // ---- the block's share of the keys, in whole steps of 32
-  const int steps = (keys + KEYS - 1) / KEYS;
-  const int per = (steps + p.splits - 1) / p.splits;
-  const int first = split * per, last = min(first + per, steps);
-
-  auto load = [&](int step, KeyBlock<BITS>& blk, uint32_t& seen) {
-    const int base = step * KEYS;
-    // sixteen keys lie in one page
-    long long k_at[KEYS / 16], v_at[KEYS / 16], st_at[KEYS / 16];
-    bool there[KEYS / 16];
-#pragma unroll
-    for (int u = 0; u < KEYS / 16; ++u) {
-      const int j = base + 16 * u;
-      int block = b, place = j;
-      there[u] = j < keys;
-      if (p.table != nullptr && there[u]) {
-        block = p.table[static_cast<long long>(b) * p.table_width + (j >> p.page_shift)];
-        place = j & ((1 << p.page_shift) - 1);
-        there[u] = block >= 0 && block < p.pages;
-      }
-      k_at[u] = block * p.k.block_stride + kvh * p.k.head_stride + place * p.k.token_stride;
-      v_at[u] = block * p.v.block_stride + kvh * p.v.head_stride + place * p.v.token_stride;
-      st_at[u] = PACKED ? ((static_cast<long long>(block) * p.kv_heads + kvh) << p.page_shift) + place : 0;
-    }
-    bool mine = lane < KEYS && base + lane < keys && there[KEYS / 16 - 1 < (lane >> 4) ? KEYS / 16 - 1 : (lane >> 4)];
-    if (mine && p.mask != nullptr) mine = p.mask[b * p.mask_stride + base + lane] != 0;
-    seen = __ballot_sync(0xffffffffu, mine);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool is = (seen >> (8 * n + g)) & 1;
-      const uint8_t* const row = p.k.rows + k_at[n >> 1] + ((n & 1) * 8 + g) * p.k.token_stride;
-      if constexpr (PACKED) {
-        if constexpr (BITS == 4) {
-          const uint2 u = is ? *reinterpret_cast<const uint2*>(row + 8 * c) : make_uint2(0, 0);
-          blk.k[n][0] = u.x; blk.k[n][1] = u.y;
-        } else if constexpr (BITS == 3) {
-          const uint16_t* const h = reinterpret_cast<const uint16_t*>(row + 6 * c);
-          const uint32_t a = is ? h[0] : 0, d = is ? h[1] : 0, e = is ? h[2] : 0;
-          blk.k[n][0] = a | ((d & 0xFFu) << 16);
-          blk.k[n][1] = (d >> 8) | (e << 8);
-        } else {
-          blk.k[n][0] = is ? *reinterpret_cast<const uint32_t*>(row + 4 * c) : 0;
-        }
-        blk.k_stats[n] = is ? *reinterpret_cast<const uint32_t*>(p.k.stats + st_at[n >> 1] + (n & 1) * 8 + g) : 0;
-      } else {
-        const uint4* const r = reinterpret_cast<const uint4*>(row + 32 * c);
-        blk.k[n][0] = is ? r[0] : make_uint4(0, 0, 0, 0);
-        blk.k[n][1] = is ? r[1] : make_uint4(0, 0, 0, 0);
-      }
-      const uint8_t* const vrow = p.v.rows + v_at[n >> 1] + ((n & 1) * 8 + 2 * c) * p.v.token_stride;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bool vis = (seen >> (8 * n + 2 * c + t)) & 1;
-        const uint8_t* const r = vrow + t * p.v.token_stride;
-        if constexpr (PACKED) {
-          if constexpr (BITS == 4) {
-            blk.v[n][t] = vis ? *reinterpret_cast<const uint32_t*>(r + 4 * g) : 0;
-          } else if constexpr (BITS == 3) {
-            const int q = (3 * g) >> 2;
-            const uint32_t* const h = reinterpret_cast<const uint32_t*>(r);
-            const uint32_t lo = vis ? h[q] : 0, hi = vis ? h[min(q + 1, 5)] : 0;
-            blk.v[n][t] = __funnelshift_r(lo, hi, 8 * ((3 * g) & 3)) & 0xFFFFFFu;
-          } else {
-            blk.v[n][t] = vis ? *reinterpret_cast<const uint16_t*>(r + 2 * g) : 0;
-          }
-          blk.v_stats[n][t] = vis ? *reinterpret_cast<const uint32_t*>(p.v.stats + st_at[n >> 1] + (n & 1) * 8 + 2 * c + t) : 0;
-        } else {
-          blk.v[n][t] = vis ? *reinterpret_cast<const uint4*>(r + 16 * g) : make_uint4(0, 0, 0, 0);
-        }
-      }
+    if (!PACKED && p.mask != nullptr) {
+      const int key = f_step * KEYS + (lane & 15);
+      f_masked = key < f.keys && p.mask[f.b * p.mask_stride + key] != 0;
     }
   };
-
-  auto compute = [&](int step, const KeyBlock<BITS>& blk, uint32_t seen) {
-    const int base = step * KEYS;
-    float s[NT][4];
+  look_up();
+  auto copy_step = [&]() {
+    if (f_left > 0) {
+      const uint32_t dst = ring + f_slot * Step::kBytes;
+      const int base = f_step * KEYS;
+      const int in_page = p.table != nullptr ? (1 << p.page_shift) - 1 : 0x7fffffff;
+      bool there[KEYS / 16];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-      uint32_t kb[8];
+      for (int h = 0; h < KEYS / 16; ++h) there[h] = page[h] >= 0 && (p.table == nullptr || page[h] < p.pages);
       if constexpr (PACKED) {
-        uint32_t lo, hi;
-        if constexpr (BITS == 2) {
-          lo = spread_codes<2>(blk.k[n][0] & 0xFFFFu);
-          hi = spread_codes<2>(blk.k[n][0] >> 16);
-        } else {
-          lo = spread_codes<BITS>(blk.k[n][0]);
-          hi = spread_codes<BITS>(blk.k[n][1]);
-        }
-        uint32_t pl[4], ph[4];
-        pair_levels(k_table, lo, pl);
-        pair_levels(k_table, hi, ph);
-        const uint32_t center = __byte_perm(blk.k_stats[n], 0, 0x1010), scale = __byte_perm(blk.k_stats[n], 0, 0x3232);
+        // sixteen rows of a page lie side by side
+        constexpr int CHUNKS = 8 * BITS;                                           // of 16 bytes, in sixteen rows
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          kb[j] = half2_fma(scale, pl[j], center);
-          kb[4 + j] = half2_fma(scale, ph[j], center);
+        for (int h = 0; h < 2; ++h) {
+          const long long row = ((static_cast<long long>(page[h]) * p.kv_heads + f.kvh) << p.page_shift) + ((base + 16 * h) & in_page);
+          if (lane < CHUNKS) {
+            cp_async_16(dst + h * 16 * Step::kRow + lane * 16, p.k.rows + (there[h] ? row * Step::kRow + lane * 16 : 0), there[h]);
+            cp_async_16(dst + Step::kRows + h * 16 * Step::kRow + lane * 16, p.v.rows + (there[h] ? row * Step::kRow + lane * 16 : 0), there[h]);
+          }
+          if (lane < 8) {
+            const __half2* const st = lane < 4 ? p.k.stats : p.v.stats;
+            cp_async_16(dst + 2 * Step::kRows + (lane >> 2) * Step::kStats + h * 64 + (lane & 3) * 16, st + (there[h] ? row + (lane & 3) * 4 : 0), there[h]);
+          }
         }
+        const uint32_t seen = __ballot_sync(0xffffffffu, base + lane < f.keys && (lane < 16 ? there[0] : there[KEYS / 16 - 1]));
+        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + Step::kBytes - 16), "r"(seen) : "memory");
       } else {
-        kb[0] = blk.k[n][0].x; kb[1] = blk.k[n][0].y; kb[2] = blk.k[n][0].z; kb[3] = blk.k[n][0].w;
-        kb[4] = blk.k[n][1].x; kb[5] = blk.k[n][1].y; kb[6] = blk.k[n][1].z; kb[7] = blk.k[n][1].w;
+        const int place = base & in_page;
+        const bool is = there[0] && base + (lane & 15) < f.keys && f_masked;
+        const uint32_t seen = __ballot_sync(0xffffffffu, is) & 0xFFFFu;
+        const uint8_t* const k = p.k.rows + page[0] * p.k.block_stride + f.kvh * p.k.head_stride + place * p.k.token_stride;
+        const uint8_t* const v = p.v.rows + page[0] * p.v.block_stride + f.kvh * p.v.head_stride + place * p.v.token_stride;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 4 * r + (lane >> 3), ch = lane & 7;
+          const bool sees = (seen >> row) & 1;
+          const uint32_t to = dst + row * 128 + ((ch ^ (row & 7)) << 4);
+          cp_async_16(to, sees ? k + row * p.k.token_stride + 16 * ch : p.k.rows, sees);
+          cp_async_16(to + Step::kRows, sees ? v + row * p.v.token_stride + 16 * ch : p.v.rows, sees);
+        }
+        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + Step::kBytes - 16), "r"(seen) : "memory");
+      }
+      f_slot = f_slot + 1 == kSplitStages ? 0 : f_slot + 1;
+      if (--f_left > 0) {
+        if (++f_step == f.steps) {
+          split_next<KEYS>(p, f);
+          f_step = 0;
+        }
+        look_up();
+      }
+    }
+    cp_async_commit();
+  };
+  copy_step();
+  copy_step();
+
+  // ---- units
+  const float ninf = __int_as_float(0xff800000);
+  const uint32_t k_column = kSplitTable + lane * 4, v_column = kSplitTable + 128 + (lane & 15) * 8;
+  long long step = start;
+  int slot = 0;
+  while (step < end) {
+    // rows g and g + 8 of the unit: queries, the keys that they see, the factor of their scores
+    int limit[2];
+    uint32_t qa[4][4];
+    float row_scale[2] = {p.scale_log2, p.scale_log2};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool row = g + 8 * h < u.rows;
+      const int r = u.tile * kSplitRows + (row ? g + 8 * h : 0), i = r / p.group, head = u.kvh * p.group + r % p.group;
+      limit[h] = p.causal ? min(u.seq.keys, max(u.seq.keys - u.seq.all_queries + i + 1, 0)) : u.seq.keys;
+      const uint16_t* const src = attend_query(p, u.seq, u.b, i, head);
+      uint32_t w[8];
+      if constexpr (PACKED) {                                                      // values 16c .. 16c + 15
+        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
+        if (row) {
+          u0 = reinterpret_cast<const uint4*>(src + 16 * c)[0];
+          u1 = reinterpret_cast<const uint4*>(src + 16 * c)[1];
+        }
+        w[0] = u0.x; w[1] = u0.y; w[2] = u0.z; w[3] = u0.w; w[4] = u1.x; w[5] = u1.y; w[6] = u1.z; w[7] = u1.w;
+        if (p.q_bf16) {
+          float top = bf16_top(w, 8);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          row_scale[h] *= bf16_to_half(w, 8, top);
+        }
+      } else {                                                                     // values 8n + 2c and the next
+#pragma unroll
+        for (int n = 0; n < 8; ++n) w[n] = row ? *reinterpret_cast<const uint32_t*>(src + 8 * n + 2 * c) : 0u;
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) mma_16816<E>(s[n], qa[t], kb[2 * t], kb[2 * t + 1]);
+      for (int s = 0; s < 4; ++s) {
+        qa[s][h] = w[2 * s];
+        qa[s][2 + h] = w[2 * s + 1];
+      }
     }
-    // ---- softmax: lane 4g + c has rows g and g + 8, keys 8n + 2c and the next
-    const bool whole = seen == (KEYS == 32 ? 0xffffffffu : 0xffffu) && base + KEYS <= limit[0] && base + KEYS <= limit[1];
-    if (!whole) {
+    float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {};
+    const long long unit_end = min(at + u.steps, end);
+#pragma unroll 1
+    for (; step < unit_end; ++step) {
+      copy_step();
+      cp_async_wait<2>();
+      __syncwarp();
+      const uint32_t src = ring + slot * Step::kBytes;
+      slot = slot + 1 == kSplitStages ? 0 : slot + 1;
+      const int base = static_cast<int>(step - at) * KEYS;
+      // ---- scores.  Column 2c + j of a tile of 8 keys is key c + 4j (packed; so reads of values have no bank conflicts), in 16 bits key 2c + j.
+      const uint32_t seen = lds32(src + Step::kBytes - 16);
+      const bool all = seen == (KEYS == 32 ? 0xffffffffu : 0xffffu);
+      float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = 8 * n + 2 * c + (j & 1);
-          if (((seen >> key) & 1) == 0 || base + key >= limit[j >> 1]) s[n][j] = ninf;
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+      if constexpr (PACKED) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int key = 8 * n + (g >> 1) + 4 * (g & 1);
+          const uint32_t row = src + key * Step::kRow;
+          uint32_t lo, hi;
+          if constexpr (BITS == 4) {
+            const uint2 w = lds64(row + 8 * c);
+            lo = w.x; hi = w.y;
+          } else if constexpr (BITS == 3) {
+            const uint32_t first = row + ((6 * c) & ~3), w0 = lds32(first), w1 = lds32(first + 4), sh = (c & 1) * 16;
+            lo = spread_codes<3>(__funnelshift_r(w0, w1, sh) & 0xFFFFFFu);
+            hi = spread_codes<3>((c & 1 ? w1 >> 8 : __funnelshift_r(w0, w1, 24)) & 0xFFFFFFu);
+          } else {
+            const uint32_t w = lds32(row + 4 * c);
+            lo = spread_codes<2>(w & 0xFFFFu);
+            hi = spread_codes<2>(w >> 16);
+          }
+          uint32_t stats = lds32(src + 2 * Step::kRows + key * 4);
+          if (!all) stats = (seen >> key) & 1 ? stats : 0u;                        // whatever lies there: x = 0
+          const uint32_t center = __byte_perm(stats, 0, 0x1010), scale = __byte_perm(stats, 0, 0x3232);
+          uint32_t kb[8];
+          kb[0] = half2_fma(scale, lds_const_u32(table_address<0>(lo, k_column)), center);
+          kb[1] = half2_fma(scale, lds_const_u32(table_address<1>(lo, k_column)), center);
+          kb[2] = half2_fma(scale, lds_const_u32(table_address<2>(lo, k_column)), center);
+          kb[3] = half2_fma(scale, lds_const_u32(table_address<3>(lo, k_column)), center);
+          kb[4] = half2_fma(scale, lds_const_u32(table_address<0>(hi, k_column)), center);
+          kb[5] = half2_fma(scale, lds_const_u32(table_address<1>(hi, k_column)), center);
+          kb[6] = half2_fma(scale, lds_const_u32(table_address<2>(hi, k_column)), center);
+          kb[7] = half2_fma(scale, lds_const_u32(table_address<3>(hi, k_column)), center);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) mma_16816<E>(s[n], qa[t], kb[2 * t], kb[2 * t + 1]);
         }
+      } else {
+        // matrices of 8 keys x 8 values: lanes 0-7 keys 0-7, 8-15 the next eight values, 16-31 keys 8-15
+        const int row = (lane & 7) + 8 * (lane >> 4), ch = (lane >> 3) & 1;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4(src + row * 128 + (((2 * t + ch) ^ (row & 7)) << 4), b0, b1, b2, b3);
+          mma_16816<E>(s[0], qa[t], b0, b1);
+          mma_16816<E>(s[1], qa[t], b2, b3);
+        }
+      }
+      // ---- softmax: lane 4g + c has rows g and g + 8
+      if (!__all_sync(0xffffffffu, all && base + KEYS <= limit[0] && base + KEYS <= limit[1])) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = 8 * n + (PACKED ? c + 4 * (j & 1) : 2 * c + (j & 1));
+            if (((seen >> key) & 1) == 0 || base + key >= limit[j >> 1]) s[n][j] = ninf;
+          }
+      }
+      float m[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+        for (int n = 1; n < NT; ++n) x = max3(x, s[n][2 * h], s[n][2 * h + 1]);
+        x *= row_scale[h];                                                         // a positive factor
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        m[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      }
+      // a maximum is renewed when it is passed by 2^8: probabilities up to 256, and sums as exact
+      const bool renew[2] = {m[0] > top[0] + 8.0f || (top[0] == ninf && m[0] > ninf), m[1] > top[1] + 8.0f || (top[1] == ninf && m[1] > ninf)};
+      if (__any_sync(0xffffffffu, renew[0] || renew[1])) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float next = renew[h] ? m[h] : top[h];
+          const float f = renew[h] ? exp2_approx(top[h] - next) : 1.0f;
+          top[h] = next;
+          sum[h] *= f;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            o[n][2 * h] *= f;
+            o[n][2 * h + 1] *= f;
+          }
+        }
+      }
+      const float nm[2] = {top[0] == ninf ? 0.0f : -top[0], top[1] == ninf ? 0.0f : -top[1]};
+      uint32_t pa[NT][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x2 f2 = pack2(row_scale[h], row_scale[h]), nm2 = pack2(nm[h], nm[h]);
+        f32x2 part = pack2(sum[h], 0.0f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float x, y;
+          unpack2(fma2(pack2(s[n][2 * h], s[n][2 * h + 1]), f2, nm2), x, y);
+          const f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
+          part = add2(part, e);
+          pa[n][h] = pair_to_sixteen<E>(e);                                        // rounded for the second product
+        }
+        float x, y;
+        unpack2(part, x, y);
+        sum[h] = x + y;
+      }
+      // ---- values
+#pragma unroll
+      for (int d = 0; d < KEYS / 16; ++d) {
+        const uint32_t a[4] = {pa[2 * d][0], pa[2 * d][1], pa[2 * d + 1][0], pa[2 * d + 1][1]};
+        if constexpr (PACKED) {
+          uint32_t vb[2][8];                                                       // [first or second eight keys][value 8g + n]
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t w[2], st[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int key = 16 * d + 8 * e + c + 4 * t;
+              const uint32_t row = src + Step::kRows + key * Step::kRow;
+              if constexpr (BITS == 4) {
+                w[t] = lds32(row + 4 * g);
+              } else if constexpr (BITS == 3) {
+                const uint32_t first = row + ((3 * g) & ~3);
+                w[t] = spread_codes<3>(__funnelshift_r(lds32(first), lds32(row + min((3 * g & ~3) + 4, 20)), 8 * ((3 * g) & 3)) & 0xFFFFFFu);
+              } else {
+                w[t] = spread_codes<2>(lds16(row + 2 * g));
+              }
+              st[t] = lds32(src + 2 * Step::kRows + Step::kStats + key * 4);
+              if (!all) st[t] = (seen >> key) & 1 ? st[t] : 0u;
+            }
+            const f32x2 center = sixteen_to_pair<__half>(__byte_perm(st[0], st[1], 0x5410)), scale = sixteen_to_pair<__half>(__byte_perm(st[0], st[1], 0x7632));
+            const uint32_t even = (w[0] & 0x0F0F0F0Fu) | ((w[1] << 4) & 0xF0F0F0F0u), odd = ((w[0] >> 4) & 0x0F0F0F0Fu) | (w[1] & 0xF0F0F0F0u);
+            vb[e][0] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<0>(even, v_column)), center));
+            vb[e][2] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<1>(even, v_column)), center));
+            vb[e][4] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<2>(even, v_column)), center));
+            vb[e][6] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<3>(even, v_column)), center));
+            vb[e][1] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<0>(odd, v_column)), center));
+            vb[e][3] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<1>(odd, v_column)), center));
+            vb[e][5] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<2>(odd, v_column)), center));
+            vb[e][7] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<3>(odd, v_column)), center));
+          }
+#pragma unroll
+          for (int n = 0; n < 8; ++n) mma_16816<E>(o[n], a, vb[0][n], vb[1][n]);
+        } else {
+          // transposed: lanes 0-7 keys 0-7, 8-15 keys 8-15, 16-31 the next eight values
+          const int row = lane & 15, ch = lane >> 4;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            uint32_t b0, b1, b2, b3;
+            ldmatrix_x4_trans(src + Step::kRows + row * 128 + (((2 * t + ch) ^ (row & 7)) << 4), b0, b1, b2, b3);
+            mma_16816<E>(o[2 * t], a, b0, b1);
+            mma_16816<E>(o[2 * t + 1], a, b2, b3);
+          }
+        }
+      }
+      __syncwarp();                                                                // the slot may be copied over
     }
-    float m[2] = {top[0], top[1]};
+    // ---- the unit, or its part.  o[n][2h + j]: row g + 8h, value 16c + 8j + n (packed), 8n + 2c + j (16 bits)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float x = ninf;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) x = fmaxf(x, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-      x *= row_scale[h];                                       // a positive factor
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-      m[h] = fmaxf(m[h], x);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
     }
-    if (__any_sync(0xffffffffu, m[0] > top[0] || m[1] > top[1])) {
+    const bool begins = at >= start, complete = begins && at + u.steps <= end;
+    if (begins && lane == 0) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, complete ? 1 : 0};
+    float* const part = split_part(p, 2 * me + (begins ? 1 : 0));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float f = m[h] == ninf ? 1.0f : exp2_approx(top[h] - m[h]);
-        top[h] = m[h];
-        sum[h] *= f;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          o[n][2 * h] *= f;
-          o[n][2 * h + 1] *= f;
-        }
-      }
-    }
-    const float nm[2] = {top[0] == ninf ? 0.0f : -top[0], top[1] == ninf ? 0.0f : -top[1]};
-    uint32_t pa[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float x = exp2_approx(fmaf(s[n][2 * h], row_scale[h], nm[h])), y = exp2_approx(fmaf(s[n][2 * h + 1], row_scale[h], nm[h]));
-        sum[h] += x + y;
-        pa[n][h] = pair_to_sixteen<E>(pack2(x, y));            // probabilities of at most 1, rounded for the second product
-      }
-    // ---- values
-#pragma unroll
-    for (int u = 0; u < KEYS / 16; ++u) {
-      uint32_t vb[2][8];                                       // [first or second eight keys][value 8g + n]
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int n = 2 * u + e;
+    for (int h = 0; h < 2; ++h) {
+      if (g + 8 * h >= u.rows) continue;
+      const int r = u.tile * kSplitRows + g + 8 * h;
+      float f = 1.0f;
+      if (complete) f = sum[h] > 0.0f ? 1.0f / sum[h] : (sum[h] == 0.0f ? 0.0f : sum[h]);      // a query that sees no key: zeros; NaN stays NaN
+      if (complete) {
+        const long long token = u.seq.first_row + r / p.group;
+        uint16_t* const dst = static_cast<uint16_t*>(p.out) + (token * p.heads + u.kvh * p.group + r % p.group) * 64;
+        auto two = [&](float x, float y) { return p.q_bf16 ? pair_to_sixteen<__nv_bfloat16>(pack2(x * f, y * f)) : pair_to_sixteen<__half>(pack2(x * f, y * f)); };
         if constexpr (PACKED) {
-          const uint32_t w0 = spread_codes<BITS>(blk.v[n][0]), w1 = spread_codes<BITS>(blk.v[n][1]);
-          f32x2 even[4], odd[4];
-          pair_levels_f32(v_table, (w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), even);
-          pair_levels_f32(v_table, ((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), odd);
-          const f32x2 center = sixteen_to_pair<__half>(__byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x5410));
-          const f32x2 scale = sixteen_to_pair<__half>(__byte_perm(blk.v_stats[n][0], blk.v_stats[n][1], 0x7632));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            vb[e][2 * j] = pair_to_sixteen<__half>(fma2(scale, even[j], center));
-            vb[e][2 * j + 1] = pair_to_sixteen<__half>(fma2(scale, odd[j], center));
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<uint4*>(dst + 16 * c + 8 * j) = make_uint4(two(o[0][2 * h + j], o[1][2 * h + j]), two(o[2][2 * h + j], o[3][2 * h + j]),
+                                                                         two(o[4][2 * h + j], o[5][2 * h + j]), two(o[6][2 * h + j], o[7][2 * h + j]));
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) *reinterpret_cast<uint32_t*>(dst + 8 * n + 2 * c) = two(o[n][2 * h], o[n][2 * h + 1]);
+        }
+      } else {
+        float* const dst = part + (g + 8 * h) * kSplitPartRow;
+        if constexpr (PACKED) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            *reinterpret_cast<float4*>(dst + 16 * c + 8 * j) = make_float4(o[0][2 * h + j], o[1][2 * h + j], o[2][2 * h + j], o[3][2 * h + j]);
+            *reinterpret_cast<float4*>(dst + 16 * c + 8 * j + 4) = make_float4(o[4][2 * h + j], o[5][2 * h + j], o[6][2 * h + j], o[7][2 * h + j]);
           }
         } else {
-          const uint4 a = blk.v[n][0], d = blk.v[n][1];
-          const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            vb[e][2 * j] = __byte_perm(x[j], y[j], 0x5410);
-            vb[e][2 * j + 1] = __byte_perm(x[j], y[j], 0x7632);
-          }
+          for (int n = 0; n < 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * c) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         }
+        if (c == 0) *reinterpret_cast<float2*>(dst + 64) = make_float2(top[h], sum[h]);
       }
-      const uint32_t a[4] = {pa[2 * u][0], pa[2 * u][1], pa[2 * u + 1][0], pa[2 * u + 1][1]};
-#pragma unroll
-      for (int n = 0; n < 8; ++n) mma_16816<E>(o[n], a, vb[0][n], vb[1][n]);
     }
-  };
+    at += u.steps;
+    if (step < end) split_next<KEYS>(p, u);
+  }
+  cp_async_wait<0>();
+}
 
-  {
-    KeyBlock<BITS> cur, next;
-    uint32_t seen = 0, seen_next = 0;
-    int step = first + warp;
-    if (step < last) load(step, cur, seen);
-    while (step < last) {
-      const int after = step + kSplitWarps;
-      if (after < last) load(after, next, seen_next);
-      compute(step, cur, seen);
-      cur = next;
-      seen = seen_next;
-      step = after;
+// Adds up the parts of the units that lie in more than one warp's piece: a block a unit; the parts are dealt out over groups of threads with
+// four values of a row each.
+constexpr int kJoinThreads = 256;
+template <int KEYS> __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
+  pdl_launch_dependents();
+  __shared__ float4 s_out[kJoinThreads];
+  __shared__ float s_max[kJoinThreads], s_sum[kJoinThreads];
+  SplitUnit u;
+  const long long unit = blockIdx.x;
+  u.tile = static_cast<int>(unit % p.tiles);
+  u.kvh = static_cast<int>(unit / p.tiles % p.kv_heads);
+  u.b = static_cast<int>(unit / p.tiles / p.kv_heads);
+  pdl_wait();
+  u.seq = attend_sequence(p, u.b);
+  if (u.tile >= split_tiles(p, u.seq)) return;
+  split_tile<KEYS>(p, u);
+  const SplitRecord rec = split_records(p)[unit];
+  if (rec.whole) return;
+  const long long piece = static_cast<SplitHeader*>(p.workspace)->piece;
+  const long long first = rec.start / piece, last = (rec.start + rec.steps - 1) / piece;
+  const int width = u.rows * 16, groups = kJoinThreads / width, group = threadIdx.x / width, e = threadIdx.x % width, r = e >> 4, c = e & 15;
+  const float ninf = __int_as_float(0xff800000);
+  float m = ninf, l = 0.0f;
+  float4 o = make_float4(0, 0, 0, 0);
+  if (group < groups) {
+    for (long long w = first + group; w <= last; w += groups) {
+      const float* const part = split_part(p, 2 * w + (rec.start >= w * piece ? 1 : 0)) + r * kSplitPartRow;
+      const float2 ml = *reinterpret_cast<const float2*>(part + 64);
+      const float4 x = *reinterpret_cast<const float4*>(part + 4 * c);
+      const float next = fmaxf(m, ml.x), base = next == ninf ? 0.0f : next, fa = exp2_approx(m - base), fb = exp2_approx(ml.x - base);
+      m = next;
+      l = l * fa + ml.y * fb;
+      o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
     }
   }
-
-  // ---- join the warps: o[n][j] is row g (+ 8), value 16c + n (j odd: + 8)
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    if (c == 0) {
-      s_max[warp][g + 8 * h] = top[h];
-      s_sum[warp][g + 8 * h] = sum[h];
-    }
-  }
-  __syncthreads();                                             // the tables are not read any more
-  float* const s_out = reinterpret_cast<float*>(smem);         // [warp][row][64]
-  float whole_max[2], whole_sum[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float m = ninf;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) m = fmaxf(m, s_max[w][g + 8 * h]);
-    whole_max[h] = m;
-    const float base = m == ninf ? 0.0f : m;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) whole_sum[h] += s_sum[w][g + 8 * h] * exp2_approx(s_max[w][g + 8 * h] - base);
-    const float f = exp2_approx(top[h] - base);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float4* const dst = reinterpret_cast<float4*>(s_out + (warp * kSplitRows + g + 8 * h) * 64 + 16 * c + 8 * j);
-      dst[0] = make_float4(o[0][2 * h + j] * f, o[1][2 * h + j] * f, o[2][2 * h + j] * f, o[3][2 * h + j] * f);
-      dst[1] = make_float4(o[4][2 * h + j] * f, o[5][2 * h + j] * f, o[6][2 * h + j] * f, o[7][2 * h + j] * f);
-    }
-    if (warp == 0 && c == 0) {
-      s_block_max[g + 8 * h] = whole_max[h];
-      s_block_sum[g + 8 * h] = whole_sum[h];
-    }
-  }
+  s_out[threadIdx.x] = o;
+  s_max[threadIdx.x] = m;
+  s_sum[threadIdx.x] = l;
   __syncthreads();
-  // the sum over the warps takes the first warp's place
-  for (int i = tid; i < kSplitRows * 64; i += kSplitThreads) {
-    float x = s_out[i];
-#pragma unroll
-    for (int w = 1; w < kSplitWarps; ++w) x += s_out[w * kSplitRows * 64 + i];
-    s_out[i] = x;
+  if (group != 0) return;
+  for (int q = 1; q < groups; ++q) m = fmaxf(m, s_max[q * width + e]);
+  const float base = m == ninf ? 0.0f : m;
+  l = 0.0f;
+  o = make_float4(0, 0, 0, 0);
+  for (int q = 0; q < groups; ++q) {
+    const float f = exp2_approx(s_max[q * width + e] - base);
+    const float4 x = s_out[q * width + e];
+    l += f * s_sum[q * width + e];
+    o = make_float4(o.x + f * x.x, o.y + f * x.y, o.z + f * x.z, o.w + f * x.w);
   }
-  // ---- join the blocks of the cluster: each writes its part of the rows
-  const bool many = p.splits > 1;
-  if (many) {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-  const int count = max(rows, 0) * 64, share = (count + p.splits - 1) / p.splits;
-  auto remote = [&](uint32_t addr, int rank) {
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-  };
-  for (int i = split * share + tid; i < min(count, (split + 1) * share); i += kSplitThreads) {
-    const int r = i >> 6;
-    float x, l;
-    if (many) {
-      float m = ninf;
-      for (int s = 0; s < p.splits; ++s) m = fmaxf(m, remote(smem_u32(s_block_max + r), s));
-      const float base = m == ninf ? 0.0f : m;
-      x = l = 0.0f;
-      for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2_approx(remote(smem_u32(s_block_max + r), s) - base);
-        l += f * remote(smem_u32(s_block_sum + r), s);
-        x += f * remote(smem_u32(s_out + i), s);
-      }
-    } else {
-      x = s_out[i];
-      l = s_block_sum[r];
-    }
-    x = l > 0.0f ? x / l : (l == 0.0f ? 0.0f : l);             // a query that sees no key: zeros; NaN stays NaN
-    const int at = tile * kSplitRows + r;
-    const long long token = seq.first_row + at / p.group;
-    const long long to = (token * p.heads + kvh * p.group + at % p.group) * 64 + (i & 63);
-    if (p.q_bf16) static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(x);
-    else static_cast<__half*>(p.out)[to] = __float2half_rn(x);
-  }
-  if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  const float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+  const int row = u.tile * kSplitRows + r;
+  const long long token = u.seq.first_row + row / p.group;
+  const long long dst = (token * p.heads + u.kvh * p.group + row % p.group) * 64 + 4 * c;
+  const f32x2 lo = pack2(o.x * f, o.y * f), hi = pack2(o.z * f, o.w * f);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + dst) =
+      p.q_bf16 ? make_uint2(pair_to_sixteen<__nv_bfloat16>(lo), pair_to_sixteen<__nv_bfloat16>(hi)) : make_uint2(pair_to_sixteen<__half>(lo), pair_to_sixteen<__half>(hi));
 }
 
 }  // namespace arcq

@@ -55,12 +55,6 @@ __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
 template <typename E> __device__ __forceinline__ uint32_t tile_idesc(int M, int N) {
   return umma_idesc_f16(M, N) | (sizeof(E) == 2 && std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
 }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool is) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 "

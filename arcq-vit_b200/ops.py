@@ -428,6 +428,11 @@ def kv_cache_read(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     return k, v
 
 
+def _workspace(size: int, device) -> torch.Tensor:
+    """Device memory for one call, given back to the caching allocator on return (under capture: the graph's own)."""
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
 def _attention_out(out, q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -466,9 +471,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise RuntimeError(f"q must have the type of the pages, {k_pages.dtype}, got {q.dtype}")
     out = _attention_out(out, q)
     with torch.cuda.device(q.device):
+        work = _workspace(lib.arcq_attention_workspace(batch, max_new, q.shape[1], c.heads), q.device)
         _check(lib.arcq_paged_attention(ctypes.byref(c), q.data_ptr(), _DT[q.dtype], q.shape[0], _strides(q), q.shape[1], batch, page_table.data_ptr(),
                                         width, lengths.data_ptr(), starts.data_ptr() if starts is not None else None, max_new, int(causal),
-                                        0.125 if scale is None else float(scale), out.data_ptr(), _stream()), "arcq_paged_attention")
+                                        0.125 if scale is None else float(scale), out.data_ptr(), work.data_ptr(), work.numel(), _stream()),
+               "arcq_paged_attention")
     return out
 
 
@@ -501,10 +508,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths=N
         stride = mask.stride(0)
     out = _attention_out(out, q)
     with torch.cuda.device(q.device):
+        work = _workspace(lib.arcq_attention_workspace(batch, queries, heads, kv_heads), q.device)
         _check(lib.arcq_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[q.dtype], batch, queries, states, heads, kv_heads,
                                         _strides(q), _strides(k), _strides(v), lengths.data_ptr() if lengths is not None else None,
                                         mask.data_ptr() if mask is not None else None, stride, 0.125 if scale is None else float(scale),
-                                        out.data_ptr(), _stream()), "arcq_cross_attention")
+                                        out.data_ptr(), work.data_ptr(), work.numel(), _stream()), "arcq_cross_attention")
     return out
 
 

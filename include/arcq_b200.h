@@ -441,19 +441,21 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
  * heads is a multiple of cache.heads: query head h reads key head h / (heads / cache.heads).  Packed keys and values are rebuilt in
  * fp16, one half-precision fma each, so |center| + 3 scale has to stay within fp16's range; products accumulate in fp32, probabilities are rounded
  * to 16 bits for the second one.  NaN and infinities in keys and values that are not seen have no effect.
+ *   workspace  arcq_attention_workspace bytes of the call's own until it has run, 16-byte aligned (NULL where that is 0)
  */
+int64_t arcq_attention_workspace(int64_t batch, int64_t max_new, int64_t heads, int64_t kv_heads);
 int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype, int64_t q_rows, const int64_t* q_strides, int64_t heads,
                          int64_t batch, const int32_t* page_table, int64_t table_width, const int32_t* lengths, const int32_t* starts,
-                         int64_t max_new, int causal, float scale, void* out, void* stream);
+                         int64_t max_new, int causal, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Attention of queries [batch, queries, heads, 64] to an encoder's states, keys and values [batch, states, kv_heads, 64], all fp16 or all
  * bf16; strides of a sequence, a token and a head in values, multiples of 8.  lengths int32 [batch] (the first of the states are seen)
- * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64]; otherwise as above.
+ * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64], a workspace for max_new = queries; otherwise as above.
  */
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
-                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* stream);
+                         const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

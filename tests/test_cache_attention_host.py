@@ -31,13 +31,13 @@ def _read(lib, c, slots=1 << 20, tokens=3, k=1 << 20, v=1 << 20, dt=1):
 
 
 def _paged(lib, c, q=1 << 20, dt=1, rows=2, qs=(256, 64), heads=4, batch=2, table=1 << 20, width=3, lengths=1 << 20, starts=None, new=1, causal=1,
-           scale=0.125, out=1 << 20):
-    return lib.arcq_paged_attention(ctypes.byref(c), q, dt, rows, _i64(*qs), heads, batch, table, width, lengths, starts, new, causal, scale, out, None)
+           scale=0.125, out=1 << 20, work=1 << 20):
+    return lib.arcq_paged_attention(ctypes.byref(c), q, dt, rows, _i64(*qs), heads, batch, table, width, lengths, starts, new, causal, scale, out, work, 1 << 20, None)
 
 
 def _cross(lib, q=1 << 20, k=1 << 20, v=1 << 20, dt=1, batch=2, queries=3, states=5, heads=4, kv=2, qs=(768, 256, 64), ks=(640, 128, 64),
-           vs=(640, 128, 64), lengths=None, mask=None, scale=0.125, out=1 << 20):
-    return lib.arcq_cross_attention(q, k, v, dt, batch, queries, states, heads, kv, _i64(*qs), _i64(*ks), _i64(*vs), lengths, mask, 5, scale, out, None)
+           vs=(640, 128, 64), lengths=None, mask=None, scale=0.125, out=1 << 20, work=1 << 20):
+    return lib.arcq_cross_attention(q, k, v, dt, batch, queries, states, heads, kv, _i64(*qs), _i64(*ks), _i64(*vs), lengths, mask, 5, scale, out, work, 1 << 20, None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -74,6 +74,7 @@ def test_attention_that_is_refused(lib, pkg):
     assert _cross(lib, dt=0) == BAD_ARG and _cross(lib, kv=3) == BAD_SHAPE and _cross(lib, queries=-1) == BAD_SHAPE and _cross(lib, states=-1) == BAD_SHAPE
     assert _cross(lib, k=None) == BAD_ARG and _cross(lib, lengths=1 << 20, mask=1 << 20) == BAD_ARG
     assert _cross(lib, v=(1 << 20) + 2) == ALIGN and _cross(lib, ks=(641, 128, 64)) == ALIGN
+    assert _paged(lib, c, work=(1 << 20) + 8) == ALIGN and _cross(lib, work=(1 << 20) + 4) == ALIGN
     assert _cross(lib, batch=0) == 0 and _cross(lib, queries=0) == 0
 
 

@@ -93,6 +93,18 @@ template <> __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same without an accumulator
+template <typename E> __device__ __forceinline__ void mma_16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma_16816_first<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+template <> __device__ __forceinline__ void mma_16816_first<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -161,15 +173,16 @@ __device__ __forceinline__ void pair_levels_f32(uint32_t table, uint32_t w, f32x
 }
 
 // ---------------------------------------------------------------- shared memory of split_attention_kernel
-// Packed: the tables at shared address 64 KB, 256 bytes a byte of codes: 32 copies of its pair of fp16 levels (keys), 16 of fp32 levels
-// (values); the warps' rings below and above.
+// Packed: a table at shared address 64 KB, 256 bytes for each pair of codes: 32 copies of its levels for keys, 32 for values (fp16); the warps'
+// rings below and above.
 constexpr uint32_t kSplitTable = 0x10000, kSplitTableEnd = 0x20000;
 template <int BITS> struct SplitStep {
   static constexpr int kKeys = BITS == 16 ? 16 : 32;
   static constexpr uint32_t kRow = BITS == 16 ? 128 : 8 * BITS;
-  static constexpr uint32_t kRows = kKeys * kRow;                                 // keys, or values
+  static constexpr uint32_t kPad = BITS == 16 ? 0 : 32;                           // behind each 8 rows, so that reads have no bank conflicts
+  static constexpr uint32_t kRows = kKeys * kRow + kKeys / 8 * kPad;              // keys, or values
   static constexpr uint32_t kStats = BITS == 16 ? 0 : 4 * kKeys;                  // likewise
-  static constexpr uint32_t kBytes = 2 * (kRows + kStats) + 16;      // and which keys are seen
+  static constexpr uint32_t kBytes = 2 * (kRows + kStats);
   static constexpr uint32_t kRing = kSplitStages * kBytes;
 };
 // `base`: where the block's shared memory starts; rings of warps that do not fit below the table lie above it
@@ -183,6 +196,35 @@ template <int BITS> __host__ __device__ constexpr uint32_t split_ring(uint32_t b
 constexpr uint32_t kSplitBase = 8192;
 template <int BITS> constexpr uint32_t split_smem() {
   return BITS == 16 ? kSplitWarps * SplitStep<16>::kRing + 128 : split_ring<BITS>(kSplitBase, kSplitWarps);
+}
+// A level in fp16, rounded up in a share of the copies that is the position between its neighbours: the copies of lanes 4g + c, low and high,
+// serve different keys (values) or parts of a head (keys), over which the roundings then average out.
+__device__ __forceinline__ __half dithered_level(float x, int eighth) {
+  const __half down = __float2half_rd(x), up = __float2half_ru(x);
+  const float a = __half2float(down), b = __half2float(up);
+  return (x - a) * 16.0f > (b - a) * (2 * eighth + 1) ? up : down;
+}
+// Entry i of the table: codes i & (levels - 1) and i >> BITS.  512 threads.
+template <int BITS> __device__ __forceinline__ void fill_split_table(const float* codebooks, int tid) {
+  constexpr int LEVELS = 1 << BITS;
+  const int entry = tid >> 1, values = tid & 1;
+  if (entry >= LEVELS * LEVELS) return;
+  const float lo = __ldg(codebooks + values * LEVELS + (entry & (LEVELS - 1))), hi = __ldg(codebooks + values * LEVELS + (entry >> BITS));
+  uint32_t w[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const __half2 h = __halves2half2(dithered_level(lo, 2 * c), dithered_level(hi, 2 * c + 1));
+    w[c] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sts128(kSplitTable + entry * 256 + values * 128 + ((r + (tid >> 1)) & 7) * 16, w[0], w[1], w[2], w[3]);
+}
+// Address of entry I of the four whose numbers lie side by side in x (2 * BITS bits each); `column` is in the low byte, and the table's.
+template <int BITS, int I> __device__ __forceinline__ uint32_t table_address(uint32_t x, uint32_t column) {
+  if (BITS == 4) return __byte_perm(x, column, 0x7604 | (I << 4));
+  constexpr int at = 2 * BITS * I;
+  constexpr uint32_t mask = ((1u << (2 * BITS)) - 1) << 8;
+  return ((at <= 8 ? x << (at <= 8 ? 8 - at : 0) : x >> (at > 8 ? at - 8 : 0)) & mask) | column;
 }
 
 // ---------------------------------------------------------------- units and their line
@@ -262,9 +304,6 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// byte i of w into bits 8-15 of a table address
-template <int I> __device__ __forceinline__ uint32_t table_address(uint32_t w, uint32_t column) { return __byte_perm(w, column, 0x7604 | (I << 4)); }
-
 template <int BITS, typename E>
 __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const __grid_constant__ AttendParams p) {
   pdl_launch_dependents();
@@ -274,21 +313,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kSplitThreads / 32], s_line[kSplitThreads];         // steps before each share of the sequences
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  if constexpr (PACKED) {
-    // 16-byte columns of the table: 8 of keys, 8 of values
-    const float *kl = p.codebooks, *vl = p.codebooks + (1 << BITS);
-    for (int i = tid; i < 256 * 16; i += kSplitThreads) {
-      const int byte = i >> 4, a = min(byte & 15, (1 << BITS) - 1), b = min(byte >> 4, (1 << BITS) - 1);
-      const uint32_t dst = kSplitTable + byte * 256 + (i & 15) * 16;
-      if ((i & 8) == 0) {
-        const uint32_t w = pair_to_sixteen<__half>(pack2(__ldg(kl + a), __ldg(kl + b)));
-        sts128(dst, w, w, w, w);
-      } else {
-        const uint32_t lo = __float_as_uint(__ldg(vl + a)), hi = __float_as_uint(__ldg(vl + b));
-        sts128(dst, lo, hi, lo, hi);
-      }
-    }
-  }
+  if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid);
   pdl_wait();
 
   // ---- the line of steps: each thread a share of the sequences, a scan over the block
@@ -353,90 +378,108 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   }
 
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
-  // ---- copies, ahead of the computation
-  SplitUnit f = u;                                                                 // where the next step to be copied is
-  int f_step = static_cast<int>(start - at);
-  long long f_left = end - start;
-  int page[KEYS / 16], f_slot = 0;                                                 // pages of its sixteens of keys; < 0: none
-  bool f_masked = true;
-  auto look_up = [&]() {
-#pragma unroll
-    for (int h = 0; h < KEYS / 16; ++h) {
-      const int key = f_step * KEYS + 16 * h;
-      page[h] = key < f.keys ? f.b : -1;
-      if (p.table != nullptr && key < f.keys) page[h] = p.table[static_cast<long long>(f.b) * p.table_width + (key >> p.page_shift)];
-    }
-    if (!PACKED && p.mask != nullptr) {
-      const int key = f_step * KEYS + (lane & 15);
-      f_masked = key < f.keys && p.mask[f.b * p.mask_stride + key] != 0;
-    }
+  // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest
+  // of a page, or of an image's states; the page after it is looked up when it begins.
+  SplitUnit f = u;
+  int f_step = static_cast<int>(start - at), f_left = static_cast<int>(end - start), f_slot = 0;
+  int run = 0, next_page = 0;                                                      // sixteens of the run that are left
+  bool valid = false, masked = true;
+  const uint8_t *fk = p.k.rows, *fv = p.v.rows, *fs = reinterpret_cast<const uint8_t*>(p.k.stats);      // the lane's 16 bytes of the next sixteen
+  auto look_up = [&](int key) {
+    next_page = f.b;
+    if (p.table != nullptr && key < f.keys) next_page = p.table[static_cast<long long>(f.b) * p.table_width + (key >> p.page_shift)];
   };
-  look_up();
+  auto mask_ahead = [&](int key) {
+    if (!PACKED && p.mask != nullptr) masked = key + (lane & 15) < f.keys && p.mask[f.b * p.mask_stride + key + (lane & 15)] != 0;
+  };
+  auto begin_run = [&](int key) {
+    const int page = next_page, size = p.table != nullptr ? 1 << p.page_shift : 0x7ffffff0, in = key & (size - 1);
+    const int place = p.table != nullptr ? in : key, left = (f.keys - key + 15) >> 4;
+    run = p.table != nullptr ? min((size - in) >> 4, left) : left;
+    valid = p.table == nullptr || (page >= 0 && page < p.pages);
+    if (PACKED) {
+      const long long row = valid ? ((static_cast<long long>(page) * p.kv_heads + f.kvh) << p.page_shift) + place : 0;
+      fk = p.k.rows + row * Step::kRow + lane * 16;
+      fv = p.v.rows + row * Step::kRow + lane * 16;
+      fs = reinterpret_cast<const uint8_t*>((lane & 4 ? p.v.stats : p.k.stats) + row) + (lane & 3) * 16;
+    } else {
+      const long long blk = valid ? page : 0, row = valid ? place + (lane >> 3) : 0;
+      fk = p.k.rows + blk * p.k.block_stride + f.kvh * p.k.head_stride + row * p.k.token_stride + (lane & 7) * 16;
+      fv = p.v.rows + blk * p.v.block_stride + f.kvh * p.v.head_stride + row * p.v.token_stride + (lane & 7) * 16;
+    }
+    look_up(key + run * 16);
+  };
+  look_up(f_step * KEYS);
+  mask_ahead(f_step * KEYS);
+  // returns which of the step's keys are seen
   auto copy_step = [&]() {
+    uint32_t seen = 0;
     if (f_left > 0) {
       const uint32_t dst = ring + f_slot * Step::kBytes;
-      const int base = f_step * KEYS;
-      const int in_page = p.table != nullptr ? (1 << p.page_shift) - 1 : 0x7fffffff;
-      bool there[KEYS / 16];
 #pragma unroll
-      for (int h = 0; h < KEYS / 16; ++h) there[h] = page[h] >= 0 && (p.table == nullptr || page[h] < p.pages);
-      if constexpr (PACKED) {
-        // sixteen rows of a page lie side by side
-        constexpr int CHUNKS = 8 * BITS;                                           // of 16 bytes, in sixteen rows
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const long long row = ((static_cast<long long>(page[h]) * p.kv_heads + f.kvh) << p.page_shift) + ((base + 16 * h) & in_page);
+      for (int h = 0; h < KEYS / 16; ++h) {
+        const int key = f_step * KEYS + 16 * h, left = f.keys - key;
+        if (run == 0 && left > 0) begin_run(key);
+        const bool is = valid && left > 0;
+        uint32_t half = !is ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u;
+        if constexpr (PACKED) {
+          constexpr int CHUNKS = 8 * BITS;                                         // of 16 bytes, in sixteen rows
+          const uint32_t to = dst + h * (16 * Step::kRow + 2 * Step::kPad) + lane * 16 + (lane >= CHUNKS / 2 ? Step::kPad : 0);
           if (lane < CHUNKS) {
-            cp_async_16(dst + h * 16 * Step::kRow + lane * 16, p.k.rows + (there[h] ? row * Step::kRow + lane * 16 : 0), there[h]);
-            cp_async_16(dst + Step::kRows + h * 16 * Step::kRow + lane * 16, p.v.rows + (there[h] ? row * Step::kRow + lane * 16 : 0), there[h]);
+            cp_async_16(to, fk, is);
+            cp_async_16(to + Step::kRows, fv, is);
           }
-          if (lane < 8) {
-            const __half2* const st = lane < 4 ? p.k.stats : p.v.stats;
-            cp_async_16(dst + 2 * Step::kRows + (lane >> 2) * Step::kStats + h * 64 + (lane & 3) * 16, st + (there[h] ? row + (lane & 3) * 4 : 0), there[h]);
-          }
-        }
-        const uint32_t seen = __ballot_sync(0xffffffffu, base + lane < f.keys && (lane < 16 ? there[0] : there[KEYS / 16 - 1]));
-        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + Step::kBytes - 16), "r"(seen) : "memory");
-      } else {
-        const int place = base & in_page;
-        const bool is = there[0] && base + (lane & 15) < f.keys && f_masked;
-        const uint32_t seen = __ballot_sync(0xffffffffu, is) & 0xFFFFu;
-        const uint8_t* const k = p.k.rows + page[0] * p.k.block_stride + f.kvh * p.k.head_stride + place * p.k.token_stride;
-        const uint8_t* const v = p.v.rows + page[0] * p.v.block_stride + f.kvh * p.v.head_stride + place * p.v.token_stride;
+          if (lane < 8) cp_async_16(dst + 2 * Step::kRows + (lane >> 2) * Step::kStats + h * 64 + (lane & 3) * 16, fs, is);
+          fk += 16 * Step::kRow;
+          fv += 16 * Step::kRow;
+          fs += 64;
+        } else {
+          if (p.mask != nullptr) half &= __ballot_sync(0xffffffffu, masked);
+          const uint32_t to = dst + (lane >> 3) * 128;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 4 * r + (lane >> 3), ch = lane & 7;
-          const bool sees = (seen >> row) & 1;
-          const uint32_t to = dst + row * 128 + ((ch ^ (row & 7)) << 4);
-          cp_async_16(to, sees ? k + row * p.k.token_stride + 16 * ch : p.k.rows, sees);
-          cp_async_16(to + Step::kRows, sees ? v + row * p.v.token_stride + 16 * ch : p.v.rows, sees);
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t at = to + r * 512 + (((lane & 7) ^ ((4 * r + (lane >> 3)) & 7)) << 4);
+            const bool sees = (half >> (4 * r + (lane >> 3))) & 1;
+            cp_async_16(at, fk + r * 4 * p.k.token_stride, sees);
+            cp_async_16(at + Step::kRows, fv + r * 4 * p.v.token_stride, sees);
+          }
+          fk += 16 * p.k.token_stride;
+          fv += 16 * p.v.token_stride;
         }
-        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + Step::kBytes - 16), "r"(seen) : "memory");
+        run -= left > 0 ? 1 : 0;
+        seen |= half << (16 * h);
       }
       f_slot = f_slot + 1 == kSplitStages ? 0 : f_slot + 1;
       if (--f_left > 0) {
         if (++f_step == f.steps) {
           split_next<KEYS>(p, f);
-          f_step = 0;
+          f_step = run = 0;
+          look_up(0);
         }
-        look_up();
+        mask_ahead(f_step * KEYS);
       }
     }
     cp_async_commit();
+    return seen;
   };
-  copy_step();
-  copy_step();
+  uint32_t seen_now, seen_next = copy_step(), seen_after = copy_step();
 
   // ---- units
+  // Which key the columns of the 8-wide products are: packed, column 2c + j of tile n is key 8c + (n & 1) + 2j + 4 (n >> 1), so that a lane's eight
+  // keys lie side by side and reads of rows have no bank conflicts; 16 bits, 8n + 2c + j.
   const float ninf = __int_as_float(0xff800000);
-  const uint32_t k_column = kSplitTable + lane * 4, v_column = kSplitTable + 128 + (lane & 15) * 8;
-  long long step = start;
-  int slot = 0;
-  while (step < end) {
+  constexpr auto key_in_eight = [](int n, int j) { return (n & 1) + 2 * j + 4 * (n >> 1); };
+  const uint32_t k_column = kSplitTable + lane * 4, v_column = k_column + 128;
+  const uint32_t k_lane = (g >> 1) * (8 * Step::kRow + Step::kPad) + 2 * (g & 1) * Step::kRow;
+  const uint32_t v_lane = Step::kRows + c * (8 * Step::kRow + Step::kPad);
+  int step = 0, slot = 0;                                                          // of the piece
+  const int steps = static_cast<int>(end - start);
+  while (step < steps) {
     // rows g and g + 8 of the unit: queries, the keys that they see, the factor of their scores
+    const bool both = u.rows > 8;                                                  // the upper eight are there
     int limit[2];
     uint32_t qa[4][4];
-    float row_scale[2] = {p.scale_log2, p.scale_log2};
+    float row_scale[2] = {p.scale_log2, p.scale_log2}, q_sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool row = g + 8 * h < u.rows;
@@ -457,6 +500,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           row_scale[h] *= bf16_to_half(w, 8, top);
         }
+        f32x2 q2 = pack2(0.0f, 0.0f);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) q2 = add2(q2, sixteen_to_pair<__half>(w[n]));
+        float x, y;
+        unpack2(q2, x, y);
+        x += y;
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        q_sum[h] = x + __shfl_xor_sync(0xffffffffu, x, 2);
       } else {                                                                     // values 8n + 2c and the next
 #pragma unroll
         for (int n = 0; n < 8; ++n) w[n] = row ? *reinterpret_cast<const uint32_t*>(src + 8 * n + 2 * c) : 0u;
@@ -467,56 +518,73 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         qa[s][2 + h] = w[2 * s + 1];
       }
     }
-    float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {};
-    const long long unit_end = min(at + u.steps, end);
+    // packed: o holds sum p (scale / 2^e) level, v_inverse = 2^-e (0: none yet), centers the sum of p * center
+    float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {}, centers[2] = {0.0f, 0.0f}, v_inverse = 0.0f;
+    const int unit_first = static_cast<int>(max(at - start, -0x40000000ll)), unit_last = static_cast<int>(min(at + u.steps, end) - start);
+    const int key_base = static_cast<int>((start - at) * KEYS);                    // key of step s: key_base + s * KEYS
 #pragma unroll 1
-    for (; step < unit_end; ++step) {
-      copy_step();
+    for (; step < unit_last; ++step) {
+      seen_now = seen_next;
+      seen_next = seen_after;
+      seen_after = copy_step();
       cp_async_wait<2>();
       __syncwarp();
-      const uint32_t src = ring + slot * Step::kBytes;
+      const uint32_t src = ring + slot * Step::kBytes, seen = seen_now;
       slot = slot + 1 == kSplitStages ? 0 : slot + 1;
-      const int base = static_cast<int>(step - at) * KEYS;
-      // ---- scores.  Column 2c + j of a tile of 8 keys is key c + 4j (packed; so reads of values have no bank conflicts), in 16 bits key 2c + j.
-      const uint32_t seen = lds32(src + Step::kBytes - 16);
+      const int base = key_base + step * KEYS;
       const bool all = seen == (KEYS == 32 ? 0xffffffffu : 0xffffu);
+      // ---- scores
       float s[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+      uint32_t vst[8];                                                             // center and scale of the lane's eight values
       if constexpr (PACKED) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const int key = 8 * n + (g >> 1) + 4 * (g & 1);
-          const uint32_t row = src + key * Step::kRow;
+          const uint32_t row = src + k_lane + key_in_eight(n, 0) * Step::kRow;
           uint32_t lo, hi;
           if constexpr (BITS == 4) {
             const uint2 w = lds64(row + 8 * c);
             lo = w.x; hi = w.y;
           } else if constexpr (BITS == 3) {
-            const uint32_t first = row + ((6 * c) & ~3), w0 = lds32(first), w1 = lds32(first + 4), sh = (c & 1) * 16;
-            lo = spread_codes<3>(__funnelshift_r(w0, w1, sh) & 0xFFFFFFu);
-            hi = spread_codes<3>((c & 1 ? w1 >> 8 : __funnelshift_r(w0, w1, 24)) & 0xFFFFFFu);
+            const uint32_t first = row + ((6 * c) & ~3), w0 = lds32(first), w1 = lds32(first + 4);
+            lo = __funnelshift_r(w0, w1, (c & 1) * 16);
+            hi = __funnelshift_r(c & 1 ? w1 : w0, c & 1 ? 0u : w1, c & 1 ? 8 : 24);
           } else {
-            const uint32_t w = lds32(row + 4 * c);
-            lo = spread_codes<2>(w & 0xFFFFu);
-            hi = spread_codes<2>(w >> 16);
+            lo = lds32(row + 4 * c);
+            hi = lo >> 16;
           }
-          uint32_t stats = lds32(src + 2 * Step::kRows + key * 4);
-          if (!all) stats = (seen >> key) & 1 ? stats : 0u;                        // whatever lies there: x = 0
-          const uint32_t center = __byte_perm(stats, 0, 0x1010), scale = __byte_perm(stats, 0, 0x3232);
-          uint32_t kb[8];
-          kb[0] = half2_fma(scale, lds_const_u32(table_address<0>(lo, k_column)), center);
-          kb[1] = half2_fma(scale, lds_const_u32(table_address<1>(lo, k_column)), center);
-          kb[2] = half2_fma(scale, lds_const_u32(table_address<2>(lo, k_column)), center);
-          kb[3] = half2_fma(scale, lds_const_u32(table_address<3>(lo, k_column)), center);
-          kb[4] = half2_fma(scale, lds_const_u32(table_address<0>(hi, k_column)), center);
-          kb[5] = half2_fma(scale, lds_const_u32(table_address<1>(hi, k_column)), center);
-          kb[6] = half2_fma(scale, lds_const_u32(table_address<2>(hi, k_column)), center);
-          kb[7] = half2_fma(scale, lds_const_u32(table_address<3>(hi, k_column)), center);
+          const uint32_t b0 = lds_const_u32(table_address<BITS, 0>(lo, k_column)), b1 = lds_const_u32(table_address<BITS, 1>(lo, k_column));
+          const uint32_t b2 = lds_const_u32(table_address<BITS, 2>(lo, k_column)), b3 = lds_const_u32(table_address<BITS, 3>(lo, k_column));
+          const uint32_t b4 = lds_const_u32(table_address<BITS, 0>(hi, k_column)), b5 = lds_const_u32(table_address<BITS, 1>(hi, k_column));
+          const uint32_t b6 = lds_const_u32(table_address<BITS, 2>(hi, k_column)), b7 = lds_const_u32(table_address<BITS, 3>(hi, k_column));
+          mma_16816_first<E>(s[n], qa[0], b0, b1);
+          mma_16816<E>(s[n], qa[1], b2, b3);
+          mma_16816<E>(s[n], qa[2], b4, b5);
+          mma_16816<E>(s[n], qa[3], b6, b7);
+        }
+        // q . k = scale * (q . level) + center * sum q
+        const uint32_t stats = src + 2 * Step::kRows + c * 32;
+        const uint4 k0 = lds128(stats), k1 = lds128(stats + 16), v0 = lds128(stats + Step::kStats), v1 = lds128(stats + Step::kStats + 16);
+        uint32_t kst[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+        vst[0] = v0.x; vst[1] = v0.y; vst[2] = v0.z; vst[3] = v0.w; vst[4] = v1.x; vst[5] = v1.y; vst[6] = v1.z; vst[7] = v1.w;
+        if (!all) {                                                                // whatever lies behind the last key: 0
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma_16816<E>(s[n], qa[t], kb[2 * t], kb[2 * t + 1]);
+          for (int j = 0; j < 8; ++j) {
+            const bool is = (seen >> (8 * c + j)) & 1;
+            kst[j] = is ? kst[j] : 0u;
+            vst[j] = is ? vst[j] : 0u;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float c0, s0, c1, s1;
+          unpack2(sixteen_to_pair<__half>(kst[key_in_eight(n, 0)]), c0, s0);
+          unpack2(sixteen_to_pair<__half>(kst[key_in_eight(n, 1)]), c1, s1);
+          const f32x2 scale = pack2(s0, s1), center = pack2(c0, c1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !both) continue;
+            unpack2(fma2(pack2(s[n][2 * h], s[n][2 * h + 1]), scale, mul2(center, pack2(q_sum[h], q_sum[h]))), s[n][2 * h], s[n][2 * h + 1]);
+          }
         }
       } else {
         // matrices of 8 keys x 8 values: lanes 0-7 keys 0-7, 8-15 the next eight values, 16-31 keys 8-15
@@ -525,8 +593,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         for (int t = 0; t < 4; ++t) {
           uint32_t b0, b1, b2, b3;
           ldmatrix_x4(src + row * 128 + (((2 * t + ch) ^ (row & 7)) << 4), b0, b1, b2, b3);
-          mma_16816<E>(s[0], qa[t], b0, b1);
-          mma_16816<E>(s[1], qa[t], b2, b3);
+          if (t == 0) {
+            mma_16816_first<E>(s[0], qa[t], b0, b1);
+            mma_16816_first<E>(s[1], qa[t], b2, b3);
+          } else {
+            mma_16816<E>(s[0], qa[t], b0, b1);
+            mma_16816<E>(s[1], qa[t], b2, b3);
+          }
         }
       }
       // ---- softmax: lane 4g + c has rows g and g + 8
@@ -535,13 +608,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int key = 8 * n + (PACKED ? c + 4 * (j & 1) : 2 * c + (j & 1));
+            const int key = PACKED ? 8 * c + key_in_eight(n, j & 1) : 8 * n + 2 * c + (j & 1);
             if (((seen >> key) & 1) == 0 || base + key >= limit[j >> 1]) s[n][j] = ninf;
           }
       }
-      float m[2];
+      float m[2] = {ninf, ninf};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !both) continue;
         float x = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
         for (int n = 1; n < NT; ++n) x = max3(x, s[n][2 * h], s[n][2 * h + 1]);
@@ -558,6 +632,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           const float f = renew[h] ? exp2_approx(top[h] - next) : 1.0f;
           top[h] = next;
           sum[h] *= f;
+          centers[h] *= f;
 #pragma unroll
           for (int n = 0; n < 8; ++n) {
             o[n][2 * h] *= f;
@@ -565,23 +640,56 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           }
         }
       }
-      const float nm[2] = {top[0] == ninf ? 0.0f : -top[0], top[1] == ninf ? 0.0f : -top[1]};
+      // packed: the values' scales go into the probabilities, relative to a power of two that is renewed when a scale passes it by 2^4
+      if constexpr (PACKED) {
+        uint32_t largest = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) largest = max(largest, vst[j] >> 16);
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        const float v_scale = __half2float(__ushort_as_half(static_cast<unsigned short>(largest)));
+        if (v_scale * v_inverse > 16.0f || (v_inverse == 0.0f && largest != 0u)) {
+          const float next = __int_as_float(0x7F000000 - (__float_as_int(v_scale) & 0x7F800000));
+          const float f = next / (v_inverse == 0.0f ? next : v_inverse);
+          v_inverse = next;
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][j] *= f;
+        }
+      }
       uint32_t pa[NT][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x2 f2 = pack2(row_scale[h], row_scale[h]), nm2 = pack2(nm[h], nm[h]);
-        f32x2 part = pack2(sum[h], 0.0f);
+        if (h == 1 && !both) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) pa[n][1] = 0u;
+          continue;
+        }
+        const float nm = top[h] == ninf ? 0.0f : -top[h];
+        const f32x2 f2 = pack2(row_scale[h], row_scale[h]), nm2 = pack2(nm, nm), inv2 = pack2(v_inverse, v_inverse);
+        f32x2 part = pack2(sum[h], 0.0f), part_c = pack2(centers[h], 0.0f);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float x, y;
           unpack2(fma2(pack2(s[n][2 * h], s[n][2 * h + 1]), f2, nm2), x, y);
-          const f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
+          f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
           part = add2(part, e);
+          if constexpr (PACKED) {
+            float c0, s0, c1, s1;
+            unpack2(sixteen_to_pair<__half>(vst[key_in_eight(n, 0)]), c0, s0);
+            unpack2(sixteen_to_pair<__half>(vst[key_in_eight(n, 1)]), c1, s1);
+            part_c = fma2(e, pack2(c0, c1), part_c);
+            e = mul2(e, mul2(pack2(s0, s1), inv2));
+          }
           pa[n][h] = pair_to_sixteen<E>(e);                                        // rounded for the second product
         }
         float x, y;
         unpack2(part, x, y);
         sum[h] = x + y;
+        if constexpr (PACKED) {
+          unpack2(part_c, x, y);
+          centers[h] = x + y;
+        }
       }
       // ---- values
 #pragma unroll
@@ -591,32 +699,30 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           uint32_t vb[2][8];                                                       // [first or second eight keys][value 8g + n]
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t w[2], st[2];
+            uint32_t w[2], even, odd;                                              // numbers of pairs of the two keys' codes
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int key = 16 * d + 8 * e + c + 4 * t;
-              const uint32_t row = src + Step::kRows + key * Step::kRow;
+              const uint32_t row = src + v_lane + key_in_eight(2 * d + e, t) * Step::kRow;
               if constexpr (BITS == 4) {
                 w[t] = lds32(row + 4 * g);
               } else if constexpr (BITS == 3) {
                 const uint32_t first = row + ((3 * g) & ~3);
-                w[t] = spread_codes<3>(__funnelshift_r(lds32(first), lds32(row + min((3 * g & ~3) + 4, 20)), 8 * ((3 * g) & 3)) & 0xFFFFFFu);
+                w[t] = __funnelshift_r(lds32(first), lds32(row + min((3 * g & ~3) + 4, 20)), 8 * ((3 * g) & 3));
               } else {
-                w[t] = spread_codes<2>(lds16(row + 2 * g));
+                w[t] = lds16(row + 2 * g);
               }
-              st[t] = lds32(src + 2 * Step::kRows + Step::kStats + key * 4);
-              if (!all) st[t] = (seen >> key) & 1 ? st[t] : 0u;
             }
-            const f32x2 center = sixteen_to_pair<__half>(__byte_perm(st[0], st[1], 0x5410)), scale = sixteen_to_pair<__half>(__byte_perm(st[0], st[1], 0x7632));
-            const uint32_t even = (w[0] & 0x0F0F0F0Fu) | ((w[1] << 4) & 0xF0F0F0F0u), odd = ((w[0] >> 4) & 0x0F0F0F0Fu) | (w[1] & 0xF0F0F0F0u);
-            vb[e][0] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<0>(even, v_column)), center));
-            vb[e][2] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<1>(even, v_column)), center));
-            vb[e][4] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<2>(even, v_column)), center));
-            vb[e][6] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<3>(even, v_column)), center));
-            vb[e][1] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<0>(odd, v_column)), center));
-            vb[e][3] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<1>(odd, v_column)), center));
-            vb[e][5] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<2>(odd, v_column)), center));
-            vb[e][7] = pair_to_sixteen<__half>(fma2(scale, lds_const_pair(table_address<3>(odd, v_column)), center));
+            constexpr uint32_t M = BITS == 4 ? 0x0F0F0F0Fu : BITS == 3 ? 0x001C71C7u : 0x3333u;      // codes 0, 2, 4, 6
+            even = (w[0] & M) | ((w[1] << (BITS & 7)) & (M << (BITS & 7)));
+            odd = ((w[0] >> (BITS & 7)) & M) | (w[1] & (M << (BITS & 7)));
+            vb[e][0] = lds_const_u32(table_address<BITS, 0>(even, v_column));
+            vb[e][2] = lds_const_u32(table_address<BITS, 1>(even, v_column));
+            vb[e][4] = lds_const_u32(table_address<BITS, 2>(even, v_column));
+            vb[e][6] = lds_const_u32(table_address<BITS, 3>(even, v_column));
+            vb[e][1] = lds_const_u32(table_address<BITS, 0>(odd, v_column));
+            vb[e][3] = lds_const_u32(table_address<BITS, 1>(odd, v_column));
+            vb[e][5] = lds_const_u32(table_address<BITS, 2>(odd, v_column));
+            vb[e][7] = lds_const_u32(table_address<BITS, 3>(odd, v_column));
           }
 #pragma unroll
           for (int n = 0; n < 8; ++n) mma_16816<E>(o[n], a, vb[0][n], vb[1][n]);
@@ -639,17 +745,25 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     for (int h = 0; h < 2; ++h) {
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      if constexpr (PACKED) {
+        centers[h] += __shfl_xor_sync(0xffffffffu, centers[h], 1);
+        centers[h] += __shfl_xor_sync(0xffffffffu, centers[h], 2);
+        const float up = v_inverse == 0.0f ? 0.0f : 1.0f / v_inverse;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) o[n][2 * h + j] = fmaf(o[n][2 * h + j], up, centers[h]);
+      }
     }
-    const bool begins = at >= start, complete = begins && at + u.steps <= end;
+    const bool begins = unit_first >= 0, complete = begins && at + u.steps <= end;
     if (begins && lane == 0) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, complete ? 1 : 0};
     float* const part = split_part(p, 2 * me + (begins ? 1 : 0));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (g + 8 * h >= u.rows) continue;
       const int r = u.tile * kSplitRows + g + 8 * h;
-      float f = 1.0f;
-      if (complete) f = sum[h] > 0.0f ? 1.0f / sum[h] : (sum[h] == 0.0f ? 0.0f : sum[h]);      // a query that sees no key: zeros; NaN stays NaN
       if (complete) {
+        const float f = sum[h] > 0.0f ? 1.0f / sum[h] : (sum[h] == 0.0f ? 0.0f : sum[h]);      // a query that sees no key: zeros; NaN stays NaN
         const long long token = u.seq.first_row + r / p.group;
         uint16_t* const dst = static_cast<uint16_t*>(p.out) + (token * p.heads + u.kvh * p.group + r % p.group) * 64;
         auto two = [&](float x, float y) { return p.q_bf16 ? pair_to_sixteen<__nv_bfloat16>(pack2(x * f, y * f)) : pair_to_sixteen<__half>(pack2(x * f, y * f)); };
@@ -678,7 +792,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     at += u.steps;
-    if (step < end) split_next<KEYS>(p, u);
+    if (step < steps) split_next<KEYS>(p, u);
   }
   cp_async_wait<0>();
 }

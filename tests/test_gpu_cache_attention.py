@@ -1,7 +1,8 @@
 """The paged key/value cache, attention over it and attention to an encoder's states, against plain evaluations in 64 bits.
 
 Bounds of the attentions, per output, are those of the roundings that the kernels make (u = 2^-11 for fp16, 2^-8 for bf16):
-  packed keys and values   a level rounded to fp16, then one fma: u16 * (|scale * level| + |x|) each
+  packed keys and values   a level rounded to fp16, up or down (two half steps), or to the nearest with one fma behind it:
+                           u16 * (2 |scale * level| + |x|) at most; center and scale * level come together in fp32, 2^-20 of the center
   a score                  the keys' errors times |q|, and 64 products summed in fp32 (2^-23 each, the tensor cores may truncate)
   a weight                 twice the largest score error of the row, the exponential (2^-20 with its argument), one rounding to 16 bits
                            (in fp16 2^-25 at least) before the second product
@@ -45,7 +46,7 @@ def _cached(pkg, c, which, rows):
     st = c[which + "_stats"][rows[:, 0], :, rows[:, 1]].double()
     part = st[..., 1:] * c["codebooks"][i].double()[codes]
     x = st[..., :1] + part
-    return x, U[torch.float16] * (part.abs() + x.abs())
+    return x, U[torch.float16] * (2 * part.abs() + x.abs()) + 2.0 ** -20 * st[..., :1].abs()
 
 
 def _attend(q, k, dk, v, dv, seen, scale, dtype, packed):

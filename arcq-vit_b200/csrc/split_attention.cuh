@@ -131,7 +131,10 @@ __device__ __forceinline__ float bf16_to_half(uint32_t* w, int n, float top) {
   return __int_as_float((127 - up) << 23);
 }
 
-constexpr int kSplitWarps = 16, kSplitThreads = kSplitWarps * 32, kSplitRows = 16, kSplitStages = 3;
+#ifndef SPLIT_WARPS
+#define SPLIT_WARPS 12
+#endif
+constexpr int kSplitWarps = SPLIT_WARPS, kSplitThreads = kSplitWarps * 32, kSplitRows = 16, kSplitStages = 3;
 constexpr uint32_t kPairTableBytes = 256 * 32 * 4;                  // [byte][lane]
 
 // [byte][lane]: the levels of the byte's two codes, low nibble first
@@ -204,20 +207,21 @@ __device__ __forceinline__ __half dithered_level(float x, int eighth) {
   const float a = __half2float(down), b = __half2float(up);
   return (x - a) * 16.0f > (b - a) * (2 * eighth + 1) ? up : down;
 }
-// Entry i of the table: codes i & (levels - 1) and i >> BITS.  512 threads.
-template <int BITS> __device__ __forceinline__ void fill_split_table(const float* codebooks, int tid) {
+// Entry i of the table: codes i & (levels - 1) and i >> BITS.
+template <int BITS> __device__ __forceinline__ void fill_split_table(const float* codebooks, int tid, int threads) {
   constexpr int LEVELS = 1 << BITS;
-  const int entry = tid >> 1, values = tid & 1;
-  if (entry >= LEVELS * LEVELS) return;
-  const float lo = __ldg(codebooks + values * LEVELS + (entry & (LEVELS - 1))), hi = __ldg(codebooks + values * LEVELS + (entry >> BITS));
-  uint32_t w[4];
+  for (int i = tid; i < 2 * LEVELS * LEVELS; i += threads) {
+    const int entry = i >> 1, values = i & 1;
+    const float lo = __ldg(codebooks + values * LEVELS + (entry & (LEVELS - 1))), hi = __ldg(codebooks + values * LEVELS + (entry >> BITS));
+    uint32_t w[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const __half2 h = __halves2half2(dithered_level(lo, 2 * c), dithered_level(hi, 2 * c + 1));
-    w[c] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int c = 0; c < 4; ++c) {
+      const __half2 h = __halves2half2(dithered_level(lo, 2 * c), dithered_level(hi, 2 * c + 1));
+      w[c] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sts128(kSplitTable + entry * 256 + values * 128 + ((r + entry) & 7) * 16, w[0], w[1], w[2], w[3]);
   }
-#pragma unroll
-  for (int r = 0; r < 8; ++r) sts128(kSplitTable + entry * 256 + values * 128 + ((r + (tid >> 1)) & 7) * 16, w[0], w[1], w[2], w[3]);
 }
 // Address of entry I of the four whose numbers lie side by side in x (2 * BITS bits each); `column` is in the low byte, and the table's.
 template <int BITS, int I> __device__ __forceinline__ uint32_t table_address(uint32_t x, uint32_t column) {
@@ -254,9 +258,14 @@ template <int KEYS> __device__ __forceinline__ long long split_sequence_steps(co
   }
   return n * p.kv_heads;
 }
-// Behind the last unit: b = batch.
-template <int KEYS> __device__ __forceinline__ void split_next(const AttendParams& p, SplitUnit& u) {
-  if (++u.tile >= split_tiles(p, u.seq)) {
+// The unit after (b, kvh, tile); behind the last one: b = batch.  What the kernel keeps of a unit while it works on it is little.
+template <int KEYS> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
+  SplitUnit u;
+  u.b = b;
+  u.kvh = kvh;
+  u.tile = tile + 1;
+  u.seq = attend_sequence(p, b);
+  if (u.tile >= split_tiles(p, u.seq)) {
     u.tile = 0;
     if (++u.kvh == p.kv_heads) {
       u.kvh = 0;
@@ -264,10 +273,11 @@ template <int KEYS> __device__ __forceinline__ void split_next(const AttendParam
         u.seq = attend_sequence(p, u.b);
         if (u.seq.queries > 0) break;
       }
-      if (u.b >= p.batch) return;
+      if (u.b >= p.batch) return u;
     }
   }
   split_tile<KEYS>(p, u);
+  return u;
 }
 
 // Workspace: a header, a record for each unit, and two parts a warp (of a unit that began before the warp's piece, and of one that goes on
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kSplitThreads / 32], s_line[kSplitThreads];         // steps before each share of the sequences
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid);
+  if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid, kSplitThreads);
   pdl_wait();
 
   // ---- the line of steps: each thread a share of the sequences, a scan over the block
@@ -380,7 +390,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
   // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest
   // of a page, or of an image's states; the page after it is looked up when it begins.
-  SplitUnit f = u;
+  struct { int b, kvh, tile, keys, steps; } f = {u.b, u.kvh, u.tile, u.keys, u.steps};
   int f_step = static_cast<int>(start - at), f_left = static_cast<int>(end - start), f_slot = 0;
   int run = 0, next_page = 0;                                                      // sixteens of the run that are left
   bool valid = false, masked = true;
@@ -452,7 +462,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       f_slot = f_slot + 1 == kSplitStages ? 0 : f_slot + 1;
       if (--f_left > 0) {
         if (++f_step == f.steps) {
-          split_next<KEYS>(p, f);
+          const SplitUnit n = split_next<KEYS>(p, f.b, f.kvh, f.tile);
+          f = {n.b, n.kvh, n.tile, n.keys, n.steps};
           f_step = run = 0;
           look_up(0);
         }
@@ -518,8 +529,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         qa[s][2 + h] = w[2 * s + 1];
       }
     }
-    // packed: o holds sum p (scale / 2^e) level, v_inverse = 2^-e (0: none yet), centers the sum of p * center
-    float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {}, centers[2] = {0.0f, 0.0f}, v_inverse = 0.0f;
+    float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {}, centers[2] = {0.0f, 0.0f};
     const int unit_first = static_cast<int>(max(at - start, -0x40000000ll)), unit_last = static_cast<int>(min(at + u.steps, end) - start);
     const int key_base = static_cast<int>((start - at) * KEYS);                    // key of step s: key_base + s * KEYS
 #pragma unroll 1
@@ -535,7 +545,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       const bool all = seen == (KEYS == 32 ? 0xffffffffu : 0xffffu);
       // ---- scores
       float s[NT][4];
-      uint32_t vst[8];                                                             // center and scale of the lane's eight values
       if constexpr (PACKED) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -563,29 +572,20 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         }
         // q . k = scale * (q . level) + center * sum q
         const uint32_t stats = src + 2 * Step::kRows + c * 32;
-        const uint4 k0 = lds128(stats), k1 = lds128(stats + 16), v0 = lds128(stats + Step::kStats), v1 = lds128(stats + Step::kStats + 16);
+        const uint4 k0 = lds128(stats), k1 = lds128(stats + 16);
         uint32_t kst[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-        vst[0] = v0.x; vst[1] = v0.y; vst[2] = v0.z; vst[3] = v0.w; vst[4] = v1.x; vst[5] = v1.y; vst[6] = v1.z; vst[7] = v1.w;
         if (!all) {                                                                // whatever lies behind the last key: 0
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const bool is = (seen >> (8 * c + j)) & 1;
-            kst[j] = is ? kst[j] : 0u;
-            vst[j] = is ? vst[j] : 0u;
-          }
+          for (int j = 0; j < 8; ++j) kst[j] = (seen >> (8 * c + j)) & 1 ? kst[j] : 0u;
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float c0, s0, c1, s1;
-          unpack2(sixteen_to_pair<__half>(kst[key_in_eight(n, 0)]), c0, s0);
-          unpack2(sixteen_to_pair<__half>(kst[key_in_eight(n, 1)]), c1, s1);
-          const f32x2 scale = pack2(s0, s1), center = pack2(c0, c1);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && !both) continue;
-            unpack2(fma2(pack2(s[n][2 * h], s[n][2 * h + 1]), scale, mul2(center, pack2(q_sum[h], q_sum[h]))), s[n][2 * h], s[n][2 * h + 1]);
+          for (int j = 0; j < 2; ++j) {
+            const float2 cs = __half22float2(*reinterpret_cast<const __half2*>(&kst[key_in_eight(n, j)]));
+            s[n][j] = fmaf(s[n][j], cs.y, cs.x * q_sum[0]);
+            if (both) s[n][2 + j] = fmaf(s[n][2 + j], cs.y, cs.x * q_sum[1]);
           }
-        }
       } else {
         // matrices of 8 keys x 8 values: lanes 0-7 keys 0-7, 8-15 the next eight values, 16-31 keys 8-15
         const int row = (lane & 7) + 8 * (lane >> 4), ch = (lane >> 3) & 1;
@@ -612,6 +612,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
             if (((seen >> key) & 1) == 0 || base + key >= limit[j >> 1]) s[n][j] = ninf;
           }
       }
+      // Packed: the values' scales go into the probabilities, sum p (scale * level + center) = sum (p scale) level + sum p center.  A row's
+      // exponents are taken against its maximum plus that of the scales (log2, rounded down), so that p * scale stays in fp16's range; what this
+      // multiplies all three sums by cancels in the end.
+      float v_log = 0.0f;
+      if constexpr (PACKED) {
+        const uint32_t own = (seen >> lane) & 1 ? lds32(src + 2 * Step::kRows + Step::kStats + lane * 4) >> 16 : 0u;
+        v_log = static_cast<float>(static_cast<int>(__reduce_max_sync(0xffffffffu, own) >> 10) - 15);
+      }
       float m[2] = {ninf, ninf};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -621,9 +629,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         for (int n = 1; n < NT; ++n) x = max3(x, s[n][2 * h], s[n][2 * h + 1]);
         x *= row_scale[h];                                                         // a positive factor
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        m[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        m[h] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) + v_log;
       }
-      // a maximum is renewed when it is passed by 2^8: probabilities up to 256, and sums as exact
+      // a maximum is renewed when it is passed by 2^8: sums are as exact, and it happens a few times a unit
       const bool renew[2] = {m[0] > top[0] + 8.0f || (top[0] == ninf && m[0] > ninf), m[1] > top[1] + 8.0f || (top[1] == ninf && m[1] > ninf)};
       if (__any_sync(0xffffffffu, renew[0] || renew[1])) {
 #pragma unroll
@@ -640,55 +648,46 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           }
         }
       }
-      // packed: the values' scales go into the probabilities, relative to a power of two that is renewed when a scale passes it by 2^4
+      uint32_t pa[NT][2];
+      uint32_t vst[8];                                                             // center and scale of the lane's eight values
       if constexpr (PACKED) {
-        uint32_t largest = 0;
+        const uint32_t stats = src + 2 * Step::kRows + Step::kStats + c * 32;
+        const uint4 v0 = lds128(stats), v1 = lds128(stats + 16);
+        vst[0] = v0.x; vst[1] = v0.y; vst[2] = v0.z; vst[3] = v0.w; vst[4] = v1.x; vst[5] = v1.y; vst[6] = v1.z; vst[7] = v1.w;
+        if (!all) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) largest = max(largest, vst[j] >> 16);
-        largest = __reduce_max_sync(0xffffffffu, largest);
-        const float v_scale = __half2float(__ushort_as_half(static_cast<unsigned short>(largest)));
-        if (v_scale * v_inverse > 16.0f || (v_inverse == 0.0f && largest != 0u)) {
-          const float next = __int_as_float(0x7F000000 - (__float_as_int(v_scale) & 0x7F800000));
-          const float f = next / (v_inverse == 0.0f ? next : v_inverse);
-          v_inverse = next;
-#pragma unroll
-          for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][j] *= f;
+          for (int j = 0; j < 8; ++j) vst[j] = (seen >> (8 * c + j)) & 1 ? vst[j] : 0u;
         }
       }
-      uint32_t pa[NT][2];
+      const float nm[2] = {top[0] == ninf ? 0.0f : -top[0], top[1] == ninf ? 0.0f : -top[1]};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1 && !both) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) pa[n][1] = 0u;
-          continue;
-        }
-        const float nm = top[h] == ninf ? 0.0f : -top[h];
-        const f32x2 f2 = pack2(row_scale[h], row_scale[h]), nm2 = pack2(nm, nm), inv2 = pack2(v_inverse, v_inverse);
-        f32x2 part = pack2(sum[h], 0.0f), part_c = pack2(centers[h], 0.0f);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float x, y;
-          unpack2(fma2(pack2(s[n][2 * h], s[n][2 * h + 1]), f2, nm2), x, y);
-          f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
-          part = add2(part, e);
-          if constexpr (PACKED) {
-            float c0, s0, c1, s1;
-            unpack2(sixteen_to_pair<__half>(vst[key_in_eight(n, 0)]), c0, s0);
-            unpack2(sixteen_to_pair<__half>(vst[key_in_eight(n, 1)]), c1, s1);
-            part_c = fma2(e, pack2(c0, c1), part_c);
-            e = mul2(e, mul2(pack2(s0, s1), inv2));
-          }
-          pa[n][h] = pair_to_sixteen<E>(e);                                        // rounded for the second product
-        }
-        float x, y;
-        unpack2(part, x, y);
-        sum[h] = x + y;
+      for (int n = 0; n < NT; ++n) {
+        float scale[2], center[2];
         if constexpr (PACKED) {
-          unpack2(part_c, x, y);
-          centers[h] = x + y;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 cs = __half22float2(*reinterpret_cast<const __half2*>(&vst[key_in_eight(n, j)]));
+            center[j] = cs.x;
+            scale[j] = cs.y;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !both) {
+            pa[n][1] = 0u;
+            continue;
+          }
+          float e[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            e[j] = exp2_approx(fmaf(s[n][2 * h + j], row_scale[h], nm[h]));
+            sum[h] += e[j];
+            if constexpr (PACKED) {
+              centers[h] = fmaf(e[j], center[j], centers[h]);
+              e[j] *= scale[j];
+            }
+          }
+          pa[n][h] = pair_to_sixteen<E>(pack2(e[0], e[1]));                        // rounded for the second product
         }
       }
       // ---- values
@@ -748,11 +747,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       if constexpr (PACKED) {
         centers[h] += __shfl_xor_sync(0xffffffffu, centers[h], 1);
         centers[h] += __shfl_xor_sync(0xffffffffu, centers[h], 2);
-        const float up = v_inverse == 0.0f ? 0.0f : 1.0f / v_inverse;
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) o[n][2 * h + j] = fmaf(o[n][2 * h + j], up, centers[h]);
+          for (int j = 0; j < 2; ++j) o[n][2 * h + j] += centers[h];
       }
     }
     const bool begins = unit_first >= 0, complete = begins && at + u.steps <= end;
@@ -792,7 +790,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     at += u.steps;
-    if (step < steps) split_next<KEYS>(p, u);
+    if (step < steps) u = split_next<KEYS>(p, u.b, u.kvh, u.tile);
   }
   cp_async_wait<0>();
 }

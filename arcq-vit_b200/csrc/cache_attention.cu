@@ -126,10 +126,14 @@ void split_shape(arcq::AttendParams& p) {
 }
 bool few_rows(const arcq::AttendParams& p) { return static_cast<long long>(p.max_new) * p.group <= 2 * arcq::kSplitRows; }
 
+// Units of up to so many steps are not cut between blocks: no second kernel.
+constexpr int kWholeUnitSteps = 48;
+
 template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
   auto join = arcq::join_attention_kernel<arcq::SplitStep<BITS>::kKeys>;
-  constexpr size_t smem = arcq::split_smem<BITS>();
+  constexpr size_t smem = arcq::split_parts<BITS>() + arcq::kSplitSharedParts + 128;
+  static_assert(smem + arcq::kSplitBase <= 227 * 1024, "");
   static thread_local int done_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -150,8 +154,9 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
     return fail(ARCQ_E_BAD_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)arcq::split_workspace(p, sms));
   const long long units = arcq::split_units(p), steps = units * (p.max_keys / arcq::SplitStep<BITS>::kKeys + 1);
   if (units > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
+  p.whole_units = p.max_keys <= kWholeUnitSteps * arcq::SplitStep<BITS>::kKeys;
   cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
-  if (e == cudaSuccess) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
+  if (e == cudaSuccess && !p.whole_units) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 

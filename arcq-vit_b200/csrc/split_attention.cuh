@@ -54,6 +54,7 @@ struct AttendParams {
   int heads, kv_heads, group, tiles, splits, batch;
   void* workspace;                      // split_attention_kernel
   int part_rows;                        // of a part: 16, or all rows that there can be
+  int whole_units;                      // each block has whole units
   uint32_t poll_limit;                  // tile_attention.cuh
   int* status;
 };
@@ -195,10 +196,11 @@ template <int BITS> __host__ __device__ constexpr uint32_t split_ring(uint32_t b
   const int below = static_cast<int>((kSplitTable - base) / ring);
   return warp < below ? base + warp * ring : kSplitTableEnd + (warp - below) * ring;
 }
-// dynamic shared memory for a base of at most kSplitBase
+// where the rings and the table end for a base of at most kSplitBase (16 bits: relative to it); the warps' parts lie behind
 constexpr uint32_t kSplitBase = 8192;
-template <int BITS> constexpr uint32_t split_smem() {
-  return BITS == 16 ? kSplitWarps * SplitStep<16>::kRing + 128 : split_ring<BITS>(kSplitBase, kSplitWarps);
+template <int BITS> __host__ __device__ constexpr uint32_t split_parts() {
+  const uint32_t end = split_ring<BITS>(kSplitBase, kSplitWarps);
+  return BITS == 16 ? kSplitWarps * SplitStep<16>::kRing : end < kSplitTableEnd ? kSplitTableEnd : end;
 }
 // A level in fp16, rounded up in a share of the copies that is the position between its neighbours: the copies of lanes 4g + c, low and high,
 // serve different keys (values) or parts of a head (keys), over which the roundings then average out.
@@ -280,26 +282,55 @@ template <int KEYS> __device__ __forceinline__ SplitUnit split_next(const Attend
   return u;
 }
 
-// Workspace: a header, a record for each unit, and two parts a warp (of a unit that began before the warp's piece, and of one that goes on
-// behind it); a part is a row of 64 outputs, maximum and sum for each of its rows.
+// A part of a unit: for each of its rows 64 outputs, maximum and sum.  A warp has two of them (of a unit that began before its piece, and of one
+// that goes on behind it), in shared memory where they fit, and so has a block, in the workspace: a header, a record for each unit, the blocks'
+// parts, and the warps' where shared memory is too small.
 struct SplitHeader {
-  long long piece, unused;
+  long long piece, unused;                                                        // steps of a block
 };
 struct SplitRecord {
   long long start;
   int steps, whole;
 };
-constexpr int kSplitPartRow = 68;
+constexpr int kSplitPartRow = 68, kSplitSharedRows = 8;                            // rows of parts in shared memory
+constexpr uint32_t kSplitSharedParts = 2 * kSplitWarps * kSplitSharedRows * kSplitPartRow * 4;
 __host__ __device__ inline long long split_units(const AttendParams& p) { return static_cast<long long>(p.batch) * p.kv_heads * p.tiles; }
 __host__ __device__ inline long long split_workspace(const AttendParams& p, int blocks) {
+  const long long part = static_cast<long long>(p.part_rows) * kSplitPartRow * 4;
   return static_cast<long long>(sizeof(SplitHeader)) + split_units(p) * sizeof(SplitRecord) +
-         2ll * blocks * kSplitWarps * p.part_rows * kSplitPartRow * 4;
+         2ll * blocks * part * (p.part_rows > kSplitSharedRows ? 1 + kSplitWarps : 1);
 }
 __device__ __forceinline__ SplitRecord* split_records(const AttendParams& p) {
   return reinterpret_cast<SplitRecord*>(static_cast<uint8_t*>(p.workspace) + sizeof(SplitHeader));
 }
 __device__ __forceinline__ float* split_part(const AttendParams& p, long long slot) {
   return reinterpret_cast<float*>(split_records(p) + split_units(p)) + slot * p.part_rows * kSplitPartRow;
+}
+// The parts of one unit added up in the order of the keys, four values of a row a thread (the first rows * 16 threads).  next(i): part i.
+template <typename Next> __device__ __forceinline__ float4 add_parts(int count, int row, int column, float& top, float& sum, Next next) {
+  top = __int_as_float(0xff800000);
+  sum = 0.0f;
+  float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float* const part = next(i) + row * kSplitPartRow;
+    const float2 ts = *reinterpret_cast<const float2*>(part + 64);
+    const float4 x = *reinterpret_cast<const float4*>(part + 4 * column);
+    const float m = fmaxf(top, ts.x), base = m == __int_as_float(0xff800000) ? 0.0f : m, fa = exp2_approx(top - base), fb = exp2_approx(ts.x - base);
+    top = m;
+    sum = sum * fa + ts.y * fb;
+    o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
+  }
+  return o;
+}
+// a query that sees no key: zeros; NaN stays NaN
+__device__ __forceinline__ float inverse_sum(float sum) { return sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum); }
+__device__ __forceinline__ void write_four(const AttendParams& p, long long first_row, int kvh, int row, int column, float4 o, float f) {
+  const long long token = first_row + row / p.group;
+  const long long dst = (token * p.heads + kvh * p.group + row % p.group) * 64 + 4 * column;
+  const f32x2 lo = pack2(o.x * f, o.y * f), hi = pack2(o.z * f, o.w * f);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + dst) =
+      p.q_bf16 ? make_uint2(pair_to_sixteen<__nv_bfloat16>(lo), pair_to_sixteen<__nv_bfloat16>(hi)) : make_uint2(pair_to_sixteen<__half>(lo), pair_to_sixteen<__half>(hi));
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
@@ -310,6 +341,9 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, ui
 }
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool is) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -322,6 +356,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   constexpr int KEYS = Step::kKeys, NT = KEYS / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kSplitThreads / 32], s_line[kSplitThreads];         // steps before each share of the sequences
+  __shared__ struct {
+    long long at;
+    int b, kvh, tile, rows, steps, first_row;
+  } s_groups[kSplitWarps + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid, kSplitThreads);
   pdl_wait();
@@ -346,46 +384,63 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   }
   s_line[tid] = base_of_warp + before - mine;
   __syncthreads();
-  const long long warps = static_cast<long long>(gridDim.x) * kSplitWarps;
-  const long long piece = max((total + warps - 1) / warps, 1ll);
-  const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;      // small jobs: a warp a multiprocessor
-  if (blockIdx.x == 0 && tid == 0) static_cast<SplitHeader*>(p.workspace)->piece = piece;
-  const long long start = me * piece, end = min(start + piece, total);
-  if (start >= end) return;
-
-  // ---- the unit that the piece starts in
-  SplitUnit u;
-  long long at;                                                                    // first step of the unit
-  {
+  // the unit that a step of the line is in, and the unit's first step
+  auto locate = [&](long long x, long long& at) {
+    SplitUnit u;
     int lo = 0, hi = kSplitThreads - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (s_line[mid] <= start) lo = mid; else hi = mid - 1;
+      if (s_line[mid] <= x) lo = mid; else hi = mid - 1;
     }
     at = s_line[lo];
-    int b = lo * share;
-    for (;; ++b) {
-      const long long n = split_sequence_steps<KEYS>(p, b);
-      if (at + n > start) break;
+    for (u.b = lo * share;; ++u.b) {
+      const long long n = split_sequence_steps<KEYS>(p, u.b);
+      if (at + n > x) {
+        u.kvh = static_cast<int>((x - at) / (n / p.kv_heads));
+        at += u.kvh * (n / p.kv_heads);
+        break;
+      }
       at += n;
     }
-    u.b = b;
-    u.seq = attend_sequence(p, b);
-    const int tiles = split_tiles(p, u.seq);
-    long long n = 0;
-    for (u.tile = 0; u.tile < tiles; ++u.tile) {
+    u.seq = attend_sequence(p, u.b);
+    for (u.tile = 0;; ++u.tile) {
       split_tile<KEYS>(p, u);
-      n += u.steps;
-    }
-    u.kvh = static_cast<int>((start - at) / n);
-    at += u.kvh * n;
-    u.tile = 0;
-    for (;; ++u.tile) {
-      split_tile<KEYS>(p, u);
-      if (at + u.steps > start) break;
+      if (at + u.steps > x) break;
       at += u.steps;
     }
+    return u;
+  };
+  // ---- the block's piece of the line, and the warp's
+  const long long piece = max((total + gridDim.x - 1) / gridDim.x, 1ll);
+  long long from = min(blockIdx.x * piece, total), to = min(from + piece, total);
+  if (p.whole_units) {                                                             // the units that begin in the piece
+    if (warp < 2) {
+      const long long x = warp == 0 ? from : to;
+      long long at = x;
+      if (x < total) {
+        const SplitUnit u = locate(x, at);
+        if (at < x) at += u.steps;
+      }
+      if (lane == 0) s_scan[warp] = at;
+    }
+    __syncthreads();
+    from = s_scan[0];
+    to = s_scan[1];
+  } else if (blockIdx.x == 0 && tid == 0) {
+    static_cast<SplitHeader*>(p.workspace)->piece = piece;
   }
+  if (from >= to) return;
+  const int per = static_cast<int>((to - from + kSplitWarps - 1) / kSplitWarps);
+  const long long start = min(from + static_cast<long long>(warp) * per, to), end = min(start + per, to);
+  // parts of this block's warps; the units they are of, by the warp that has the first: 0 .. (begun there), kSplitWarps (before the block's piece)
+  float* const parts = p.part_rows <= kSplitSharedRows ? reinterpret_cast<float*>(smem + split_parts<BITS>() - (PACKED ? smem_u32(smem) : 0))
+                                                       : split_part(p, 2ll * gridDim.x + 2ll * kSplitWarps * blockIdx.x);
+  const int part_size = p.part_rows * kSplitPartRow;
+  if (tid <= kSplitWarps) s_groups[tid].rows = 0;
+  __syncthreads();
+  if (start < end) {
+  long long at;
+  SplitUnit u = locate(start, at);
 
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
   // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest
@@ -411,7 +466,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       const long long row = valid ? ((static_cast<long long>(page) * p.kv_heads + f.kvh) << p.page_shift) + place : 0;
       fk = p.k.rows + row * Step::kRow + lane * 16;
       fv = p.v.rows + row * Step::kRow + lane * 16;
-      fs = reinterpret_cast<const uint8_t*>((lane & 4 ? p.v.stats : p.k.stats) + row) + (lane & 3) * 16;
+      fs = reinterpret_cast<const uint8_t*>((lane & 4 ? p.v.stats : p.k.stats) + row) + (lane & 3) * 16 + (lane & 8) * 8;
     } else {
       const long long blk = valid ? page : 0, row = valid ? place + (lane >> 3) : 0;
       fk = p.k.rows + blk * p.k.block_stride + f.kvh * p.k.head_stride + row * p.k.token_stride + (lane & 7) * 16;
@@ -426,6 +481,23 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     uint32_t seen = 0;
     if (f_left > 0) {
       const uint32_t dst = ring + f_slot * Step::kBytes;
+      if (PACKED && valid && run >= 2 && f_step * KEYS + KEYS <= f.keys) {          // both halves there, side by side
+        constexpr int CHUNKS = 8 * BITS;
+        const uint32_t to = dst + lane * 16 + (lane >= CHUNKS / 2 ? Step::kPad : 0);
+        constexpr uint32_t half = 16 * Step::kRow;
+        if (lane < CHUNKS) {
+          cp_async_16(to, fk);
+          cp_async_16(to + half + 2 * Step::kPad, fk + half);
+          cp_async_16(to + Step::kRows, fv);
+          cp_async_16(to + Step::kRows + half + 2 * Step::kPad, fv + half);
+        }
+        if (lane < 16) cp_async_16(dst + 2 * Step::kRows + ((lane >> 2) & 1) * Step::kStats + (lane >> 3) * 64 + (lane & 3) * 16, fs);
+        fk += 2 * half;
+        fv += 2 * half;
+        fs += 128;
+        run -= 2;
+        seen = 0xffffffffu;
+      } else
 #pragma unroll
       for (int h = 0; h < KEYS / 16; ++h) {
         const int key = f_step * KEYS + 16 * h, left = f.keys - key;
@@ -487,7 +559,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   const int steps = static_cast<int>(end - start);
   while (step < steps) {
     // rows g and g + 8 of the unit: queries, the keys that they see, the factor of their scores
-    const bool both = u.rows > 8;                                                  // the upper eight are there
     int limit[2];
     uint32_t qa[4][4];
     float row_scale[2] = {p.scale_log2, p.scale_log2}, q_sum[2] = {0.0f, 0.0f};
@@ -532,6 +603,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {}, centers[2] = {0.0f, 0.0f};
     const int unit_first = static_cast<int>(max(at - start, -0x40000000ll)), unit_last = static_cast<int>(min(at + u.steps, end) - start);
     const int key_base = static_cast<int>((start - at) * KEYS);                    // key of step s: key_base + s * KEYS
+    // the loop twice: with the upper eight rows and without, whose work would else be issued for nothing
+    auto steps_of = [&](auto two) {
+    constexpr bool both = decltype(two)::value;
 #pragma unroll 1
     for (; step < unit_last; ++step) {
       seen_now = seen_next;
@@ -739,6 +813,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
       __syncwarp();                                                                // the slot may be copied over
     }
+    };
+    if (u.rows > 8) steps_of(std::true_type{});
+    else steps_of(std::false_type{});
     // ---- the unit, or its part.  o[n][2h + j]: row g + 8h, value 16c + 8j + n (packed), 8n + 2c + j (16 bits)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -754,14 +831,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     const bool begins = unit_first >= 0, complete = begins && at + u.steps <= end;
-    if (begins && lane == 0) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, complete ? 1 : 0};
-    float* const part = split_part(p, 2 * me + (begins ? 1 : 0));
+    if (lane == 0) {
+      if (complete && !p.whole_units) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, 1};
+      if (!complete && (begins || warp == 0)) s_groups[begins ? warp : kSplitWarps] = {at, u.b, u.kvh, u.tile, u.rows, u.steps, u.seq.first_row};
+    }
+    float* const part = parts + (2 * warp + (begins ? 1 : 0)) * part_size;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (g + 8 * h >= u.rows) continue;
       const int r = u.tile * kSplitRows + g + 8 * h;
       if (complete) {
-        const float f = sum[h] > 0.0f ? 1.0f / sum[h] : (sum[h] == 0.0f ? 0.0f : sum[h]);      // a query that sees no key: zeros; NaN stays NaN
+        const float f = inverse_sum(sum[h]);
         const long long token = u.seq.first_row + r / p.group;
         uint16_t* const dst = static_cast<uint16_t*>(p.out) + (token * p.heads + u.kvh * p.group + r % p.group) * 64;
         auto two = [&](float x, float y) { return p.q_bf16 ? pair_to_sixteen<__nv_bfloat16>(pack2(x * f, y * f)) : pair_to_sixteen<__half>(pack2(x * f, y * f)); };
@@ -793,65 +873,50 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     if (step < steps) u = split_next<KEYS>(p, u.b, u.kvh, u.tile);
   }
   cp_async_wait<0>();
+  }
+  // ---- units that lie in more than one warp's piece
+  __syncthreads();
+  for (int i = 0; i <= kSplitWarps; ++i) {
+    const auto& u = s_groups[i];
+    if (tid >= u.rows * 16) continue;
+    const int first = i < kSplitWarps ? i : 0, last = static_cast<int>((min(u.at + u.steps, to) - 1 - from) / per), row = tid >> 4, column = tid & 15;
+    float top, sum;
+    const float4 o = add_parts(last - first + 1, row, column, top, sum, [&](int q) { return parts + (2 * (first + q) + (q == 0 && i < kSplitWarps ? 1 : 0)) * part_size; });
+    const bool complete = u.at >= from && u.at + u.steps <= to;
+    if (tid == 0 && u.at >= from && !p.whole_units)
+      split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {u.at, u.steps, complete ? 1 : 0};
+    if (complete) {
+      write_four(p, u.first_row, u.kvh, u.tile * kSplitRows + row, column, o, inverse_sum(sum));
+    } else {
+      float* const dst = split_part(p, 2ll * blockIdx.x + (u.at >= from ? 1 : 0)) + row * kSplitPartRow;
+      *reinterpret_cast<float4*>(dst + 4 * column) = o;
+      if (column == 0) *reinterpret_cast<float2*>(dst + 64) = make_float2(top, sum);
+    }
+  }
 }
 
-// Adds up the parts of the units that lie in more than one warp's piece: a block a unit; the parts are dealt out over groups of threads with
-// four values of a row each.
-constexpr int kJoinThreads = 256;
+// Adds up the blocks' parts of the units that lie in more than one block's piece: a block a unit.
+constexpr int kJoinThreads = kSplitRows * 16;
 template <int KEYS> __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
   pdl_launch_dependents();
-  __shared__ float4 s_out[kJoinThreads];
-  __shared__ float s_max[kJoinThreads], s_sum[kJoinThreads];
-  SplitUnit u;
   const long long unit = blockIdx.x;
+  SplitUnit u;
   u.tile = static_cast<int>(unit % p.tiles);
   u.kvh = static_cast<int>(unit / p.tiles % p.kv_heads);
   u.b = static_cast<int>(unit / p.tiles / p.kv_heads);
   pdl_wait();
-  u.seq = attend_sequence(p, u.b);
-  if (u.tile >= split_tiles(p, u.seq)) return;
-  split_tile<KEYS>(p, u);
-  const SplitRecord rec = split_records(p)[unit];
-  if (rec.whole) return;
+  const SplitRecord rec = split_records(p)[unit];                                  // not written where there is no such tile
   const long long piece = static_cast<SplitHeader*>(p.workspace)->piece;
+  u.seq = attend_sequence(p, u.b);
+  if (u.tile >= split_tiles(p, u.seq) || rec.whole) return;
+  split_tile<KEYS>(p, u);
+  const int tid = threadIdx.x, row = tid >> 4, column = tid & 15;
+  if (row >= u.rows) return;
   const long long first = rec.start / piece, last = (rec.start + rec.steps - 1) / piece;
-  const int width = u.rows * 16, groups = kJoinThreads / width, group = threadIdx.x / width, e = threadIdx.x % width, r = e >> 4, c = e & 15;
-  const float ninf = __int_as_float(0xff800000);
-  float m = ninf, l = 0.0f;
-  float4 o = make_float4(0, 0, 0, 0);
-  if (group < groups) {
-    for (long long w = first + group; w <= last; w += groups) {
-      const float* const part = split_part(p, 2 * w + (rec.start >= w * piece ? 1 : 0)) + r * kSplitPartRow;
-      const float2 ml = *reinterpret_cast<const float2*>(part + 64);
-      const float4 x = *reinterpret_cast<const float4*>(part + 4 * c);
-      const float next = fmaxf(m, ml.x), base = next == ninf ? 0.0f : next, fa = exp2_approx(m - base), fb = exp2_approx(ml.x - base);
-      m = next;
-      l = l * fa + ml.y * fb;
-      o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
-    }
-  }
-  s_out[threadIdx.x] = o;
-  s_max[threadIdx.x] = m;
-  s_sum[threadIdx.x] = l;
-  __syncthreads();
-  if (group != 0) return;
-  for (int q = 1; q < groups; ++q) m = fmaxf(m, s_max[q * width + e]);
-  const float base = m == ninf ? 0.0f : m;
-  l = 0.0f;
-  o = make_float4(0, 0, 0, 0);
-  for (int q = 0; q < groups; ++q) {
-    const float f = exp2_approx(s_max[q * width + e] - base);
-    const float4 x = s_out[q * width + e];
-    l += f * s_sum[q * width + e];
-    o = make_float4(o.x + f * x.x, o.y + f * x.y, o.z + f * x.z, o.w + f * x.w);
-  }
-  const float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  const int row = u.tile * kSplitRows + r;
-  const long long token = u.seq.first_row + row / p.group;
-  const long long dst = (token * p.heads + u.kvh * p.group + row % p.group) * 64 + 4 * c;
-  const f32x2 lo = pack2(o.x * f, o.y * f), hi = pack2(o.z * f, o.w * f);
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + dst) =
-      p.q_bf16 ? make_uint2(pair_to_sixteen<__nv_bfloat16>(lo), pair_to_sixteen<__nv_bfloat16>(hi)) : make_uint2(pair_to_sixteen<__half>(lo), pair_to_sixteen<__half>(hi));
+  float top, sum;
+  const float4 o = add_parts(static_cast<int>(last - first + 1), row, column, top, sum,
+                             [&](int q) { return split_part(p, 2 * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
+  write_four(p, u.seq.first_row, u.kvh, u.tile * kSplitRows + row, column, o, inverse_sum(sum));
 }
 
 }  // namespace arcq

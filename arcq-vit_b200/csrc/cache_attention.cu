@@ -98,16 +98,39 @@ int blocks_for(long long items, int per_block, int per_sm) {
   return static_cast<int>(need < 1 ? 1 : need < cap ? need : cap);
 }
 
+// From so many groups of keys on a lane a group is the faster way; below, eight lanes a group finish sooner: 1200 groups in 4 bits 3.2 against
+// 2.7 us, 3600 groups 3.3 against 3.7, 12 000 3.8 against 6.1, 196 608 24 against 61.
+constexpr long long kWriteTileGroups = 2500;
+
+template <typename T, int BITS> cudaError_t write_packed(const arcq::KvCacheParams& p, cudaStream_t st) {
+  const long long groups = p.tokens * p.heads;
+  if constexpr (sizeof(T) == 2) {
+    if (groups >= kWriteTileGroups) {
+      auto k = arcq::kv_write_tile_kernel<T, BITS>;
+      static thread_local int done_dev = -1;
+      int dev = 0;
+      cudaGetDevice(&dev);
+      if (done_dev != dev) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(arcq::kWriteSmem));
+        if (e != cudaSuccess) return e;
+        done_dev = dev;
+      }
+      return launch(k, dim3(blocks_for(groups, arcq::kWriteWarps * 32, 2), 2), arcq::kWriteThreads, arcq::kWriteSmem, 1, st, p);
+    }
+  }
+  return launch(arcq::kv_write_kernel<T, BITS>, dim3(blocks_for(groups, 32, 4), 2), 256, 0, 1, st, p);
+}
 template <typename T> cudaError_t write_packed(const arcq::KvCacheParams& p, int bits, cudaStream_t st) {
-  const dim3 grid(blocks_for(p.tokens * p.heads, 32, 4), 2);
   switch (bits) {
-    case 4: return launch(arcq::kv_write_kernel<T, 4>, grid, 256, 0, 1, st, p);
-    case 3: return launch(arcq::kv_write_kernel<T, 3>, grid, 256, 0, 1, st, p);
-    default: return launch(arcq::kv_write_kernel<T, 2>, grid, 256, 0, 1, st, p);
+    case 4: return write_packed<T, 4>(p, st);
+    case 3: return write_packed<T, 3>(p, st);
+    default: return write_packed<T, 2>(p, st);
   }
 }
+
+constexpr int kReadBlocks = 4;                 // an SM, of keys and as many of values
 template <typename O> cudaError_t read_cache(const arcq::KvCacheParams& p, int bits, int dtype, cudaStream_t st) {
-  const dim3 grid(blocks_for(p.tokens * p.heads * 8, 256, 4), 2);
+  const dim3 grid(blocks_for(p.tokens * p.heads * 4, 256, kReadBlocks), 2);
   switch (bits) {
     case 16:
       if (dtype == ARCQ_DT_F16) return launch(arcq::kv_read_kernel<__half, 16, O>, grid, 256, 0, 1, st, p);
@@ -268,7 +291,7 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
   if (tokens < 0 || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
   if (tokens == 0) return ARCQ_OK;
   if (k_out == nullptr || v_out == nullptr || slots == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
-  if (!aligned(k_out, 16) || !aligned(v_out, 16)) return fail(ARCQ_E_ALIGN, "outputs must be 16-byte aligned");
+  if (!aligned(k_out, 32) || !aligned(v_out, 32)) return fail(ARCQ_E_ALIGN, "outputs must be 32-byte aligned");
   arcq::KvCacheParams p = cache_params(cache, slots, tokens);
   p.kv[0].out = k_out;
   p.kv[1].out = v_out;

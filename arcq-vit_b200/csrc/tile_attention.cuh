@@ -25,8 +25,8 @@
 namespace arcq {
 
 constexpr int kStatusTileAttentionTimeout = 0x502;
-constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128, kTileSlots = 3;
-constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 192, kTileLoadRegs = 88, kTileIssueRegs = 40;
+constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128, kTileSlots = 3, kTileSeen = 8;
+constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 184, kTileLoadRegs = 88, kTileIssueRegs = 56;
 static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
 constexpr uint32_t kTileBytes = 128 * 128;                        // 128 rows of 64 16-bit values
 constexpr uint32_t kTileTmemCols = 512;
@@ -45,7 +45,7 @@ __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
   s.v = s.k + kTileSlots * kTileBytes;
   s.tables = s.v + kTileSlots * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
   s.seen = s.tables + (packed ? 2 * kPairTableBytes : 0);
-  s.max = s.seen + kTileSlots * 16;
+  s.max = s.seen + kTileSeen * 16;
   s.sum = s.max + 2 * kTileRows * 4;
   s.bars = s.sum + 2 * kTileRows * 4;
   s.total = s.bars + 32 * 8 + 1024;                               // and alignment
@@ -54,16 +54,6 @@ __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
 
 template <typename E> __device__ __forceinline__ uint32_t tile_idesc(int M, int N) {
   return umma_idesc_f16(M, N) | (sizeof(E) == 2 && std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
-}
-__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 "
-      "[%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
 }
 __device__ __forceinline__ float lds_cluster(uint32_t addr) {
   float v;
@@ -87,7 +77,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   uint64_t *const q_full = bars + 12, *const s_full = bars + 14, *const s_read = bars + 16, *const p_full = bars + 18, *const o_done = bars + 20;   // [stream]
   uint64_t* const stopped = bars + 22;
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 24);
-  uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [slot][warp]
+  uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [tile % kTileSeen][warp]: written before the tile's keys are handed over
   float* const s_max = reinterpret_cast<float*>(smem + L.max);                    // [stream][row]
   float* const s_sum = reinterpret_cast<float*>(smem + L.sum);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -213,6 +203,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       bool is = base + lane < keys && (lane < 16 ? there[0] : there[1]);
       if (is && p.mask != nullptr) is = p.mask[b * p.mask_stride + base + lane] != 0;
       pl.seen = __ballot_sync(0xffffffffu, is);
+      if (lane == 0) s_seen[j % kTileSeen * 4 + w] = pl.seen;
       return pl;
     };
     auto free_slot = [&](uint64_t* bar, int j) {
@@ -250,7 +241,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         }
         free_slot(v_free, j);
         copy(p.v, pl.v, pl.seen, v_smem + slot * kTileBytes);
-        if (lane == 0) s_seen[slot * 4 + w] = pl.seen;
       }
       if (count > 0) {
         cp_async_wait<1>();
@@ -309,20 +299,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         }
       };
       Row kr, vr;
-      uint32_t seen = 0;
       auto fetch = [&](int j) {
         const Place pl = place(j);
         const int u = lane >> 4;
         const bool is = (pl.seen >> lane) & 1;
         load_row(p.k, pl.k[u] + (lane & 15) * p.k.token_stride, pl.st[u] + (lane & 15), is, kr);
         load_row(p.v, pl.v[u] + (lane & 15) * p.v.token_stride, pl.st[u] + (lane & 15), is, vr);
-        seen = pl.seen;
       };
       if (count > 0) fetch(0);
       for (int j = 0; j < count; ++j) {
         const int slot = j % kTileSlots;
         const Row k = kr, v = vr;
-        const uint32_t now = seen;
         if (j + 1 < count) fetch(j + 1);
         free_slot(k_free, j);
         write_keys(k_smem + slot * kTileBytes + row, k);
@@ -331,7 +318,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         if (lane == 0) mbar_arrive(k_full + slot);
         free_slot(v_free, j);
         write_values(v_smem + slot * kTileBytes + row, v);
-        if (lane == 0) s_seen[slot * 4 + w] = now;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_full + slot);
@@ -376,7 +362,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     float top = ninf;                                                             // in units of the exponent
     f32x2 sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
     for (int i = 0; i < mine; ++i) {
-      const int j = halves ? i : 2 * i + t, slot = j % kTileSlots;
+      const int j = halves ? i : 2 * i + t;
       ok = ok && mbar_wait_warp(s_full + t, i & 1, polls);
       tc_fence_after_sync();
       if (rows_here && ok) {
@@ -388,8 +374,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         __syncwarp();
         if (lane == 0) mbar_arrive(s_read + t);
         // ---- what is not seen
-        ok = ok && mbar_wait_warp(v_full + slot, (j / kTileSlots) & 1, polls);
-        const uint4 seen = lds128(smem_u32(s_seen + slot * 4));
+        __syncwarp();
+        const uint4 seen = lds128(smem_u32(s_seen + j % kTileSeen * 4));
         const int base = (first + j) * kTileKeys;
         if (!__all_sync(0xffffffffu, (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && base + kTileKeys <= limit)) {
           const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
@@ -424,13 +410,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
           sum1 = mul2(sum1, f2);
           if (i > 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_at + 32 * h, o);
+            for (int h = 0; h < 4; ++h) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_at + 16 * h, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
-              tmem_st_32x32(o_at + 32 * h, o);
+              for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
+              tmem_st_32x16(o_at + 16 * h, o);
             }
           }
         }

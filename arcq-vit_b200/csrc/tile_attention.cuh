@@ -25,7 +25,10 @@
 namespace arcq {
 
 constexpr int kStatusTileAttentionTimeout = 0x502;
-constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128, kTileSlots = 3, kTileSeen = 8;
+constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128;
+// tiles of keys, and of values, in shared memory: 16 bits have no tables there
+__host__ __device__ constexpr int tile_slots(bool packed) { return packed ? 3 : 5; }
+constexpr int kTileSeen = 8;
 constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 184, kTileLoadRegs = 88, kTileIssueRegs = 56;
 static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
 constexpr uint32_t kTileBytes = 128 * 128;                        // 128 rows of 64 16-bit values
@@ -42,8 +45,8 @@ __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
   TileSmem s = {};
   s.q = 0;
   s.k = s.q + 2 * kTileBytes;
-  s.v = s.k + kTileSlots * kTileBytes;
-  s.tables = s.v + kTileSlots * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
+  s.v = s.k + tile_slots(packed) * kTileBytes;
+  s.tables = s.v + tile_slots(packed) * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
   s.seen = s.tables + (packed ? 2 * kPairTableBytes : 0);
   s.max = s.seen + kTileSeen * 16;
   s.sum = s.max + 2 * kTileRows * 4;
@@ -69,14 +72,15 @@ __device__ __forceinline__ float4 lds128_cluster(uint32_t addr) {
 template <int BITS, typename E>
 __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const __grid_constant__ AttendParams p) {
   constexpr bool PACKED = BITS != 16;
+  constexpr int SLOTS = tile_slots(PACKED);
   extern __shared__ uint8_t tile_smem_raw[];
   uint8_t* const smem = tile_smem_raw + ((1024u - (smem_u32(tile_smem_raw) & 1023u)) & 1023u);
   constexpr TileSmem L = tile_smem_layout(PACKED);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L.bars);
-  uint64_t *const k_full = bars, *const k_free = bars + 3, *const v_full = bars + 6, *const v_free = bars + 9;     // [slot]
-  uint64_t *const q_full = bars + 12, *const s_full = bars + 14, *const s_read = bars + 16, *const p_full = bars + 18, *const o_done = bars + 20;   // [stream]
-  uint64_t* const stopped = bars + 22;
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t *const k_full = bars, *const k_free = bars + 5, *const v_full = bars + 10, *const v_free = bars + 15;     // [slot]
+  uint64_t *const q_full = bars + 20, *const s_full = bars + 22, *const s_read = bars + 24, *const p_full = bars + 26, *const o_done = bars + 28;   // [stream]
+  uint64_t* const stopped = bars + 30;
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 31);
   uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [tile % kTileSeen][warp]: written before the tile's keys are handed over
   float* const s_max = reinterpret_cast<float*>(smem + L.max);                    // [stream][row]
   float* const s_sum = reinterpret_cast<float*>(smem + L.sum);
@@ -103,7 +107,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   }
   if (tid == 0) {
     const int users = halves ? 2 : 1;                                             // streams that read a tile of keys
-    for (int i = 0; i < kTileSlots; ++i) {
+    for (int i = 0; i < SLOTS; ++i) {
       mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
       mbar_init(k_free + i, users); mbar_init(v_free + i, users);
     }
@@ -144,8 +148,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       auto at = [&](int i) { return halves ? i : 2 * i + t; };
       for (int i = 0; i <= mine; ++i) {
         if (i < mine) {
-          const int j = at(i), slot = j % kTileSlots;
-          ok = ok && (i > 0 || mbar_wait(q_full + (halves ? t : 0), 0, polls)) && mbar_wait(k_full + slot, (j / kTileSlots) & 1, polls) &&
+          const int j = at(i), slot = j % SLOTS;
+          ok = ok && (i > 0 || mbar_wait(q_full + (halves ? t : 0), 0, polls)) && mbar_wait(k_full + slot, (j / SLOTS) & 1, polls) &&
                (i == 0 || mbar_wait(s_read + t, (i - 1) & 1, polls));
           tc_fence_after_sync();
           if (elect_one() && ok) {
@@ -156,8 +160,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
           __syncwarp();
         }
         if (i > 0) {
-          const int j = at(i - 1), slot = j % kTileSlots;
-          ok = ok && mbar_wait(v_full + slot, (j / kTileSlots) & 1, polls) && mbar_wait(p_full + t, (i - 1) & 1, polls);
+          const int j = at(i - 1), slot = j % SLOTS;
+          ok = ok && mbar_wait(v_full + slot, (j / SLOTS) & 1, polls) && mbar_wait(p_full + t, (i - 1) & 1, polls);
           tc_fence_after_sync();
           if (elect_one() && ok) {
 #pragma unroll
@@ -177,9 +181,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     fewer_registers<kTileLoadRegs>();
     const int w = warp - 8;
     const uint32_t k_smem = smem_u32(smem) + L.k + w * 4096, v_smem = smem_u32(smem) + L.v + w * 4096;
-    // where the two sixteens of keys of the warp lie (in one page each), and which keys are seen
+    // where the two sixteens of keys of the warp lie, each in one page; looked up a tile ahead, as are the masks
+    int page[2];
+    bool masked = true;
+    auto look_up = [&](int j) {
+      const int base = (first + j) * kTileKeys + 32 * w;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        page[u] = b;
+        if (p.table != nullptr && base + 16 * u < keys) page[u] = p.table[static_cast<long long>(b) * p.table_width + ((base + 16 * u) >> p.page_shift)];
+      }
+      if (!PACKED && p.mask != nullptr) masked = base + lane < keys && p.mask[b * p.mask_stride + base + lane] != 0;
+    };
     struct Place {
-      long long k[2], v[2], st[2];
+      long long k[2], v[2], stats[2];
       uint32_t seen;
     };
     auto place = [&](int j) {
@@ -188,65 +203,75 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       bool there[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int key = base + 16 * u;
-        int block = b, in = key;
-        there[u] = key < keys;
-        if (p.table != nullptr && there[u]) {
-          block = p.table[static_cast<long long>(b) * p.table_width + (key >> p.page_shift)];
-          in = key & ((1 << p.page_shift) - 1);
-          there[u] = block >= 0 && block < p.pages;
+        const int in = p.table != nullptr ? (base + 16 * u) & ((1 << p.page_shift) - 1) : base + 16 * u;
+        there[u] = base + 16 * u < keys && (p.table == nullptr || (page[u] >= 0 && page[u] < p.pages));
+        if (PACKED) {
+          pl.stats[u] = ((static_cast<long long>(page[u]) * p.kv_heads + kvh) << p.page_shift) + in;
+        } else {
+          pl.k[u] = page[u] * p.k.block_stride + kvh * p.k.head_stride + in * p.k.token_stride;
+          pl.v[u] = page[u] * p.v.block_stride + kvh * p.v.head_stride + in * p.v.token_stride;
         }
-        pl.k[u] = block * p.k.block_stride + kvh * p.k.head_stride + in * p.k.token_stride;
-        pl.v[u] = block * p.v.block_stride + kvh * p.v.head_stride + in * p.v.token_stride;
-        pl.st[u] = PACKED ? ((static_cast<long long>(block) * p.kv_heads + kvh) << p.page_shift) + in : 0;
       }
-      bool is = base + lane < keys && (lane < 16 ? there[0] : there[1]);
-      if (is && p.mask != nullptr) is = p.mask[b * p.mask_stride + base + lane] != 0;
-      pl.seen = __ballot_sync(0xffffffffu, is);
+      pl.seen = __ballot_sync(0xffffffffu, base + lane < keys && (lane < 16 ? there[0] : there[1]) && masked);
       if (lane == 0) s_seen[j % kTileSeen * 4 + w] = pl.seen;
+      if (j + 1 < count) look_up(j + 1);
       return pl;
     };
-    auto free_slot = [&](uint64_t* bar, int j) {
-      if (j >= kTileSlots) ok = mbar_wait(bar + j % kTileSlots, (j / kTileSlots - 1) & 1, polls) && ok;
+    // a slot's phase that the products have to have ended
+    auto wait_free = [&](uint64_t* bar, int j) {
+      if (j >= SLOTS) ok = mbar_wait(bar + j % SLOTS, (j / SLOTS - 1) & 1, polls) && ok;
     };
+    auto hand_over = [&](uint64_t* bar) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    if (count > 0) look_up(0);
     if constexpr (!PACKED) {
       // 16 bits: eight lanes a row, asynchronous copies.  A tile is handed over before a slot is waited for: the slot may be freed by a product
-      // that is issued behind one with that tile.
-      auto copy = [&](const AttendView& a, const long long (&at)[2], uint32_t seen, uint32_t dst) {
+      // that is issued behind one with that tile.  Where the slots are free already, the copies go first.
+      auto copy = [&](const AttendView& a, const long long (&from)[2], uint32_t seen, uint32_t dst) {
+        const uint32_t row0 = lane >> 3, ch = lane & 7;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const int row = 4 * r + (lane >> 3), c = lane & 7;
-          const bool is = (seen >> row) & 1;
-          cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), a.rows + (is ? at[r >> 2] + (row & 15) * a.token_stride + 16 * c : 0), is);
+        for (int u = 0; u < 2; ++u) {
+          const uint8_t* const src = a.rows + from[u] + row0 * a.token_stride + 16 * ch;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t row = 16 * u + 4 * r + row0, to = dst + row * 128 + ((ch ^ (row & 7)) << 4);
+            if (seen == 0xffffffffu) cp_async_16(to, src + r * 4 * a.token_stride);
+            else cp_async_16(to, (seen >> row) & 1 ? src + r * 4 * a.token_stride : a.rows, (seen >> row) & 1);
+          }
         }
         cp_async_commit();
       };
-      auto hand_over = [&](uint64_t* bar) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-      };
       for (int j = 0; j < count; ++j) {
         const Place pl = place(j);
-        const int slot = j % kTileSlots, before = (j + kTileSlots - 1) % kTileSlots;
-        if (j > 0) {
+        const int slot = j % SLOTS, before = (j + SLOTS - 1) % SLOTS;
+        bool pending = j > 0;
+        if (pending && j >= SLOTS &&
+            !__all_sync(0xffffffffu, mbar_test_wait(k_free + slot, (j / SLOTS - 1) & 1) && mbar_test_wait(v_free + slot, (j / SLOTS - 1) & 1))) {
           cp_async_wait<1>();
           hand_over(k_full + before);
+          cp_async_wait<0>();
+          hand_over(v_full + before);
+          pending = false;
         }
-        free_slot(k_free, j);
+        wait_free(k_free, j);
         copy(p.k, pl.k, pl.seen, k_smem + slot * kTileBytes);
-        if (j > 0) {
-          cp_async_wait<1>();
+        wait_free(v_free, j);
+        copy(p.v, pl.v, pl.seen, v_smem + slot * kTileBytes);
+        if (pending) {
+          cp_async_wait<3>();
+          hand_over(k_full + before);
+          cp_async_wait<2>();
           hand_over(v_full + before);
         }
-        free_slot(v_free, j);
-        copy(p.v, pl.v, pl.seen, v_smem + slot * kTileBytes);
       }
       if (count > 0) {
         cp_async_wait<1>();
-        hand_over(k_full + (count - 1) % kTileSlots);
+        hand_over(k_full + (count - 1) % SLOTS);
         cp_async_wait<0>();
-        hand_over(v_full + (count - 1) % kTileSlots);
+        hand_over(v_full + (count - 1) % SLOTS);
       }
     } else {
       // packed: a lane has a key's row, eight values of it at a time
@@ -255,14 +280,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       struct Row {
         uint32_t w[2 * BITS], stats;
       };
-      auto load_row = [&](const AttendView& a, long long at, long long st, bool is, Row& r) {
-        const uint32_t* const src = reinterpret_cast<const uint32_t*>(a.rows + at);
+      auto load_row = [&](const AttendView& a, long long at, bool is, Row& r) {
+        const uint2* const src = reinterpret_cast<const uint2*>(a.rows + at * (8 * BITS));
 #pragma unroll
-        for (int i = 0; i < 2 * BITS; i += 2) {
-          const uint2 u = is ? *reinterpret_cast<const uint2*>(src + i) : make_uint2(0, 0);
-          r.w[i] = u.x; r.w[i + 1] = u.y;
+        for (int i = 0; i < BITS; ++i) {
+          const uint2 u = is ? src[i] : make_uint2(0, 0);
+          r.w[2 * i] = u.x; r.w[2 * i + 1] = u.y;
         }
-        r.stats = is ? *reinterpret_cast<const uint32_t*>(a.stats + st) : 0;
+        r.stats = is ? *reinterpret_cast<const uint32_t*>(a.stats + at) : 0;
       };
       // the codes of values 8c .. 8c + 7, one per nibble
       auto codes = [](const Row& r, int c) {
@@ -301,26 +326,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       Row kr, vr;
       auto fetch = [&](int j) {
         const Place pl = place(j);
-        const int u = lane >> 4;
+        const long long at = pl.stats[lane >> 4] + (lane & 15);
         const bool is = (pl.seen >> lane) & 1;
-        load_row(p.k, pl.k[u] + (lane & 15) * p.k.token_stride, pl.st[u] + (lane & 15), is, kr);
-        load_row(p.v, pl.v[u] + (lane & 15) * p.v.token_stride, pl.st[u] + (lane & 15), is, vr);
+        load_row(p.k, at, is, kr);
+        load_row(p.v, at, is, vr);
       };
       if (count > 0) fetch(0);
       for (int j = 0; j < count; ++j) {
-        const int slot = j % kTileSlots;
+        const int slot = j % SLOTS;
         const Row k = kr, v = vr;
         if (j + 1 < count) fetch(j + 1);
-        free_slot(k_free, j);
+        wait_free(k_free, j);
         write_keys(k_smem + slot * kTileBytes + row, k);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(k_full + slot);
-        free_slot(v_free, j);
+        hand_over(k_full + slot);
+        wait_free(v_free, j);
         write_values(v_smem + slot * kTileBytes + row, v);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_full + slot);
+        hand_over(v_full + slot);
       }
     }
   } else {

@@ -183,12 +183,31 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 
+// How many clusters of a size run at a time; 0: none, or it cannot be said
+template <typename Kernel> int clusters_at_a_time(Kernel k, int size, size_t smem) {
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  lc.gridDim = dim3(size * arcq_host::sm_count());
+  lc.blockDim = dim3(arcq::kTileThreads);
+  lc.dynamicSmemBytes = smem;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, k, &lc) == cudaSuccess) return n;
+  cudaGetLastError();
+  return 0;
+}
+constexpr double kTileSetUp = 7.0;         // of a block, in tiles of keys: 13 us against 1.75 us
+
 // Blocks of a row tile, 1 to 8: the cluster size for which the rounds of blocks over the SMs take the fewest tiles of keys, a block's set-up and
 // the joining of results counted as tiles.
 template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStream_t st) {
   auto k = arcq::tile_attention_kernel<BITS, E>;
   constexpr size_t smem = arcq::tile_smem_layout(BITS != 16).total;
-  static thread_local int done_dev = -1;
+  static thread_local int done_dev = -1, room[9];                               // clusters of a size that run at a time
   int dev = 0;
   cudaGetDevice(&dev);
   if (done_dev != dev) {
@@ -199,6 +218,8 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
     const int got = arcq_host::launch_regs() > 0 ? arcq_host::launch_regs() : a.numRegs;
     if (got < arcq::kTileLaunchRegs)             // the warp groups' hand-over would wait for good
       return fail(ARCQ_E_CUDA, "attention: compiled for %d registers a thread, its warp groups share out %d", got, arcq::kTileLaunchRegs);
+    room[1] = arcq_host::sm_count();
+    for (int s = 2; s <= 8; ++s) room[s] = clusters_at_a_time(k, s, smem);
     done_dev = dev;
   }
   const long long all_rows = static_cast<long long>(p.max_new) * p.group;
@@ -208,9 +229,8 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
   int splits = 1;
   double best = 1e30;
   for (int s = 1; s <= 8 && (s == 1 || s <= key_tiles); ++s) {
-    const int room = arcq_host::sm_count() / s - (s > 2 ? 2 : 0);             // clusters at a time: some SMs of a group are left over
-    const double rounds = ceil(static_cast<double>(units) / (room > 0 ? room : 1));
-    const double cost = rounds * (ceil(key_tiles / s) * each + 3.0 + (s > 1 ? 1.0 : 0.0));
+    if (room[s] <= 0) continue;
+    const double cost = ceil(static_cast<double>(units) / room[s]) * (ceil(key_tiles / s) * each + kTileSetUp + (s > 1 ? 1.0 : 0.0));
     if (cost < best) {
       best = cost;
       splits = s;

@@ -32,6 +32,7 @@ constexpr int kTileSeen = 8;
 constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 184, kTileLoadRegs = 88, kTileIssueRegs = 56;
 static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
 constexpr uint32_t kTileBytes = 128 * 128;                        // 128 rows of 64 16-bit values
+constexpr int kTileWeights = 2 * (kTileRows + 8);                  // rows of a block times parts: rounded up for 8 blocks and two streams
 constexpr uint32_t kTileTmemCols = 512;
 // tensor memory of stream t: scores, probabilities (pairs), output
 __host__ __device__ constexpr uint32_t tile_s_col(int t) { return 128u * t; }
@@ -39,7 +40,7 @@ __host__ __device__ constexpr uint32_t tile_p_col(int t) { return 256u + 64u * t
 __host__ __device__ constexpr uint32_t tile_o_col(int t) { return 384u + 64u * t; }
 
 struct TileSmem {
-  uint32_t q, k, v, tables, seen, max, sum, bars, total;
+  uint32_t q, k, v, tables, seen, max, sum, weight, offset, bars, total;
 };
 __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
   TileSmem s = {};
@@ -50,7 +51,9 @@ __host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
   s.seen = s.tables + (packed ? 2 * kPairTableBytes : 0);
   s.max = s.seen + kTileSeen * 16;
   s.sum = s.max + 2 * kTileRows * 4;
-  s.bars = s.sum + 2 * kTileRows * 4;
+  s.weight = s.sum + 2 * kTileRows * 4;                           // of a part in a row's result
+  s.offset = s.weight + kTileWeights * 4;                         // of a row in the result
+  s.bars = s.offset + 2 * kTileRows * 8;
   s.total = s.bars + 32 * 8 + 1024;                               // and alignment
   return s;
 }
@@ -84,6 +87,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [tile % kTileSeen][warp]: written before the tile's keys are handed over
   float* const s_max = reinterpret_cast<float*>(smem + L.max);                    // [stream][row]
   float* const s_sum = reinterpret_cast<float*>(smem + L.sum);
+  float* const s_weight = reinterpret_cast<float*>(smem + L.weight);
+  long long* const s_offset = reinterpret_cast<long long*>(smem + L.offset);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t polls = p.poll_limit;
 
@@ -105,15 +110,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     pdl_launch_dependents();
     return;
   }
-  if (tid == 0) {
+  if (tid == 13 * 32) {
     const int users = halves ? 2 : 1;                                             // streams that read a tile of keys
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
       mbar_init(k_free + i, users); mbar_init(v_free + i, users);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(q_full + t, 4); mbar_init(s_read + t, 4); mbar_init(p_full + t, 4);
+      mbar_init(s_read + t, 4); mbar_init(p_full + t, 4);
       mbar_init(s_full + t, 1); mbar_init(o_done + t, 1);
+      mbar_init(q_full + t, halves ? 4 : 8);
     }
     mbar_init(stopped, 2);
     mbar_fence_init();
@@ -181,10 +187,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     fewer_registers<kTileLoadRegs>();
     const int w = warp - 8;
     const uint32_t k_smem = smem_u32(smem) + L.k + w * 4096, v_smem = smem_u32(smem) + L.v + w * 4096;
-    // where the two sixteens of keys of the warp lie, each in one page; looked up a tile ahead, as are the masks
-    int page[2];
-    bool masked = true;
-    auto look_up = [&](int j) {
+    // where the two sixteens of keys of the warp lie, each in one page; looked up two tiles ahead, as are the masks
+    int page[2] = {0, 0}, page_after[2] = {0, 0};
+    bool masked = true, masked_after = true;
+    auto look_up = [&](int j, int (&page)[2], bool& masked) {
+      masked = true;
       const int base = (first + j) * kTileKeys + 32 * w;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -214,7 +221,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       }
       pl.seen = __ballot_sync(0xffffffffu, base + lane < keys && (lane < 16 ? there[0] : there[1]) && masked);
       if (lane == 0) s_seen[j % kTileSeen * 4 + w] = pl.seen;
-      if (j + 1 < count) look_up(j + 1);
+      page[0] = page_after[0];
+      page[1] = page_after[1];
+      masked = masked_after;
+      if (j + 2 < count) look_up(j + 2, page_after, masked_after);
       return pl;
     };
     // a slot's phase that the products have to have ended
@@ -226,7 +236,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    if (count > 0) look_up(0);
+    if (count > 0) look_up(0, page, masked);
+    if (count > 1) look_up(1, page_after, masked_after);
     if constexpr (!PACKED) {
       // 16 bits: eight lanes a row, asynchronous copies.  A tile is handed over before a slot is waited for: the slot may be freed by a product
       // that is issued behind one with that tile.  Where the slots are free already, the copies go first.
@@ -350,31 +361,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const int at = row0 + (halves ? t * kTileRows : 0) + r;                       // of the sequence's rows
     const bool live = at < row0 + rows;
-    const int i_query = at / p.group, head = kvh * p.group + at % p.group;
-    const int limit = !live ? 0 : p.causal ? min(seq.keys, max(seq.keys - seq.all_queries + i_query + 1, 0)) : seq.keys;
-    float scale = p.scale_log2;
-    // ---- the row of queries; without halves the second stream's are the first's
-    if (halves || t == 0) {
-      uint32_t w[32];
+    const int limit = !live ? 0 : p.causal ? min(seq.keys, max(seq.keys - seq.all_queries + at / p.group + 1, 0)) : seq.keys;
+    // ---- the queries, eight lanes a row: a stream its own, without halves (the second stream's are the first's) both half of them; what their
+    // products are scaled by goes through s_max
+    {
+      uint4 u[8];
+      const int c = lane & 7, of = halves ? 8 : 4, first_row = halves ? t * kTileRows : t * 64;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (live) u = reinterpret_cast<const uint4*>(attend_query(p, seq, b, i_query, head))[c];
-        w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
+      for (int k = 0; k < 8; ++k) {
+        const int q = first_row + k * 16 + quarter * 4 + (lane >> 3), row = row0 + q;
+        u[k] = make_uint4(0, 0, 0, 0);
+        if (k < of && q < rows) u[k] = reinterpret_cast<const uint4*>(attend_query(p, seq, b, row / p.group, kvh * p.group + row % p.group))[c];
       }
-      if (PACKED && p.q_bf16) scale *= bf16_to_half(w, 32, bf16_top(w, 32));
-      const uint32_t dst = smem_u32(smem) + L.q + t * kTileBytes + r * 128;
-      row_store<1>(w, dst, r & 7);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= of) break;
+        const int q = first_row + k * 16 + quarter * 4 + (lane >> 3);
+        float factor = p.scale_log2;
+        if (PACKED && p.q_bf16) {
+          uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+          float largest = bf16_top(w, 4);
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, d));
+          factor *= bf16_to_half(w, 4, largest);
+          u[k] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        sts128(smem_u32(smem) + L.q + q * 128 + ((c ^ (q & 7)) << 4), u[k].x, u[k].y, u[k].z, u[k].w);
+        if (c == 0) s_max[q] = factor;
+      }
       fence_proxy_async_smem();
-      if (!halves) s_max[r] = scale;
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full + t);
+      if (lane == 0) mbar_arrive(q_full + (halves ? t : 0));
     }
-    if (!halves) {
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      scale = s_max[r];
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float scale = s_max[halves ? t * kTileRows + r : r];
+    asm volatile("bar.sync 1, 256;" ::: "memory");                                // all have read theirs: s_max is free again
     const int mine = halves ? count : (count + 1 - t) / 2;
     const float ninf = __int_as_float(0xff800000);
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -524,37 +545,48 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   }
   if (warp == 12) tmem_dealloc(tmem, kTileTmemCols);
   if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-  // four values a thread; the rows are shared out over the blocks of the cluster
+  // The rows are shared out over the blocks of the cluster: first what each part counts in a row and where the row goes, then four values a
+  // thread.
   {
-    const int share = (rows + p.splits - 1) / p.splits, from = split * share, to = min(rows, from + share);
+    const int share = (rows + p.splits - 1) / p.splits, from = min(split * share, rows), mine = min(share, rows - from);
     const int parts = (halves ? 1 : 2) * p.splits;
-    for (int e = from * 16 + tid; e < to * 16; e += kTileThreads) {
-      const int r = e >> 4, c = e & 15;
+    auto address = [&](int q, int r, uint32_t offset, int row_bytes) {
+      const int rank = halves ? q : q >> 1, t = halves ? r >> 7 : q & 1;
+      uint32_t d;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(smem) + offset + (t * kTileRows + (r & 127)) * row_bytes), "r"(rank));
+      return d;
+    };
+    if (tid < mine) {
+      const int r = from + tid, at = row0 + r;
       float m = __int_as_float(0xff800000), l = 0.0f;
-      float4 o = make_float4(0, 0, 0, 0);
-      auto address = [&](int q, uint32_t offset, int stream_bytes) {
-        const int rank = halves ? q : q >> 1, t = halves ? r >> 7 : q & 1;
-        uint32_t a = smem_u32(smem) + offset + t * stream_bytes, d;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(rank));
-        return d;
-      };
-      const int rr = r & 127;
-      for (int q = 0; q < parts; ++q) m = fmaxf(m, lds_cluster(address(q, L.max, kTileRows * 4) + rr * 4));
+#pragma unroll 1
+      for (int q = 0; q < parts; ++q) m = fmaxf(m, lds_cluster(address(q, r, L.max, 4)));
       const float base = m == __int_as_float(0xff800000) ? 0.0f : m;
+#pragma unroll 1
       for (int q = 0; q < parts; ++q) {
-        const float f = exp2_approx(lds_cluster(address(q, L.max, kTileRows * 4) + rr * 4) - base);
-        l += f * lds_cluster(address(q, L.sum, kTileRows * 4) + rr * 4);
-        const float4 v = lds128_cluster(address(q, L.k, kTileRows * 256) + rr * 256 + ((c ^ (rr & 7)) << 4));
+        const float f = exp2_approx(lds_cluster(address(q, r, L.max, 4)) - base);
+        l += f * lds_cluster(address(q, r, L.sum, 4));
+        s_weight[tid * parts + q] = f;
+      }
+      const float inv = inverse_sum(l);
+#pragma unroll 1
+      for (int q = 0; q < parts; ++q) s_weight[tid * parts + q] *= inv;
+      s_offset[tid] = ((static_cast<long long>(seq.first_row) + at / p.group) * p.heads + kvh * p.group + at % p.group) * 64;
+    }
+    __syncthreads();
+    for (int e = tid; e < mine * 16; e += kTileThreads) {
+      const int i = e >> 4, r = from + i, c = e & 15;
+      float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+      for (int q = 0; q < parts; ++q) {
+        const float f = s_weight[i * parts + q];
+        const float4 v = lds128_cluster(address(q, r, L.k, 256) + ((c ^ (r & 7)) << 4));
         o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
       }
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);             // a query that sees no key: zeros; NaN stays NaN
-      const int at = row0 + r;
-      const long long token = seq.first_row + at / p.group;
-      const long long dst = (token * p.heads + kvh * p.group + at % p.group) * 64 + 4 * c;
-      const f32x2 lo = pack2(o.x * inv, o.y * inv), hi = pack2(o.z * inv, o.w * inv);
+      const f32x2 lo = pack2(o.x, o.y), hi = pack2(o.z, o.w);
       const uint2 u = p.q_bf16 ? make_uint2(pair_to_sixteen<__nv_bfloat16>(lo), pair_to_sixteen<__nv_bfloat16>(hi))
                                : make_uint2(pair_to_sixteen<__half>(lo), pair_to_sixteen<__half>(hi));
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + dst) = u;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + s_offset[i] + 4 * c) = u;
     }
   }
   __syncwarp();

@@ -154,7 +154,7 @@ constexpr int kWholeUnitSteps = 48;
 
 template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
-  auto join = arcq::join_attention_kernel<arcq::SplitStep<BITS>::kKeys>;
+  auto join = arcq::join_attention_kernel<arcq::SplitUnits<arcq::SplitStep<BITS>::kKeys>>;
   constexpr size_t smem = arcq::split_parts<BITS>() + arcq::kSplitSharedParts + 128;
   static_assert(smem + arcq::kSplitBase <= 227 * 1024, "");
   static thread_local int done_dev = -1;

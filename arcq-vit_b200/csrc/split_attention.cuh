@@ -234,40 +234,45 @@ template <int BITS, int I> __device__ __forceinline__ uint32_t table_address(uin
 }
 
 // ---------------------------------------------------------------- units and their line
+// U: how many rows a unit has and how many steps it takes
+template <int KEYS> struct SplitUnits {
+  static constexpr int kRows = kSplitRows;
+  static __device__ __forceinline__ int steps(int, int keys) { return max((keys + KEYS - 1) / KEYS, 1); }      // without keys a step, in which nothing is seen
+};
 struct SplitUnit {
   int b, kvh, tile;
   AttendSequence seq;
   int rows, keys, steps;
 };
-__device__ __forceinline__ int split_tiles(const AttendParams& p, const AttendSequence& s) {
-  return static_cast<int>((static_cast<long long>(s.queries) * p.group + kSplitRows - 1) / kSplitRows);
+template <typename U> __device__ __forceinline__ int split_tiles(const AttendParams& p, const AttendSequence& s) {
+  return static_cast<int>((static_cast<long long>(s.queries) * p.group + U::kRows - 1) / U::kRows);
 }
-template <int KEYS> __device__ __forceinline__ void split_tile(const AttendParams& p, SplitUnit& u) {
-  u.rows = static_cast<int>(min(static_cast<long long>(u.seq.queries) * p.group - static_cast<long long>(u.tile) * kSplitRows, static_cast<long long>(kSplitRows)));
+template <typename U> __device__ __forceinline__ void split_tile(const AttendParams& p, SplitUnit& u) {
+  u.rows = static_cast<int>(min(static_cast<long long>(u.seq.queries) * p.group - static_cast<long long>(u.tile) * U::kRows, static_cast<long long>(U::kRows)));
   u.keys = u.seq.keys;
-  if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * kSplitRows + u.rows - 1) / p.group + 1, 0));
-  u.steps = max((u.keys + KEYS - 1) / KEYS, 1);                                   // a unit without keys has a step, in which nothing is seen
+  if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * U::kRows + u.rows - 1) / p.group + 1, 0));
+  u.steps = U::steps(u.rows, u.keys);
 }
 // steps of all units of a sequence
-template <int KEYS> __device__ __forceinline__ long long split_sequence_steps(const AttendParams& p, int b) {
+template <typename U> __device__ __forceinline__ long long split_sequence_steps(const AttendParams& p, int b) {
   SplitUnit u;
   u.seq = attend_sequence(p, b);
-  const int tiles = split_tiles(p, u.seq);
+  const int tiles = split_tiles<U>(p, u.seq);
   long long n = 0;
   for (u.tile = 0; u.tile < tiles; ++u.tile) {
-    split_tile<KEYS>(p, u);
+    split_tile<U>(p, u);
     n += u.steps;
   }
   return n * p.kv_heads;
 }
-// The unit after (b, kvh, tile); behind the last one: b = batch.  What the kernel keeps of a unit while it works on it is little.
-template <int KEYS> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
+// The unit after (b, kvh, tile); behind the last one: b = batch.  What a kernel keeps of a unit while it works on it is little.
+template <typename U> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
   SplitUnit u;
   u.b = b;
   u.kvh = kvh;
   u.tile = tile + 1;
   u.seq = attend_sequence(p, b);
-  if (u.tile >= split_tiles(p, u.seq)) {
+  if (u.tile >= split_tiles<U>(p, u.seq)) {
     u.tile = 0;
     if (++u.kvh == p.kv_heads) {
       u.kvh = 0;
@@ -278,9 +283,69 @@ template <int KEYS> __device__ __forceinline__ SplitUnit split_next(const Attend
       if (u.b >= p.batch) return u;
     }
   }
-  split_tile<KEYS>(p, u);
+  split_tile<U>(p, u);
   return u;
 }
+__device__ __forceinline__ long long divide_steps(long long a, long long b) {      // of non-negative numbers, mostly small ones
+  return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
+}
+// The line: each of a block's threads has a share of the sequences, before[tid] steps are before it.
+template <typename U, int THREADS> struct SplitLine {
+  long long* before;
+  int share;
+  long long total;
+  // whole block; of_warps: shared memory for a number a warp
+  __device__ __forceinline__ SplitLine(const AttendParams& p, long long* before_, long long* of_warps) : before(before_) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    share = (p.batch + THREADS - 1) / THREADS;
+    long long mine = 0;
+    for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_sequence_steps<U>(p, b);
+    long long sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 31) of_warps[warp] = sum;
+    __syncthreads();
+    total = 0;
+    long long base = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) base += of_warps[w];
+      total += of_warps[w];
+    }
+    before[tid] = base + sum - mine;
+    __syncthreads();
+  }
+  // the unit that step x is in, and the unit's first step
+  __device__ __forceinline__ SplitUnit locate(const AttendParams& p, long long x, long long& at) const {
+    SplitUnit u;
+    int lo = 0, hi = THREADS - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    at = before[lo];
+    for (u.b = lo * share;; ++u.b) {
+      const long long n = split_sequence_steps<U>(p, u.b);
+      if (at + n > x) {
+        const long long of_head = divide_steps(n, p.kv_heads);
+        u.kvh = static_cast<int>(divide_steps(x - at, of_head));
+        at += u.kvh * of_head;
+        break;
+      }
+      at += n;
+    }
+    u.seq = attend_sequence(p, u.b);
+    for (u.tile = 0;; ++u.tile) {
+      split_tile<U>(p, u);
+      if (at + u.steps > x) break;
+      at += u.steps;
+    }
+    return u;
+  }
+};
 
 // A part of a unit: for each of its rows 64 outputs, maximum and sum.  A warp has two of them (of a unit that began before its piece, and of one
 // that goes on behind it), in shared memory where they fit, and so has a block, in the workspace: a header, a record for each unit, the blocks'
@@ -364,61 +429,18 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid, kSplitThreads);
   pdl_wait();
 
-  // ---- the line of steps: each thread a share of the sequences, a scan over the block
-  const int share = (p.batch + kSplitThreads - 1) / kSplitThreads;
-  long long mine = 0;
-  for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_sequence_steps<KEYS>(p, b);
-  long long before = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += o;
-  }
-  if (lane == 31) s_scan[warp] = before;
-  __syncthreads();
-  long long total = 0, base_of_warp = 0;
-#pragma unroll
-  for (int w = 0; w < kSplitWarps; ++w) {
-    if (w < warp) base_of_warp += s_scan[w];
-    total += s_scan[w];
-  }
-  s_line[tid] = base_of_warp + before - mine;
-  __syncthreads();
-  // the unit that a step of the line is in, and the unit's first step
-  auto locate = [&](long long x, long long& at) {
-    SplitUnit u;
-    int lo = 0, hi = kSplitThreads - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_line[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    at = s_line[lo];
-    for (u.b = lo * share;; ++u.b) {
-      const long long n = split_sequence_steps<KEYS>(p, u.b);
-      if (at + n > x) {
-        u.kvh = static_cast<int>((x - at) / (n / p.kv_heads));
-        at += u.kvh * (n / p.kv_heads);
-        break;
-      }
-      at += n;
-    }
-    u.seq = attend_sequence(p, u.b);
-    for (u.tile = 0;; ++u.tile) {
-      split_tile<KEYS>(p, u);
-      if (at + u.steps > x) break;
-      at += u.steps;
-    }
-    return u;
-  };
+  using Units = SplitUnits<KEYS>;
+  const SplitLine<Units, kSplitThreads> line(p, s_line, s_scan);
+  const long long total = line.total;
   // ---- the block's piece of the line, and the warp's
-  const long long piece = max((total + gridDim.x - 1) / gridDim.x, 1ll);
+  const long long piece = max(divide_steps(total + gridDim.x - 1, gridDim.x), 1ll);
   long long from = min(blockIdx.x * piece, total), to = min(from + piece, total);
   if (p.whole_units) {                                                             // the units that begin in the piece
     if (warp < 2) {
       const long long x = warp == 0 ? from : to;
       long long at = x;
       if (x < total) {
-        const SplitUnit u = locate(x, at);
+        const SplitUnit u = line.locate(p, x, at);
         if (at < x) at += u.steps;
       }
       if (lane == 0) s_scan[warp] = at;
@@ -440,7 +462,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   __syncthreads();
   if (start < end) {
   long long at;
-  SplitUnit u = locate(start, at);
+  SplitUnit u = line.locate(p, start, at);
 
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
   // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest
@@ -534,7 +556,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       f_slot = f_slot + 1 == kSplitStages ? 0 : f_slot + 1;
       if (--f_left > 0) {
         if (++f_step == f.steps) {
-          const SplitUnit n = split_next<KEYS>(p, f.b, f.kvh, f.tile);
+          const SplitUnit n = split_next<Units>(p, f.b, f.kvh, f.tile);
           f = {n.b, n.kvh, n.tile, n.keys, n.steps};
           f_step = run = 0;
           look_up(0);
@@ -870,7 +892,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     at += u.steps;
-    if (step < steps) u = split_next<KEYS>(p, u.b, u.kvh, u.tile);
+    if (step < steps) u = split_next<Units>(p, u.b, u.kvh, u.tile);
   }
   cp_async_wait<0>();
   }
@@ -895,9 +917,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   }
 }
 
-// Adds up the blocks' parts of the units that lie in more than one block's piece: a block a unit.
-constexpr int kJoinThreads = kSplitRows * 16;
-template <int KEYS> __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
+// Adds up the blocks' parts of the units that lie in more than one block's piece: a block a unit, four values of a row a thread.
+constexpr int kJoinThreads = 256;
+template <typename U> __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
   pdl_launch_dependents();
   const long long unit = blockIdx.x;
   SplitUnit u;
@@ -908,15 +930,16 @@ template <int KEYS> __global__ void __launch_bounds__(kJoinThreads) join_attenti
   const SplitRecord rec = split_records(p)[unit];                                  // not written where there is no such tile
   const long long piece = static_cast<SplitHeader*>(p.workspace)->piece;
   u.seq = attend_sequence(p, u.b);
-  if (u.tile >= split_tiles(p, u.seq) || rec.whole) return;
-  split_tile<KEYS>(p, u);
-  const int tid = threadIdx.x, row = tid >> 4, column = tid & 15;
-  if (row >= u.rows) return;
-  const long long first = rec.start / piece, last = (rec.start + rec.steps - 1) / piece;
-  float top, sum;
-  const float4 o = add_parts(static_cast<int>(last - first + 1), row, column, top, sum,
-                             [&](int q) { return split_part(p, 2 * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
-  write_four(p, u.seq.first_row, u.kvh, u.tile * kSplitRows + row, column, o, inverse_sum(sum));
+  if (u.tile >= split_tiles<U>(p, u.seq) || rec.whole) return;
+  split_tile<U>(p, u);
+  const long long first = divide_steps(rec.start, piece), last = divide_steps(rec.start + rec.steps - 1, piece);
+  for (int e = threadIdx.x; e < u.rows * 16; e += kJoinThreads) {
+    const int row = e >> 4, column = e & 15;
+    float top, sum;
+    const float4 o = add_parts(static_cast<int>(last - first + 1), row, column, top, sum,
+                               [&](int q) { return split_part(p, 2 * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
+    write_four(p, u.seq.first_row, u.kvh, u.tile * U::kRows + row, column, o, inverse_sum(sum));
+  }
 }
 
 }  // namespace arcq

@@ -176,7 +176,7 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
   if (p.workspace == nullptr || workspace_bytes < arcq::split_workspace(p, sms))
     return fail(ARCQ_E_BAD_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)arcq::split_workspace(p, sms));
   const long long units = arcq::split_units(p), steps = units * (p.max_keys / arcq::SplitStep<BITS>::kKeys + 1);
-  if (units > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
+  if (steps > 0x3fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries and keys for one call");
   p.whole_units = p.max_keys <= kWholeUnitSteps * arcq::SplitStep<BITS>::kKeys;
   cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
   if (e == cudaSuccess && !p.whole_units) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);

@@ -253,17 +253,17 @@ template <typename U> __device__ __forceinline__ void split_tile(const AttendPar
   if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * U::kRows + u.rows - 1) / p.group + 1, 0));
   u.steps = U::steps(u.rows, u.keys);
 }
-// steps of all units of a sequence
-template <typename U> __device__ __forceinline__ long long split_sequence_steps(const AttendParams& p, int b) {
+// steps of all units of a sequence and key head
+template <typename U> __device__ __forceinline__ int split_head_steps(const AttendParams& p, const AttendSequence& seq) {
   SplitUnit u;
-  u.seq = attend_sequence(p, b);
+  u.seq = seq;
   const int tiles = split_tiles<U>(p, u.seq);
-  long long n = 0;
+  int n = 0;
   for (u.tile = 0; u.tile < tiles; ++u.tile) {
     split_tile<U>(p, u);
     n += u.steps;
   }
-  return n * p.kv_heads;
+  return n;
 }
 // The unit after (b, kvh, tile); behind the last one: b = batch.  What a kernel keeps of a unit while it works on it is little.
 template <typename U> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
@@ -286,58 +286,70 @@ template <typename U> __device__ __forceinline__ SplitUnit split_next(const Atte
   split_tile<U>(p, u);
   return u;
 }
-__device__ __forceinline__ long long divide_steps(long long a, long long b) {      // of non-negative numbers, mostly small ones
-  return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
-}
-// The line: each of a block's threads has a share of the sequences, before[tid] steps are before it.
+// The line: each of a block's threads has a share of the sequences, `mine` steps, with `before` steps before them.  Where all sequences are alike
+// `mine` is a sequence's.  (The host keeps the line below 2^30 steps.)
 template <typename U, int THREADS> struct SplitLine {
-  long long* before;
-  int share;
-  long long total;
+  int share, total, mine, before;
+  bool alike;
   // whole block; of_warps: shared memory for a number a warp
-  __device__ __forceinline__ SplitLine(const AttendParams& p, long long* before_, long long* of_warps) : before(before_) {
+  __device__ __forceinline__ SplitLine(const AttendParams& p, int* of_warps) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    alike = p.lengths == nullptr && p.starts == nullptr;
     share = (p.batch + THREADS - 1) / THREADS;
-    long long mine = 0;
-    for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_sequence_steps<U>(p, b);
-    long long sum = mine;
+    if (alike) {
+      mine = split_head_steps<U>(p, attend_sequence(p, 0)) * p.kv_heads;
+      total = mine * p.batch;
+      before = 0;
+      return;
+    }
+    mine = 0;
+    for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_head_steps<U>(p, attend_sequence(p, b)) * p.kv_heads;
+    int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
     if (lane == 31) of_warps[warp] = sum;
     __syncthreads();
     total = 0;
-    long long base = 0;
+    before = sum - mine;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) base += of_warps[w];
-      total += of_warps[w];
+      const int n = of_warps[w];
+      if (w < warp) before += n;
+      total += n;
     }
-    before[tid] = base + sum - mine;
-    __syncthreads();
+  }
+  // Whose share step x(i) is in, and the steps before that share; for locate, behind a barrier.
+  template <typename X> __device__ __forceinline__ void find(int count, X x, int2* found) const {
+    if (alike || mine == 0) return;
+    for (int i = 0; i < count; ++i) {
+      const int v = x(i) - before;
+      if (v >= 0 && v < mine) found[i] = make_int2(threadIdx.x, before);
+    }
   }
   // the unit that step x is in, and the unit's first step
-  __device__ __forceinline__ SplitUnit locate(const AttendParams& p, long long x, long long& at) const {
+  __device__ __forceinline__ SplitUnit locate(const AttendParams& p, int x, const int2* found, int& at) const {
     SplitUnit u;
-    int lo = 0, hi = THREADS - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (before[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    at = before[lo];
-    for (u.b = lo * share;; ++u.b) {
-      const long long n = split_sequence_steps<U>(p, u.b);
-      if (at + n > x) {
-        const long long of_head = divide_steps(n, p.kv_heads);
-        u.kvh = static_cast<int>(divide_steps(x - at, of_head));
-        at += u.kvh * of_head;
-        break;
+    int of_head;
+    if (alike) {
+      u.b = x / mine;
+      at = u.b * mine;
+      u.seq = attend_sequence(p, u.b);
+      of_head = mine / p.kv_heads;
+    } else {
+      u.b = found->x * share;
+      at = found->y;
+      for (;; ++u.b) {
+        u.seq = attend_sequence(p, u.b);
+        of_head = split_head_steps<U>(p, u.seq);
+        if (at + of_head * p.kv_heads > x) break;
+        at += of_head * p.kv_heads;
       }
-      at += n;
     }
-    u.seq = attend_sequence(p, u.b);
+    u.kvh = (x - at) / max(of_head, 1);
+    at += u.kvh * of_head;
     for (u.tile = 0;; ++u.tile) {
       split_tile<U>(p, u);
       if (at + u.steps > x) break;
@@ -351,11 +363,10 @@ template <typename U, int THREADS> struct SplitLine {
 // that goes on behind it), in shared memory where they fit, and so has a block, in the workspace: a header, a record for each unit, the blocks'
 // parts, and the warps' where shared memory is too small.
 struct SplitHeader {
-  long long piece, unused;                                                        // steps of a block
+  int piece, unused[3];                                                           // steps of a block
 };
 struct SplitRecord {
-  long long start;
-  int steps, whole;
+  int start, steps, whole, unused;
 };
 constexpr int kSplitPartRow = 68, kSplitSharedRows = 8;                            // rows of parts in shared memory
 constexpr uint32_t kSplitSharedParts = 2 * kSplitWarps * kSplitSharedRows * kSplitPartRow * 4;
@@ -374,6 +385,9 @@ __device__ __forceinline__ float* split_part(const AttendParams& p, long long sl
 // The parts of one unit added up in the order of the keys, four values of a row a thread (the first rows * 16 threads).  next(i): part i.
 template <typename Next> __device__ __forceinline__ float4 add_parts(int count, int row, int column, float& top, float& sum, Next next) {
   top = __int_as_float(0xff800000);
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) top = fmaxf(top, next(i)[row * kSplitPartRow + 64]);
+  const float base = top == __int_as_float(0xff800000) ? 0.0f : top;
   sum = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 4
@@ -381,10 +395,9 @@ template <typename Next> __device__ __forceinline__ float4 add_parts(int count, 
     const float* const part = next(i) + row * kSplitPartRow;
     const float2 ts = *reinterpret_cast<const float2*>(part + 64);
     const float4 x = *reinterpret_cast<const float4*>(part + 4 * column);
-    const float m = fmaxf(top, ts.x), base = m == __int_as_float(0xff800000) ? 0.0f : m, fa = exp2_approx(top - base), fb = exp2_approx(ts.x - base);
-    top = m;
-    sum = sum * fa + ts.y * fb;
-    o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
+    const float f = exp2_approx(ts.x - base);
+    sum += ts.y * f;
+    o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
   }
   return o;
 }
@@ -420,55 +433,56 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   using Step = SplitStep<BITS>;
   constexpr int KEYS = Step::kKeys, NT = KEYS / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_scan[kSplitThreads / 32], s_line[kSplitThreads];         // steps before each share of the sequences
+  __shared__ int s_scan[kSplitWarps], s_ends[2];
+  __shared__ int2 s_found[kSplitWarps];
   __shared__ struct {
-    long long at;
-    int b, kvh, tile, rows, steps, first_row;
+    int at, b, kvh, tile, rows, steps, first_row;
   } s_groups[kSplitWarps + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid, kSplitThreads);
   pdl_wait();
 
   using Units = SplitUnits<KEYS>;
-  const SplitLine<Units, kSplitThreads> line(p, s_line, s_scan);
-  const long long total = line.total;
+  const SplitLine<Units, kSplitThreads> line(p, s_scan);
   // ---- the block's piece of the line, and the warp's
-  const long long piece = max(divide_steps(total + gridDim.x - 1, gridDim.x), 1ll);
-  long long from = min(blockIdx.x * piece, total), to = min(from + piece, total);
+  const int piece = max(static_cast<int>((static_cast<unsigned>(line.total) + gridDim.x - 1) / gridDim.x), 1);
+  int from = static_cast<int>(min(static_cast<long long>(blockIdx.x) * piece, static_cast<long long>(line.total))), to = min(piece, line.total - from) + from;
   if (p.whole_units) {                                                             // the units that begin in the piece
+    line.find(2, [&](int i) { return i == 0 ? from : to; }, s_found);
+    __syncthreads();
     if (warp < 2) {
-      const long long x = warp == 0 ? from : to;
-      long long at = x;
-      if (x < total) {
-        const SplitUnit u = line.locate(p, x, at);
+      const int x = warp == 0 ? from : to;
+      int at = x;
+      if (x < line.total) {
+        const SplitUnit u = line.locate(p, x, s_found + warp, at);
         if (at < x) at += u.steps;
       }
-      if (lane == 0) s_scan[warp] = at;
+      if (lane == 0) s_ends[warp] = at;
     }
     __syncthreads();
-    from = s_scan[0];
-    to = s_scan[1];
+    from = s_ends[0];
+    to = s_ends[1];
   } else if (blockIdx.x == 0 && tid == 0) {
     static_cast<SplitHeader*>(p.workspace)->piece = piece;
   }
   if (from >= to) return;
-  const int per = static_cast<int>((to - from + kSplitWarps - 1) / kSplitWarps);
-  const long long start = min(from + static_cast<long long>(warp) * per, to), end = min(start + per, to);
+  const int per = (to - from + kSplitWarps - 1) / kSplitWarps, start = min(from + warp * per, to), end = min(start + per, to);
   // parts of this block's warps; the units they are of, by the warp that has the first: 0 .. (begun there), kSplitWarps (before the block's piece)
   float* const parts = p.part_rows <= kSplitSharedRows ? reinterpret_cast<float*>(smem + split_parts<BITS>() - (PACKED ? smem_u32(smem) : 0))
                                                        : split_part(p, 2ll * gridDim.x + 2ll * kSplitWarps * blockIdx.x);
   const int part_size = p.part_rows * kSplitPartRow;
   if (tid <= kSplitWarps) s_groups[tid].rows = 0;
+  line.find(kSplitWarps, [&](int w) { return from + w * per; }, s_found);
   __syncthreads();
   if (start < end) {
-  long long at;
-  SplitUnit u = line.locate(p, start, at);
+  int at;
+  SplitUnit u = line.locate(p, start, s_found + warp, at);
 
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
   // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest
   // of a page, or of an image's states; the page after it is looked up when it begins.
   struct { int b, kvh, tile, keys, steps; } f = {u.b, u.kvh, u.tile, u.keys, u.steps};
-  int f_step = static_cast<int>(start - at), f_left = static_cast<int>(end - start), f_slot = 0;
+  int f_step = start - at, f_left = end - start, f_slot = 0;
   int run = 0, next_page = 0;                                                      // sixteens of the run that are left
   bool valid = false, masked = true;
   const uint8_t *fk = p.k.rows, *fv = p.v.rows, *fs = reinterpret_cast<const uint8_t*>(p.k.stats);      // the lane's 16 bytes of the next sixteen
@@ -567,6 +581,28 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     cp_async_commit();
     return seen;
   };
+  // rows g and g + 8 of a unit's queries: values 16c .. 16c + 15 (packed), 8n + 2c and the next (16 bits); the first unit's before the copies
+  uint32_t qw[2][8];
+  auto load_queries = [&] {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool row = g + 8 * h < u.rows;
+      const int r = u.tile * kSplitRows + (row ? g + 8 * h : 0);
+      const uint16_t* const src = attend_query(p, u.seq, u.b, r / p.group, u.kvh * p.group + r % p.group);
+      if constexpr (PACKED) {
+        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
+        if (row) {
+          u0 = reinterpret_cast<const uint4*>(src + 16 * c)[0];
+          u1 = reinterpret_cast<const uint4*>(src + 16 * c)[1];
+        }
+        qw[h][0] = u0.x; qw[h][1] = u0.y; qw[h][2] = u0.z; qw[h][3] = u0.w; qw[h][4] = u1.x; qw[h][5] = u1.y; qw[h][6] = u1.z; qw[h][7] = u1.w;
+      } else {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) qw[h][n] = row ? *reinterpret_cast<const uint32_t*>(src + 8 * n + 2 * c) : 0u;
+      }
+    }
+  };
+  load_queries();
   uint32_t seen_now, seen_next = copy_step(), seen_after = copy_step();
 
   // ---- units
@@ -578,7 +614,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   const uint32_t k_lane = (g >> 1) * (8 * Step::kRow + Step::kPad) + 2 * (g & 1) * Step::kRow;
   const uint32_t v_lane = Step::kRows + c * (8 * Step::kRow + Step::kPad);
   int step = 0, slot = 0;                                                          // of the piece
-  const int steps = static_cast<int>(end - start);
+  const int steps = end - start;
   while (step < steps) {
     // rows g and g + 8 of the unit: queries, the keys that they see, the factor of their scores
     int limit[2];
@@ -586,18 +622,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     float row_scale[2] = {p.scale_log2, p.scale_log2}, q_sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool row = g + 8 * h < u.rows;
-      const int r = u.tile * kSplitRows + (row ? g + 8 * h : 0), i = r / p.group, head = u.kvh * p.group + r % p.group;
+      const int i = (u.tile * kSplitRows + (g + 8 * h < u.rows ? g + 8 * h : 0)) / p.group;
       limit[h] = p.causal ? min(u.seq.keys, max(u.seq.keys - u.seq.all_queries + i + 1, 0)) : u.seq.keys;
-      const uint16_t* const src = attend_query(p, u.seq, u.b, i, head);
-      uint32_t w[8];
-      if constexpr (PACKED) {                                                      // values 16c .. 16c + 15
-        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-        if (row) {
-          u0 = reinterpret_cast<const uint4*>(src + 16 * c)[0];
-          u1 = reinterpret_cast<const uint4*>(src + 16 * c)[1];
-        }
-        w[0] = u0.x; w[1] = u0.y; w[2] = u0.z; w[3] = u0.w; w[4] = u1.x; w[5] = u1.y; w[6] = u1.z; w[7] = u1.w;
+      uint32_t* const w = qw[h];
+      if constexpr (PACKED) {
         if (p.q_bf16) {
           float top = bf16_top(w, 8);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -612,9 +640,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         x += y;
         x += __shfl_xor_sync(0xffffffffu, x, 1);
         q_sum[h] = x + __shfl_xor_sync(0xffffffffu, x, 2);
-      } else {                                                                     // values 8n + 2c and the next
-#pragma unroll
-        for (int n = 0; n < 8; ++n) w[n] = row ? *reinterpret_cast<const uint32_t*>(src + 8 * n + 2 * c) : 0u;
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -623,8 +648,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     float top[2] = {ninf, ninf}, sum[2] = {0.0f, 0.0f}, o[8][4] = {}, centers[2] = {0.0f, 0.0f};
-    const int unit_first = static_cast<int>(max(at - start, -0x40000000ll)), unit_last = static_cast<int>(min(at + u.steps, end) - start);
-    const int key_base = static_cast<int>((start - at) * KEYS);                    // key of step s: key_base + s * KEYS
+    const int unit_last = min(at + u.steps, end) - start;
+    const int key_base = (start - at) * KEYS;                    // key of step s: key_base + s * KEYS
     // the loop twice: with the upper eight rows and without, whose work would else be issued for nothing
     auto steps_of = [&](auto two) {
     constexpr bool both = decltype(two)::value;
@@ -852,9 +877,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
           for (int j = 0; j < 2; ++j) o[n][2 * h + j] += centers[h];
       }
     }
-    const bool begins = unit_first >= 0, complete = begins && at + u.steps <= end;
+    const bool begins = at >= start, complete = begins && at + u.steps <= end;
     if (lane == 0) {
-      if (complete && !p.whole_units) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, 1};
+      if (complete && !p.whole_units) split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {at, u.steps, 1, 0};
       if (!complete && (begins || warp == 0)) s_groups[begins ? warp : kSplitWarps] = {at, u.b, u.kvh, u.tile, u.rows, u.steps, u.seq.first_row};
     }
     float* const part = parts + (2 * warp + (begins ? 1 : 0)) * part_size;
@@ -892,21 +917,26 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       }
     }
     at += u.steps;
-    if (step < steps) u = split_next<Units>(p, u.b, u.kvh, u.tile);
+    if (step < steps) {
+      u = split_next<Units>(p, u.b, u.kvh, u.tile);
+      load_queries();
+    }
   }
   cp_async_wait<0>();
   }
   // ---- units that lie in more than one warp's piece
   __syncthreads();
-  for (int i = 0; i <= kSplitWarps; ++i) {
+  for (int item = tid;; item += kSplitThreads) {                                  // four values of a row of some unit
+    int i = 0, rest = item;
+    while (i <= kSplitWarps && rest >= s_groups[i].rows * 16) rest -= s_groups[i++].rows * 16;
+    if (i > kSplitWarps) break;
     const auto& u = s_groups[i];
-    if (tid >= u.rows * 16) continue;
-    const int first = i < kSplitWarps ? i : 0, last = static_cast<int>((min(u.at + u.steps, to) - 1 - from) / per), row = tid >> 4, column = tid & 15;
+    const int first = i < kSplitWarps ? i : 0, last = (min(u.at + u.steps, to) - 1 - from) / per, row = rest >> 4, column = rest & 15;
     float top, sum;
     const float4 o = add_parts(last - first + 1, row, column, top, sum, [&](int q) { return parts + (2 * (first + q) + (q == 0 && i < kSplitWarps ? 1 : 0)) * part_size; });
     const bool complete = u.at >= from && u.at + u.steps <= to;
-    if (tid == 0 && u.at >= from && !p.whole_units)
-      split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {u.at, u.steps, complete ? 1 : 0};
+    if (rest == 0 && u.at >= from && !p.whole_units)
+      split_records(p)[(static_cast<long long>(u.b) * p.kv_heads + u.kvh) * p.tiles + u.tile] = {u.at, u.steps, complete ? 1 : 0, 0};
     if (complete) {
       write_four(p, u.first_row, u.kvh, u.tile * kSplitRows + row, column, o, inverse_sum(sum));
     } else {
@@ -928,16 +958,16 @@ template <typename U> __global__ void __launch_bounds__(kJoinThreads) join_atten
   u.b = static_cast<int>(unit / p.tiles / p.kv_heads);
   pdl_wait();
   const SplitRecord rec = split_records(p)[unit];                                  // not written where there is no such tile
-  const long long piece = static_cast<SplitHeader*>(p.workspace)->piece;
+  const int piece = static_cast<SplitHeader*>(p.workspace)->piece;
   u.seq = attend_sequence(p, u.b);
   if (u.tile >= split_tiles<U>(p, u.seq) || rec.whole) return;
   split_tile<U>(p, u);
-  const long long first = divide_steps(rec.start, piece), last = divide_steps(rec.start + rec.steps - 1, piece);
+  const int first = rec.start / piece, last = (rec.start + rec.steps - 1) / piece;
   for (int e = threadIdx.x; e < u.rows * 16; e += kJoinThreads) {
     const int row = e >> 4, column = e & 15;
     float top, sum;
-    const float4 o = add_parts(static_cast<int>(last - first + 1), row, column, top, sum,
-                               [&](int q) { return split_part(p, 2 * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
+    const float4 o = add_parts(last - first + 1, row, column, top, sum,
+                               [&](int q) { return split_part(p, 2ll * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
     write_four(p, u.seq.first_row, u.kvh, u.tile * U::kRows + row, column, o, inverse_sum(sum));
   }
 }

@@ -149,8 +149,18 @@ void split_shape(arcq::AttendParams& p) {
 }
 bool few_rows(const arcq::AttendParams& p) { return static_cast<long long>(p.max_new) * p.group <= 2 * arcq::kSplitRows; }
 
-// Units of up to so many steps are not cut between blocks: no second kernel.
-constexpr int kWholeUnitSteps = 48;
+// Up to 8 rows a key head the split kernel is always ahead (12 heads, 8 rows, 4 bits: over 300 tokens 8.3 us against the tile kernel's 9.3, over 16 000
+// 20.6 against 33.7).  For 9 to 32 rows it is where keys times key heads are many.  In 4 bits, 16 rows: 96 000 of them 16.0 us against 16.9, 192 000
+// 28.8 against 33.9; below, 48 000 21.2 against 18.0; 32 rows: 384 000 32.7 against 33.0, 768 000 55 against 64.  In 16 bits, where the tile kernel
+// has no codes to look up: 192 000 34.0 against 30.1, 360 000 41.1 against 44.8.
+template <int BITS> bool split_is_ahead(const arcq::AttendParams& p) {
+  constexpr long long kMany = BITS == 16 ? 5 << 16 : 2 << 16;
+  return few_rows(p) && (static_cast<long long>(p.max_new) * p.group <= 8 || static_cast<long long>(p.batch) * p.kv_heads * p.max_keys > kMany);
+}
+
+// Over up to so many keys units are not cut between blocks, which spares the second kernel: 12 heads, 1 token, 4 bits, 512 keys 9.4 us against 11.2,
+// 1024 keys 11.5 against 13.0, 1536 keys 13.4 against 12.5; 50 sequences of up to 1024 keys 16.6 against 16.2.
+constexpr int kWholeUnitKeys = 1152;
 
 template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
@@ -177,7 +187,7 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
     return fail(ARCQ_E_BAD_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)arcq::split_workspace(p, sms));
   const long long units = arcq::split_units(p), steps = units * (p.max_keys / arcq::SplitStep<BITS>::kKeys + 1);
   if (steps > 0x3fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries and keys for one call");
-  p.whole_units = p.max_keys <= kWholeUnitSteps * arcq::SplitStep<BITS>::kKeys;
+  p.whole_units = p.max_keys <= kWholeUnitKeys;
   cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
   if (e == cudaSuccess && !p.whole_units) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
@@ -245,7 +255,7 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
 }
 
 template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
-  return few_rows(p) ? launch_split<BITS, E>(p, workspace_bytes, st) : launch_tile<BITS, E>(p, st);
+  return split_is_ahead<BITS>(p) ? launch_split<BITS, E>(p, workspace_bytes, st) : launch_tile<BITS, E>(p, st);
 }
 
 int run_attention(arcq::AttendParams& p, int bits, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {

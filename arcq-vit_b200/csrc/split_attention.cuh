@@ -132,10 +132,7 @@ __device__ __forceinline__ float bf16_to_half(uint32_t* w, int n, float top) {
   return __int_as_float((127 - up) << 23);
 }
 
-#ifndef SPLIT_WARPS
-#define SPLIT_WARPS 12
-#endif
-constexpr int kSplitWarps = SPLIT_WARPS, kSplitThreads = kSplitWarps * 32, kSplitRows = 16, kSplitStages = 3;
+constexpr int kSplitWarps = 12, kSplitThreads = kSplitWarps * 32, kSplitRows = 16, kSplitStages = 3;
 constexpr uint32_t kPairTableBytes = 256 * 32 * 4;                  // [byte][lane]
 
 // [byte][lane]: the levels of the byte's two codes, low nibble first

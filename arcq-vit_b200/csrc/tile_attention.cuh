@@ -96,10 +96,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   const int tile = p.tiles - 1 - unit / (p.kv_heads * p.batch);                   // long rows of causal keys first
   const int kvh = unit % p.kv_heads, b = unit / p.kv_heads % p.batch;
 
-  if constexpr (PACKED) {
-    fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, tid, kTileThreads);
-    fill_pair_table_f32(smem_u32(smem) + L.tables + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, tid, kTileThreads);
-  }
   pdl_wait();
   const AttendSequence seq = attend_sequence(p, b);
   const int all_rows = seq.queries * p.group;
@@ -129,10 +125,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     tmem_relinquish();
     tc_fence_before_sync();
   }
-  __syncthreads();
-  pdl_launch_dependents();
-  tc_fence_after_sync();
-  const uint32_t tmem = *s_tmem;
+  // The block's set-up ends at this barrier, which each role reaches by itself: until then the loaders look up and fetch the first keys and the
+  // softmax warps their queries, while all but the loaders fill the tables (64 blocks' worth of 577 keys under 40 queries: XXX).
+  auto fill_tables = [&](int i) {                                                 // i of 384 threads
+    if constexpr (PACKED) {
+      fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, i, kTileThreads - 128);
+      fill_pair_table_f32(smem_u32(smem) + L.tables + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, i, kTileThreads - 128);
+    }
+  };
+  auto set_up = [&] {
+    asm volatile("bar.sync 0;" ::: "memory");
+    pdl_launch_dependents();
+    tc_fence_after_sync();
+  };
   // keys that the last row sees, the block's share of their tiles
   int keys = seq.keys;
   if (p.causal) keys = min(keys, max(seq.keys - seq.all_queries + (row0 + rows - 1) / p.group + 1, 0));
@@ -144,6 +149,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   if (warp >= 12) {
     // ------------------------------------------------------------------ products: warps 12 and 13, a stream each
     fewer_registers<kTileIssueRegs>();
+    fill_tables(tid - 128);
+    set_up();
+    const uint32_t tmem = *s_tmem;
     const int t = warp - 12;
     const int mine = t > 1 ? 0 : halves ? count : (count + 1 - t) / 2;
     if (t < 2 && mine > 0) {
@@ -238,6 +246,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     };
     if (count > 0) look_up(0, page, masked);
     if (count > 1) look_up(1, page_after, masked_after);
+    if (count == 0) set_up();
     if constexpr (!PACKED) {
       // 16 bits: eight lanes a row, asynchronous copies.  A tile is handed over before a slot is waited for: the slot may be freed by a product
       // that is issued behind one with that tile.  Where the slots are free already, the copies go first.
@@ -271,6 +280,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         copy(p.k, pl.k, pl.seen, k_smem + slot * kTileBytes);
         wait_free(v_free, j);
         copy(p.v, pl.v, pl.seen, v_smem + slot * kTileBytes);
+        if (j == 0) set_up();
         if (pending) {
           cp_async_wait<3>();
           hand_over(k_full + before);
@@ -342,7 +352,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         load_row(p.k, at, is, kr);
         load_row(p.v, at, is, vr);
       };
-      if (count > 0) fetch(0);
+      if (count > 0) {
+        fetch(0);
+        set_up();
+      }
       for (int j = 0; j < count; ++j) {
         const int slot = j % SLOTS;
         const Row k = kr, v = vr;
@@ -373,6 +386,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         u[k] = make_uint4(0, 0, 0, 0);
         if (k < of && q < rows) u[k] = reinterpret_cast<const uint4*>(attend_query(p, seq, b, row / p.group, kvh * p.group + row % p.group))[c];
       }
+      fill_tables(tid);
+      set_up();
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (k >= of) break;
@@ -399,7 +414,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     const int mine = halves ? count : (count + 1 - t) / 2;
     const float ninf = __int_as_float(0xff800000);
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_at = tmem + tile_s_col(t) + lanes, p_at = tmem + tile_p_col(t) + lanes, o_at = tmem + tile_o_col(t) + lanes;
+    const uint32_t tmem = *s_tmem, s_at = tmem + tile_s_col(t) + lanes, p_at = tmem + tile_p_col(t) + lanes, o_at = tmem + tile_o_col(t) + lanes;
     const bool rows_here = __any_sync(0xffffffffu, live);
     float top = ninf;                                                             // in units of the exponent
     f32x2 sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
@@ -511,11 +526,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   tc_fence_before_sync();
   const bool gave_up = __syncthreads_or(!ok) != 0;
   tc_fence_after_sync();
+  const uint32_t tmem = *s_tmem;
   if (gave_up && tid == 12 * 32) atomicExch(p.status, kStatusTileAttentionTimeout);
   float* const part = reinterpret_cast<float*>(smem + L.k);                       // [stream][row][64], over the slots, 16-byte chunks swizzled by row
+  const bool many = p.splits > 1, direct = halves && !many;                       // a row's result is in one place
   if (warp < 8) {
-    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, at = row0 + t * kTileRows + r;
     const int mine = halves ? count : (count + 1 - t) / 2;
+    const float inv = direct ? inverse_sum(s_sum[t * kTileRows + r]) : 0.0f;
+    uint16_t* const dst = static_cast<uint16_t*>(p.out) +
+                          ((static_cast<long long>(seq.first_row) + at / p.group) * p.heads + kvh * p.group + at % p.group) * 64;
     const uint32_t o_at = tmem + tile_o_col(t) + (static_cast<uint32_t>(quarter * 32) << 16);
     const bool none = s_max[t * kTileRows + r] == __int_as_float(0xff800000);
 #pragma unroll
@@ -529,12 +549,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       for (int n = 0; n < 32; n += 4) {
         uint4 u = make_uint4(o[n], o[n + 1], o[n + 2], o[n + 3]);
         if (mine <= 0 || gave_up || none) u = make_uint4(0, 0, 0, 0);
-        sts128(smem_u32(part) + (t * kTileRows + r) * 256 + (((h * 8 + (n >> 2)) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+        o[n] = u.x; o[n + 1] = u.y; o[n + 2] = u.z; o[n + 3] = u.w;
+        if (!direct) sts128(smem_u32(part) + (t * kTileRows + r) * 256 + (((h * 8 + (n >> 2)) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+      }
+      if (direct && at < row0 + rows) {
+#pragma unroll
+        for (int n = 0; n < 32; n += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x2 x = pack2(__uint_as_float(o[n + 2 * i]) * inv, __uint_as_float(o[n + 2 * i + 1]) * inv);
+            w[i] = p.q_bf16 ? pair_to_sixteen<__nv_bfloat16>(x) : pair_to_sixteen<__half>(x);
+          }
+          *reinterpret_cast<uint4*>(dst + 32 * h + n) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
   }
   tc_fence_before_sync();
-  const bool many = p.splits > 1;
   __syncthreads();
   tc_fence_after_sync();
   if (gave_up && (warp == 12 || warp == 13)) {                                    // products that nobody waited for end before their memory is given back
@@ -547,7 +579,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   // The rows are shared out over the blocks of the cluster: first what each part counts in a row and where the row goes, then four values a
   // thread.
-  {
+  if (!direct) {
     const int share = (rows + p.splits - 1) / p.splits, from = min(split * share, rows), mine = min(share, rows - from);
     const int parts = (halves ? 1 : 2) * p.splits;
     auto address = [&](int q, int r, uint32_t offset, int row_bytes) {

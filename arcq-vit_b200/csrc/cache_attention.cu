@@ -284,6 +284,17 @@ bool strides_ok(const int64_t* s, int n) {
   return true;
 }
 
+// Whether `out`, `bytes` long, lies over any of a tensor of 64 values a head with these sizes and strides (in values).
+bool overlaps(const void* out, int64_t bytes, const void* t, int n, const int64_t* sizes, const int64_t* strides) {
+  int64_t lo = 0, hi = 63;
+  for (int i = 0; i < n; ++i) {
+    if (sizes[i] == 0) return false;
+    (strides[i] < 0 ? lo : hi) += (sizes[i] - 1) * strides[i];
+  }
+  const char *const a = static_cast<const char*>(out), *const b = static_cast<const char*>(t);
+  return a < b + 2 * (hi + 1) && b + 2 * lo < a + bytes;
+}
+
 }  // namespace
 
 extern "C" {
@@ -291,7 +302,7 @@ extern "C" {
 int arcq_kv_cache_write(const arcq_kv_cache* cache, const float* thresholds, const void* k, const void* v, int x_dtype, int64_t tokens,
                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* slots, void* stream) {
   if (const int rc = check_cache(cache)) return rc;
-  if (tokens < 0 || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
+  if (tokens < 0 || tokens > 0x7fffffffLL || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
   if (tokens == 0 || cache->pages == 0) return ARCQ_OK;
   if (k == nullptr || v == nullptr || slots == nullptr || k_strides == nullptr || v_strides == nullptr || (cache->bits != 16 && thresholds == nullptr))
     return fail(ARCQ_E_BAD_ARG, "null pointer argument");
@@ -318,7 +329,7 @@ int arcq_kv_cache_write(const arcq_kv_cache* cache, const float* thresholds, con
 
 int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int out_dtype, void* stream) {
   if (const int rc = check_cache(cache)) return rc;
-  if (tokens < 0 || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
+  if (tokens < 0 || tokens > 0x7fffffffLL || tokens * cache->heads > 0x7fffffffLL) return fail(ARCQ_E_BAD_SHAPE, "bad number of tokens %lld", (long long)tokens);
   if (tokens == 0) return ARCQ_OK;
   if (k_out == nullptr || v_out == nullptr || slots == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (!aligned(k_out, 32) || !aligned(v_out, 32)) return fail(ARCQ_E_ALIGN, "outputs must be 32-byte aligned");
@@ -353,10 +364,12 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
   if (batch < 0 || table_width < 0 || max_new < 0 || q_rows < 0 || q_rows > 0x7fffffffLL || batch > 0x7fffffffLL || max_new > 0x7fffffffLL)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld table=%lld new=%lld rows=%lld", (long long)batch, (long long)table_width, (long long)max_new, (long long)q_rows);
   if (starts == nullptr && batch * max_new != q_rows) return fail(ARCQ_E_BAD_SHAPE, "%lld queries for %lld sequences of %lld", (long long)q_rows, (long long)batch, (long long)max_new);
-  if (table_width * cache->page_size > 0x7fffffffLL - 64) return fail(ARCQ_E_TOO_LARGE, "contexts of more than 2^31 tokens");
+  if (table_width > 0x7fffffffLL || table_width * cache->page_size > 0x7fffffffLL - 64) return fail(ARCQ_E_TOO_LARGE, "contexts of more than 2^31 tokens");
   if (batch == 0 || q_rows == 0 || max_new == 0) return ARCQ_OK;
   if (lengths == nullptr || (page_table == nullptr && table_width > 0) || q_strides == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (const int rc = check_query(q, q_dtype, out, heads, cache->heads, scale)) return rc;
+  const int64_t q_sizes[] = {q_rows, heads};
+  if (overlaps(out, q_rows * heads * 128, q, 2, q_sizes, q_strides)) return fail(ARCQ_E_BAD_ARG, "out lies over the queries");
   if (cache->bits == 16 && q_dtype != cache->dtype) return fail(ARCQ_E_BAD_ARG, "queries must have the type of the pages");
   if (!strides_ok(q_strides, 2)) return fail(ARCQ_E_ALIGN, "strides of the queries must be multiples of 8 values");
   arcq::AttendParams p = {};
@@ -397,12 +410,15 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
                          const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > 0x7fffffffLL - 64)
+  if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || queries > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > 0x7fffffffLL - 64)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld queries=%lld states=%lld", (long long)batch, (long long)queries, (long long)states);
   if (batch == 0 || queries == 0) return ARCQ_OK;
   if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || (states > 0 && (k == nullptr || v == nullptr)))
     return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (const int rc = check_query(q, dtype, out, heads, kv_heads, scale)) return rc;
+  const int64_t q_sizes[] = {batch, queries, heads}, kv_sizes[] = {batch, states, kv_heads}, bytes = batch * queries * heads * 128;
+  if (overlaps(out, bytes, q, 3, q_sizes, q_strides) || overlaps(out, bytes, k, 3, kv_sizes, k_strides) || overlaps(out, bytes, v, 3, kv_sizes, v_strides))
+    return fail(ARCQ_E_BAD_ARG, "out lies over the queries, keys or values");
   if (lengths != nullptr && mask != nullptr) return fail(ARCQ_E_BAD_ARG, "lengths or a mask, not both");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(ARCQ_E_ALIGN, "keys and values must be 16-byte aligned");
   if (!strides_ok(q_strides, 3) || !strides_ok(k_strides, 3) || !strides_ok(v_strides, 3)) return fail(ARCQ_E_ALIGN, "strides must be multiples of 8 values");

@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     tc_fence_before_sync();
   }
   // The block's set-up ends at this barrier, which each role reaches by itself: until then the loaders look up and fetch the first keys and the
-  // softmax warps their queries, while all but the loaders fill the tables (64 blocks' worth of 577 keys under 40 queries: XXX).
+  // softmax warps their queries, while all but the loaders fill the tables.  With rows of one block written from tensor memory: 2048 tokens over
+  // 16 384 in 4 bits 191 -> 187 us, 1024 queries over 2309 states 162 -> 159.
   auto fill_tables = [&](int i) {                                                 // i of 384 threads
     if constexpr (PACKED) {
       fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, i, kTileThreads - 128);

@@ -425,7 +425,7 @@ int arcq_kv_cache_write(const arcq_kv_cache* cache, const float* thresholds, con
                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* slots, void* stream);
 
 /* Reads tokens back: k_out, v_out [tokens, heads, 64] of out_dtype, each value rounded once; zeros where the slot is negative or beyond
- * the cache. */
+ * the cache.  k_out and v_out are 32-byte aligned. */
 int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, int out_dtype, void* stream);
 
 /*
@@ -437,10 +437,12 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
  *         not exist (negative, or not below cache.pages) are not seen.
  *   lengths int32 [batch]: tokens of the sequence in the cache, at most table_width * page_size
  *   causal 1: query i of n sees the first lengths[b] - n + i + 1 tokens; 0: all of them
- *   out   [q_rows, heads, 64] of q's type: softmax(scale q k^T) v, zeros for a query that sees nothing; rows of no sequence stay as they are.
+ *   out   [q_rows, heads, 64] of q's type, not over q: softmax(scale q k^T) v, zeros for a query that sees nothing; rows of no sequence stay as they are.
  * heads is a multiple of cache.heads: query head h reads key head h / (heads / cache.heads).  Packed keys and values are rebuilt in
  * fp16, one half-precision fma each, so |center| + 3 scale has to stay within fp16's range; products accumulate in fp32, probabilities are rounded
- * to 16 bits for the second one.  NaN and infinities in keys and values that are not seen have no effect.
+ * to 16 bits for the second one.  In calls with few queries a level is rounded to fp16 up or down instead, in turn over the keys, and center and
+ * scale come in fp32.  NaN and infinities in keys and values that none of a sequence's queries sees have no effect; in values that only its later
+ * queries see they may show in the earlier ones'.
  *   workspace  arcq_attention_workspace bytes of the call's own until it has run, 16-byte aligned (NULL where that is 0)
  */
 int64_t arcq_attention_workspace(int64_t batch, int64_t max_new, int64_t heads, int64_t kv_heads);
@@ -451,7 +453,7 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
 /*
  * Attention of queries [batch, queries, heads, 64] to an encoder's states, keys and values [batch, states, kv_heads, 64], all fp16 or all
  * bf16; strides of a sequence, a token and a head in values, multiples of 8.  lengths int32 [batch] (the first of the states are seen)
- * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64], a workspace for max_new = queries; otherwise as above.
+ * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64], not over q, k or v, a workspace for max_new = queries; otherwise as above.
  */
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,

@@ -31,12 +31,12 @@ def _read(lib, c, slots=1 << 20, tokens=3, k=1 << 20, v=1 << 20, dt=1):
 
 
 def _paged(lib, c, q=1 << 20, dt=1, rows=2, qs=(256, 64), heads=4, batch=2, table=1 << 20, width=3, lengths=1 << 20, starts=None, new=1, causal=1,
-           scale=0.125, out=1 << 20, work=1 << 20):
+           scale=0.125, out=1 << 21, work=1 << 20):
     return lib.arcq_paged_attention(ctypes.byref(c), q, dt, rows, _i64(*qs), heads, batch, table, width, lengths, starts, new, causal, scale, out, work, 1 << 20, None)
 
 
 def _cross(lib, q=1 << 20, k=1 << 20, v=1 << 20, dt=1, batch=2, queries=3, states=5, heads=4, kv=2, qs=(768, 256, 64), ks=(640, 128, 64),
-           vs=(640, 128, 64), lengths=None, mask=None, scale=0.125, out=1 << 20, work=1 << 20):
+           vs=(640, 128, 64), lengths=None, mask=None, scale=0.125, out=1 << 21, work=1 << 20):
     return lib.arcq_cross_attention(q, k, v, dt, batch, queries, states, heads, kv, _i64(*qs), _i64(*ks), _i64(*vs), lengths, mask, 5, scale, out, work, 1 << 20, None)
 
 
@@ -76,6 +76,26 @@ def test_attention_that_is_refused(lib, pkg):
     assert _cross(lib, v=(1 << 20) + 2) == ALIGN and _cross(lib, ks=(641, 128, 64)) == ALIGN
     assert _paged(lib, c, work=(1 << 20) + 8) == ALIGN and _cross(lib, work=(1 << 20) + 4) == ALIGN
     assert _cross(lib, batch=0) == 0 and _cross(lib, queries=0) == 0
+
+
+def test_sizes_whose_products_pass_64_bits(lib, pkg):
+    c = _cache(pkg, heads=4, page_size=16)
+    assert _write(lib, c, tokens=1 << 62) == BAD_SHAPE and _read(lib, c, tokens=1 << 62) == BAD_SHAPE
+    assert _paged(lib, c, width=1 << 60) == TOO_LARGE and _paged(lib, c, new=1 << 62) == BAD_SHAPE
+    assert _cross(lib, queries=1 << 62) == BAD_SHAPE and _cross(lib, batch=1 << 62) == BAD_SHAPE and _cross(lib, states=1 << 62) == BAD_SHAPE
+
+
+def test_outputs_over_inputs_are_refused(lib, pkg):
+    c, at = _cache(pkg), 1 << 20
+    q_end = at + 2 * (256 + 3 * 64 + 64)                                 # two rows of four heads
+    for out in (at, q_end - 16, at - 2 * 4 * 128 + 16):
+        assert _paged(lib, c, out=out) == BAD_ARG and b"over the queries" in lib.arcq_last_error_string()
+    for out in (at, at + 16):
+        for other in ("q", "k", "v"):
+            where = {n: 1 << 22 for n in "qkv"}
+            assert _cross(lib, **{**where, other: at}, out=out) == BAD_ARG and b"out lies over" in lib.arcq_last_error_string()
+    back = at + 2 * 256                                                  # rows one after the other downwards
+    assert _paged(lib, c, q=back, qs=(-256, 64), out=at) == BAD_ARG and b"over the queries" in lib.arcq_last_error_string()
 
 
 def test_operators_refuse_tensors_of_the_host(pkg):

@@ -548,3 +548,160 @@ def test_what_is_refused(pkg, cuda_device):
         paged(q=q.clone().requires_grad_())
     torch.cuda.synchronize()
     assert ops.device_status() == 0
+
+
+# ---------------------------------------------------------------- both kernels on either side of where one takes over from the other
+@pytest.mark.parametrize("bits,dtype", [(4, torch.float16), (3, torch.bfloat16), (2, torch.float16), (16, torch.float16), (16, torch.bfloat16)])
+@pytest.mark.parametrize("new,heads,kv_heads", [(8, 2, 2), (4, 6, 2), (9, 2, 2), (16, 2, 2), (17, 1, 1), (32, 2, 2), (11, 3, 1), (33, 1, 1), (128, 1, 1), (129, 1, 1)])
+def test_rows_of_a_key_head(pkg, cuda_device, bits, dtype, new, heads, kv_heads):
+    """Few sequences with narrow tables, and many keys in all (one long sequence): up to 32 rows the kernels share such calls out between them."""
+    _paged_check(pkg, cuda_device, bits, dtype, heads, kv_heads, 32, [300, 45], [new, min(new, 3)], seed=21)
+    _paged_check(pkg, cuda_device, bits, dtype, heads, kv_heads, 64, [500] + [90] * 9, [new] * 10, seed=22, causal=False)
+    far = 17000 if bits != 16 else 42000                               # keys times key heads: 136 000, 336 000
+    gen = torch.Generator().manual_seed(23)
+    B = 8 // kv_heads
+    c = _filled(pkg, gen, 20, kv_heads, 64, bits, dtype, cuda_device)
+    width = -(-far // 64)
+    table = torch.full((B, width), -1, dtype=torch.int32)              # pages that do not exist but for some, up to the last
+    places = torch.cat([torch.tensor([0, 1, width - 1]), 2 + torch.randperm(width - 3, generator=gen)[:13]]).sort().values
+    for b in range(B):
+        table[b, places] = torch.randperm(20, generator=gen)[:16].to(torch.int32)
+    lengths = torch.tensor([far - 7 * b for b in range(B)], dtype=torch.int32)
+    q = (1.3 * torch.randn(B * new, heads, 64, generator=gen)).to(dtype).to(cuda_device)
+    out = pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table.to(cuda_device), lengths.to(cuda_device), None, new,
+                                  **{n: c.get(n) for n in ("k_stats", "v_stats", "codebooks")})
+    for b in range(B):
+        j = (places[:, None] * 64 + torch.arange(64)).reshape(-1)
+        j = j[j < lengths[b]]
+        rows = torch.stack([table[b, j // 64].long(), j % 64], 1).to(cuda_device)
+        (k, dk), (v, dv) = (_cached(pkg, c, w, rows) for w in "kv")
+        seen = (j[None, :] <= (lengths[b] - new + torch.arange(new))[:, None]).to(cuda_device)
+        want, off = _attend(q[b * new:(b + 1) * new], k, dk, v, dv, seen, 0.125, dtype, bits != 16)
+        err = (out[b * new:(b + 1) * new].double() - want).abs()
+        assert bool((err <= off).all()), (b, float((err / off).max()))
+    assert pkg.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("bits,dtype", [(4, torch.bfloat16), (3, torch.float16), (2, torch.float16), (16, torch.float16)])
+def test_units_that_are_cut_and_that_are_not(pkg, cuda_device, bits, dtype):
+    """Contexts on both sides of where units are cut between blocks, with sequences of a token and of none between long ones."""
+    for longest in (1150, 1153, 2600):
+        _paged_check(pkg, cuda_device, bits, dtype, 4, 2, 16, [longest, 1, 0, 31, longest - 40, 33, 1], [1, 1, 1, 1, 2, 0, 1], seed=24)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_more_sequences_than_threads(pkg, cuda_device, bits):
+    lengths = [(7 * i) % 50 for i in range(900)]
+    _paged_check(pkg, cuda_device, bits, torch.float16, 1, 1, 16, lengths, [i % 2 if i % 40 < 30 else 0 for i in range(900)], seed=25)
+    _cross_check(pkg, cuda_device, torch.float16, 900, 1, 40, 1, 1, "lengths", seed=26)
+
+
+def test_empty_caches_tables_and_batches(pkg, cuda_device):
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    for bits in (4, 16):
+        c, th = _empty_cache(0, 2, 16, bits, torch.float16, cuda_device)
+        args = {n: c.get(n) for n in ("k_stats", "v_stats", "codebooks")}
+        x = torch.randn(3, 2, 64, device=cuda_device).half()
+        slots = torch.arange(3, device=cuda_device)
+        pkg.ops.kv_cache_write(x, x, slots, thresholds=th, **c)
+        assert not any(bool(t.any()) for t in pkg.ops.kv_cache_read(slots, **c))
+        for new in (1, 40):
+            q = torch.randn(2 * new, 4, 64, device=cuda_device).half()
+            for table in (torch.zeros(2, 3, **i32), torch.zeros(2, 0, **i32)):
+                got = pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, torch.tensor([30, 5], **i32), None, new, **args)
+                assert not bool(got.any())
+            assert pkg.ops.paged_attention(q[:0], c["k_pages"], c["v_pages"], torch.zeros(0, 3, **i32), torch.zeros(0, **i32), None, new, **args).shape == (0, 4, 64)
+    assert pkg.ops.device_status() == 0
+
+
+def test_the_same_slot_twice(pkg, cuda_device):
+    """One of the tokens, or parts of both: statistics and codes of either, and no other slot."""
+    c, th = _empty_cache(2, 1, 16, 4, torch.float16, cuda_device)
+    x = torch.randn(4000, 1, 64, generator=torch.Generator().manual_seed(5)).half().to(cuda_device)
+    pkg.ops.kv_cache_write(x, x, torch.full((4000,), 17, device=cuda_device), thresholds=th, **c)
+    got = pkg.ops.kv_cache_read(torch.arange(32, device=cuda_device), **c)
+    assert bool(torch.isfinite(got[0]).all()) and int(got[0].any(-1).sum()) == 1 and int(got[1].any(-1).sum()) == 1
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_two_captured_graphs_at_once(pkg, cuda_device, bits):
+    """Each graph keeps workspaces of its own: replayed side by side, with new lengths, both give what an eager call gives."""
+    gen = torch.Generator().manual_seed(31)
+    c = _filled(pkg, gen, 64, 2, 64, bits, torch.float16, cuda_device)
+    args = {n: c.get(n) for n in ("k_stats", "v_stats", "codebooks")}
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    table = torch.randperm(64, generator=gen).to(torch.int32).to(cuda_device).reshape(2, 32)
+    calls = []
+    for new in (1, 2):
+        q = torch.randn(2 * new, 8, 64, generator=gen).half().to(cuda_device)
+        lengths = torch.tensor([2000, 1500], **i32)
+        run = lambda q=q, lengths=lengths, new=new: pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, lengths, None, new, **args)   # noqa: E731
+        run()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run()
+        calls.append((g, run, got, lengths, torch.cuda.Stream()))
+    for values in ([2000, 1500], [2048, 3], [700, 0], [1, 2047]):
+        want = []
+        for g, run, got, lengths, s in calls:
+            lengths.copy_(torch.tensor(values, dtype=torch.int32))
+            want.append(run())
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, run, got, lengths, s in calls:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(call[2], w) for call, w in zip(calls, want))
+    assert pkg.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("polls", [0, 1, 3])
+@pytest.mark.parametrize("bits,B,n,S", [(16, 1, 40, 900), (16, 2, 300, 400), (4, 1, 40, 900), (4, 90, 200, 300)])
+def test_waits_of_the_tile_kernel_that_run_out(pkg, cuda_device, bits, B, n, S, polls):
+    """The kernel ends, a result that is not the whole one has left its code in the status word, and the next launch is none the worse."""
+    gen = torch.Generator().manual_seed(32)
+    c = _filled(pkg, gen, 2 * B + 8, 1, 512, bits, torch.float16, cuda_device)
+    args = {m: c.get(m) for m in ("k_stats", "v_stats", "codebooks")}
+    table = torch.arange(2 * B, dtype=torch.int32, device=cuda_device).reshape(B, 2)
+    q = torch.randn(B * n, 1, 64, generator=gen).half().to(cuda_device)
+    run = lambda: pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, torch.full((B,), S, dtype=torch.int32, device=cuda_device), None, n, **args)   # noqa: E731
+    want = run()
+    for _ in range(3):
+        with pkg._cabi.option("ARCQ_POLL_LIMIT", polls):
+            got = run()
+        status = pkg.ops.device_status()
+        assert status == 0x502 or (polls > 0 and status == 0 and torch.equal(got, want))
+    assert torch.equal(run(), want) and pkg.ops.device_status() == 0
+
+
+def test_registers_and_workspaces_that_are_too_few(pkg, cuda_device):
+    import ctypes
+    import threading
+    q = torch.randn(1, 200, 2, 64, device=cuda_device).half()
+    k = torch.randn(1, 300, 2, 64, device=cuda_device).half()
+    results = []
+
+    def run():                                                         # the kernel is asked once a thread
+        try:
+            results.append(pkg.ops.cross_attention(q, k, k))
+        except RuntimeError as e:
+            results.append(str(e))
+    for regs in (120, 128, 0):
+        with pkg._cabi.option("ARCQ_LAUNCH_REGS", regs):
+            t = threading.Thread(target=run)
+            t.start()
+            t.join()
+        assert torch.is_tensor(results[-1]) if regs != 120 else "compiled for 120 registers" in results[-1]
+    lib = pkg._cabi.load()
+    need = lib.arcq_attention_workspace(1, 1, 2, 2)
+    work, out = torch.empty(need, dtype=torch.uint8, device=cuda_device), torch.full((1, 1, 2, 64), 3.0, device=cuda_device).half()
+    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, k)]
+    call = lambda bytes_, at: lib.arcq_cross_attention(q.data_ptr(), k.data_ptr(), k.data_ptr(), 1, 1, 1, 300, 2, 2, *strides, None, None, 0, 0.125,   # noqa: E731
+                                                       out.data_ptr(), at, bytes_, None)
+    assert call(need - 1, work.data_ptr()) == -1 and call(need, None) == -1 and bool((out == 3.0).all())
+    assert call(need, work.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert not bool((out == 3.0).all()) and pkg.ops.device_status() == 0
+    with pytest.raises(RuntimeError, match="out lies over"):
+        pkg.ops.cross_attention(q, k, k, out=q)

@@ -194,14 +194,14 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
 }
 
 // How many clusters of a size run at a time; 0: none, or it cannot be said
-template <typename Kernel> int clusters_at_a_time(Kernel k, int size, size_t smem) {
+template <typename Kernel> int clusters_at_a_time(Kernel k, int size, int threads, size_t smem) {
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = size;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  lc.gridDim = dim3(size * arcq_host::sm_count());
-  lc.blockDim = dim3(arcq::kTileThreads);
+  lc.gridDim = dim3(size * arcq_host::sm_count() * 2);
+  lc.blockDim = dim3(threads);
   lc.dynamicSmemBytes = smem;
   lc.attrs = &attr;
   lc.numAttrs = 1;
@@ -214,9 +214,10 @@ constexpr double kTileSetUp = 7.0;         // of a block, in tiles of keys: 13 u
 
 // Blocks of a row tile, 1 to 8: the cluster size for which the rounds of blocks over the SMs take the fewest tiles of keys, a block's set-up and
 // the joining of results counted as tiles.
-template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStream_t st) {
-  auto k = arcq::tile_attention_kernel<BITS, E>;
-  constexpr size_t smem = arcq::tile_smem_layout(BITS != 16).total;
+template <int BITS, typename E, int STREAMS> int launch_tile(arcq::AttendParams& p, cudaStream_t st) {
+  auto k = arcq::tile_attention_kernel<BITS, E, STREAMS>;
+  constexpr size_t smem = arcq::tile_smem_layout(BITS != 16, STREAMS).total;
+  constexpr int threads = arcq::tile_threads(STREAMS), block_rows = STREAMS * arcq::kTileRows;
   static thread_local int done_dev = -1, room[9];                               // clusters of a size that run at a time
   int dev = 0;
   cudaGetDevice(&dev);
@@ -226,16 +227,16 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, k);
     if (e != cudaSuccess) return arcq_host::cuda_fail(e, "attention set-up");
     const int got = arcq_host::launch_regs() > 0 ? arcq_host::launch_regs() : a.numRegs;
-    if (got < arcq::kTileLaunchRegs)             // the warp groups' hand-over would wait for good
+    if (STREAMS > 1 && got < arcq::kTileLaunchRegs)             // the warp groups' hand-over would wait for good
       return fail(ARCQ_E_CUDA, "attention: compiled for %d registers a thread, its warp groups share out %d", got, arcq::kTileLaunchRegs);
-    room[1] = arcq_host::sm_count();
-    for (int s = 2; s <= 8; ++s) room[s] = clusters_at_a_time(k, s, smem);
+    room[1] = arcq_host::sm_count() * (3 - STREAMS);
+    for (int s = 2; s <= 8; ++s) room[s] = clusters_at_a_time(k, s, threads, smem);
     done_dev = dev;
   }
   const long long all_rows = static_cast<long long>(p.max_new) * p.group;
-  p.tiles = static_cast<int>((all_rows + 2 * arcq::kTileRows - 1) / (2 * arcq::kTileRows));
+  p.tiles = static_cast<int>((all_rows + block_rows - 1) / block_rows);
   const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.tiles;
-  const double key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys, each = all_rows > arcq::kTileRows ? 1.0 : 0.5;
+  const double key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys, each = STREAMS == 1 || all_rows > arcq::kTileRows ? 1.0 : 0.5;
   int splits = 1;
   double best = 1e30;
   for (int s = 1; s <= 8 && (s == 1 || s <= key_tiles); ++s) {
@@ -250,12 +251,24 @@ template <int BITS, typename E> int launch_tile(arcq::AttendParams& p, cudaStrea
   p.poll_limit = arcq_host::poll_limit();
   p.status = arcq_host::status_ptr();
   if (units * splits > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
-  const cudaError_t e = launch(k, dim3(static_cast<unsigned>(units * splits)), arcq::kTileThreads, smem, splits, st, p);
+  const cudaError_t e = launch(k, dim3(static_cast<unsigned>(units * splits)), threads, smem, splits, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 
+// Up to 128 rows: blocks of one stream, two on an SM, where there is a second for it and the keys are few, so that one block's set-up, loads and
+// join run beside the other's products; or where there is one tile of keys.  384 key heads, 40 rows: 128 keys 13.4 us against two streams'
+// 21.4, 384 keys 24.2 against 29.6, 700 keys 39.3 against 40.5, 900 keys 48.9 against 47.4; 140 key heads, 48 rows: 128 keys 7.0 against 7.9,
+// 250 keys 9.2 against 9.1, 500 keys 13.1 against 11.2.
+bool one_stream_is_ahead(const arcq::AttendParams& p) {
+  const int key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys;
+  return key_tiles <= 1 || (key_tiles <= 6 && static_cast<long long>(p.batch) * p.kv_heads > arcq_host::sm_count());
+}
+
 template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
-  return split_is_ahead<BITS>(p) ? launch_split<BITS, E>(p, workspace_bytes, st) : launch_tile<BITS, E>(p, st);
+  if (split_is_ahead<BITS>(p)) return launch_split<BITS, E>(p, workspace_bytes, st);
+  if constexpr (BITS == 16)
+    if (static_cast<long long>(p.max_new) * p.group <= arcq::kTileRows && one_stream_is_ahead(p)) return launch_tile<BITS, E, 1>(p, st);
+  return launch_tile<BITS, E, 2>(p, st);
 }
 
 int run_attention(arcq::AttendParams& p, int bits, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {

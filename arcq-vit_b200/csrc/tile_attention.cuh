@@ -25,29 +25,30 @@
 namespace arcq {
 
 constexpr int kStatusTileAttentionTimeout = 0x502;
-constexpr int kTileThreads = 512, kTileRows = 128, kTileKeys = 128;
-// tiles of keys, and of values, in shared memory: 16 bits have no tables there
-__host__ __device__ constexpr int tile_slots(bool packed) { return packed ? 3 : 5; }
+constexpr int kTileRows = 128, kTileKeys = 128;
+__host__ __device__ constexpr int tile_threads(int streams) { return 256 * streams; }
+// tiles of keys, and of values, in shared memory: 16 bits have no tables there, and one stream's blocks share an SM
+__host__ __device__ constexpr int tile_slots(bool packed, int streams) { return streams == 1 ? 2 : packed ? 3 : 5; }
 constexpr int kTileSeen = 8;
+// two streams' warps share out their registers
 constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 184, kTileLoadRegs = 88, kTileIssueRegs = 56;
 static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
 constexpr uint32_t kTileBytes = 128 * 128;                        // 128 rows of 64 16-bit values
 constexpr int kTileWeights = 2 * (kTileRows + 8);                  // rows of a block times parts: rounded up for 8 blocks and two streams
-constexpr uint32_t kTileTmemCols = 512;
-// tensor memory of stream t: scores, probabilities (pairs), output
-__host__ __device__ constexpr uint32_t tile_s_col(int t) { return 128u * t; }
-__host__ __device__ constexpr uint32_t tile_p_col(int t) { return 256u + 64u * t; }
-__host__ __device__ constexpr uint32_t tile_o_col(int t) { return 384u + 64u * t; }
+// tensor memory, 256 columns a stream: scores, probabilities (pairs), output
+__host__ __device__ constexpr uint32_t tile_s_col(int t) { return 256u * t; }
+__host__ __device__ constexpr uint32_t tile_p_col(int t) { return 256u * t + 128u; }
+__host__ __device__ constexpr uint32_t tile_o_col(int t) { return 256u * t + 192u; }
 
 struct TileSmem {
   uint32_t q, k, v, tables, seen, max, sum, weight, offset, bars, total;
 };
-__host__ __device__ constexpr TileSmem tile_smem_layout(bool packed) {
+__host__ __device__ constexpr TileSmem tile_smem_layout(bool packed, int streams) {
   TileSmem s = {};
   s.q = 0;
-  s.k = s.q + 2 * kTileBytes;
-  s.v = s.k + tile_slots(packed) * kTileBytes;
-  s.tables = s.v + tile_slots(packed) * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
+  s.k = s.q + streams * kTileBytes;
+  s.v = s.k + tile_slots(packed, streams) * kTileBytes;
+  s.tables = s.v + tile_slots(packed, streams) * kTileBytes;                       // [byte][lane] pairs of levels, keys then values
   s.seen = s.tables + (packed ? 2 * kPairTableBytes : 0);
   s.max = s.seen + kTileSeen * 16;
   s.sum = s.max + 2 * kTileRows * 4;
@@ -72,13 +73,15 @@ __device__ __forceinline__ float4 lds128_cluster(uint32_t addr) {
   return v;
 }
 
-template <int BITS, typename E>
-__global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const __grid_constant__ AttendParams p) {
+template <int BITS, typename E, int STREAMS>
+__global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_attention_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int kThreads = tile_threads(STREAMS), kBlockRows = STREAMS * kTileRows;
+  constexpr int kLoad = 4 * STREAMS, kIssue = STREAMS == 1 ? 0 : kLoad + 4;      // first warps
   constexpr bool PACKED = BITS != 16;
-  constexpr int SLOTS = tile_slots(PACKED);
+  constexpr int SLOTS = tile_slots(PACKED, STREAMS);
   extern __shared__ uint8_t tile_smem_raw[];
   uint8_t* const smem = tile_smem_raw + ((1024u - (smem_u32(tile_smem_raw) & 1023u)) & 1023u);
-  constexpr TileSmem L = tile_smem_layout(PACKED);
+  constexpr TileSmem L = tile_smem_layout(PACKED, STREAMS);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L.bars);
   uint64_t *const k_full = bars, *const k_free = bars + 5, *const v_full = bars + 10, *const v_free = bars + 15;     // [slot]
   uint64_t *const q_full = bars + 20, *const s_full = bars + 22, *const s_read = bars + 24, *const p_full = bars + 26, *const o_done = bars + 28;   // [stream]
@@ -99,39 +102,39 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   pdl_wait();
   const AttendSequence seq = attend_sequence(p, b);
   const int all_rows = seq.queries * p.group;
-  const bool halves = all_rows > kTileRows;                                       // the streams are halves of the rows
-  const int row0 = tile * 2 * kTileRows, rows = min(all_rows - row0, 2 * kTileRows);
+  const bool halves = STREAMS == 1 || all_rows > kTileRows;                       // the streams are halves of the rows; or there is one
+  const int row0 = tile * kBlockRows, rows = min(all_rows - row0, kBlockRows);
   // Tiles of rows that are not there: the whole cluster leaves.
   if (rows <= 0) {
     pdl_launch_dependents();
     return;
   }
-  if (tid == 13 * 32) {
-    const int users = halves ? 2 : 1;                                             // streams that read a tile of keys
+  if (tid == (kIssue + 1) * 32) {
+    const int users = halves ? STREAMS : 1;                                             // streams that read a tile of keys
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
       mbar_init(k_free + i, users); mbar_init(v_free + i, users);
     }
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < STREAMS; ++t) {
       mbar_init(s_read + t, 4); mbar_init(p_full + t, 4);
       mbar_init(s_full + t, 1); mbar_init(o_done + t, 1);
       mbar_init(q_full + t, halves ? 4 : 8);
     }
-    mbar_init(stopped, 2);
+    mbar_init(stopped, STREAMS);
     mbar_fence_init();
   }
-  if (warp == 12) {
-    tmem_alloc(s_tmem, kTileTmemCols);
+  if (warp == kIssue) {
+    tmem_alloc(s_tmem, 256 * STREAMS);
     tmem_relinquish();
     tc_fence_before_sync();
   }
   // The block's set-up ends at this barrier, which each role reaches by itself: until then the loaders look up and fetch the first keys and the
   // softmax warps their queries, while all but the loaders fill the tables.  With rows of one block written from tensor memory: 2048 tokens over
   // 16 384 in 4 bits 191 -> 187 us, 1024 queries over 2309 states 162 -> 159.
-  auto fill_tables = [&](int i) {                                                 // i of 384 threads
+  auto fill_tables = [&](int i) {                                                 // i of all but 128 threads
     if constexpr (PACKED) {
-      fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, i, kTileThreads - 128);
-      fill_pair_table_f32(smem_u32(smem) + L.tables + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, i, kTileThreads - 128);
+      fill_pair_table(smem_u32(smem) + L.tables, p.codebooks, 1 << BITS, i, kThreads - 128);
+      fill_pair_table_f32(smem_u32(smem) + L.tables + kPairTableBytes, p.codebooks + (1 << BITS), 1 << BITS, i, kThreads - 128);
     }
   };
   auto set_up = [&] {
@@ -147,18 +150,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   // tile j of the block is tile i of stream t: halves: j = i for both; else j = 2 i + t
   bool ok = true;
 
-  if (warp >= 12) {
-    // ------------------------------------------------------------------ products: warps 12 and 13, a stream each
+  // A tile's products, for a whole warp; q, k and v: descriptors of the queries and of the slot
+  const uint32_t idesc_s = tile_idesc<E>(kTileRows, kTileKeys);
+  const uint32_t idesc_o = tile_idesc<E>(kTileRows, 64) | (1u << 16);             // B with its rows (keys) along K
+  auto desc_lo = [&](uint32_t off) { return ((smem_u32(smem + off) & 0x3FFFFu) >> 4) | (1u << 16); };
+  auto issue_scores = [&](uint32_t tmem, int t, uint32_t q, uint32_t k, int slot) {
+    tc_fence_after_sync();
+    if (elect_one() && ok) {
+      umma_f16_x4(tmem + tile_s_col(t), q, k + slot * (kTileBytes >> 4), idesc_s);
+      umma_commit(s_full + t);
+      umma_commit(k_free + slot);
+    }
+    __syncwarp();
+  };
+  auto issue_output = [&](uint32_t tmem, int t, uint32_t v, int slot, bool fresh) {
+    tc_fence_after_sync();
+    if (elect_one() && ok) {
+#pragma unroll
+      for (int k = 0; k < kTileKeys; k += 16)
+        umma_f16_tmem_a_lo(tmem + tile_o_col(t), tmem + tile_p_col(t) + (k >> 1), v + slot * (kTileBytes >> 4) + 8 * k, idesc_o, !fresh || k > 0 ? 1u : 0u);
+      umma_commit(o_done + t);
+      umma_commit(v_free + slot);
+    }
+    __syncwarp();
+  };
+
+  if (STREAMS > 1 && warp >= kIssue) {
+    // ------------------------------------------------------------------ products: a warp a stream
     fewer_registers<kTileIssueRegs>();
     fill_tables(tid - 128);
     set_up();
     const uint32_t tmem = *s_tmem;
-    const int t = warp - 12;
-    const int mine = t > 1 ? 0 : halves ? count : (count + 1 - t) / 2;
-    if (t < 2 && mine > 0) {
-      const uint32_t idesc_s = tile_idesc<E>(kTileRows, kTileKeys);
-      const uint32_t idesc_o = tile_idesc<E>(kTileRows, 64) | (1u << 16);         // B with its rows (keys) along K
-      auto desc_lo = [&](uint32_t off) { return ((smem_u32(smem + off) & 0x3FFFFu) >> 4) | (1u << 16); };
+    const int t = warp - kIssue;
+    const int mine = t >= STREAMS ? 0 : halves ? count : (count + 1 - t) / 2;
+    if (t < STREAMS && mine > 0) {
       const uint32_t q = desc_lo(L.q + (halves ? t : 0) * kTileBytes), k0 = desc_lo(L.k), v0 = desc_lo(L.v);
       auto at = [&](int i) { return halves ? i : 2 * i + t; };
       for (int i = 0; i <= mine; ++i) {
@@ -166,35 +191,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
           const int j = at(i), slot = j % SLOTS;
           ok = ok && (i > 0 || mbar_wait(q_full + (halves ? t : 0), 0, polls)) && mbar_wait(k_full + slot, (j / SLOTS) & 1, polls) &&
                (i == 0 || mbar_wait(s_read + t, (i - 1) & 1, polls));
-          tc_fence_after_sync();
-          if (elect_one() && ok) {
-            umma_f16_x4(tmem + tile_s_col(t), q, k0 + slot * (kTileBytes >> 4), idesc_s);
-            umma_commit(s_full + t);
-            umma_commit(k_free + slot);
-          }
-          __syncwarp();
+          issue_scores(tmem, t, q, k0, slot);
         }
         if (i > 0) {
           const int j = at(i - 1), slot = j % SLOTS;
           ok = ok && mbar_wait(v_full + slot, (j / SLOTS) & 1, polls) && mbar_wait(p_full + t, (i - 1) & 1, polls);
-          tc_fence_after_sync();
-          if (elect_one() && ok) {
-#pragma unroll
-            for (int k = 0; k < kTileKeys; k += 16)
-              umma_f16_tmem_a_lo(tmem + tile_o_col(t), tmem + tile_p_col(t) + (k >> 1), v0 + slot * (kTileBytes >> 4) + 8 * k, idesc_o,
-                                 i > 1 || k > 0 ? 1u : 0u);
-            umma_commit(o_done + t);
-            umma_commit(v_free + slot);
-          }
-          __syncwarp();
+          issue_output(tmem, t, v0, slot, i == 1);
         }
       }
     }
     __syncwarp();
-  } else if (warp >= 8) {
+  } else if (warp >= kLoad) {
     // ------------------------------------------------------------------ keys and values: a warp 32 keys of a tile
-    fewer_registers<kTileLoadRegs>();
-    const int w = warp - 8;
+    if constexpr (STREAMS > 1) fewer_registers<kTileLoadRegs>();
+    const int w = warp - kLoad;
     const uint32_t k_smem = smem_u32(smem) + L.k + w * 4096, v_smem = smem_u32(smem) + L.v + w * 4096;
     // where the two sixteens of keys of the warp lie, each in one page; looked up two tiles ahead, as are the masks
     int page[2] = {0, 0}, page_after[2] = {0, 0};
@@ -371,7 +381,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     }
   } else {
     // ------------------------------------------------------------------ softmax: a thread a row
-    more_registers<kTileSoftmaxRegs>();
+    if constexpr (STREAMS > 1) more_registers<kTileSoftmaxRegs>();
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const int at = row0 + (halves ? t * kTileRows : 0) + r;                       // of the sequence's rows
     const bool live = at < row0 + rows;
@@ -407,15 +417,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full + (halves ? t : 0));
+      if (STREAMS > 1 && lane == 0) mbar_arrive(q_full + (halves ? t : 0));
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory");
     const float scale = s_max[halves ? t * kTileRows + r : r];
-    asm volatile("bar.sync 1, 256;" ::: "memory");                                // all have read theirs: s_max is free again
+    const uint32_t tmem = *s_tmem;
+    // One stream issues its products itself, behind barriers of its warps.
+    auto own_scores = [&](int j) {
+      if (warp != 0) return;
+      ok = ok && mbar_wait_warp(k_full + j % SLOTS, (j / SLOTS) & 1, polls);
+      issue_scores(tmem, 0, desc_lo(L.q), desc_lo(L.k), j % SLOTS);
+    };
+    auto own_output = [&](int j) {
+      if (warp != 0) return;
+      ok = ok && mbar_wait_warp(v_full + j % SLOTS, (j / SLOTS) & 1, polls);
+      issue_output(tmem, 0, desc_lo(L.v), j % SLOTS, j == 0);
+    };
+    auto all_rows_here = [] { asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory"); };
+    if (STREAMS == 1 && count > 0) own_scores(0);
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory");           // all have read theirs: s_max is free again
     const int mine = halves ? count : (count + 1 - t) / 2;
     const float ninf = __int_as_float(0xff800000);
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tmem = *s_tmem, s_at = tmem + tile_s_col(t) + lanes, p_at = tmem + tile_p_col(t) + lanes, o_at = tmem + tile_o_col(t) + lanes;
+    const uint32_t s_at = tmem + tile_s_col(t) + lanes, p_at = tmem + tile_p_col(t) + lanes, o_at = tmem + tile_o_col(t) + lanes;
     const bool rows_here = __any_sync(0xffffffffu, live);
     float top = ninf;                                                             // in units of the exponent
     f32x2 sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
@@ -423,8 +447,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
     // products, reads its scores and finds the maximum.  Left alone they fall into step, and the pipe idles during all of that: 3720 cycles
     // a tile of keys (both streams), in turns 3170, of which the exponentials of a stream take 1500.
     // A stream has as many turns as tiles; the second has as many as the first or one fewer.
-    auto my_turn = [&] { asm volatile("bar.sync %0, 256;" ::"r"(2 + t) : "memory"); };
-    auto your_turn = [&] { asm volatile("bar.arrive %0, 256;" ::"r"(3 - t) : "memory"); };
+    auto my_turn = [&] { if constexpr (STREAMS > 1) asm volatile("bar.sync %0, 256;" ::"r"(2 + t) : "memory"); };
+    auto your_turn = [&] { if constexpr (STREAMS > 1) asm volatile("bar.arrive %0, 256;" ::"r"(3 - t) : "memory"); };
     if (t == 1) your_turn();
     for (int i = 0; i < mine; ++i) {
       const int j = halves ? i : 2 * i + t;
@@ -432,34 +456,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       tc_fence_after_sync();
       if (rows_here && ok) {
         const uint4 seen = lds128(smem_u32(s_seen + j % kTileSeen * 4));
-        uint32_t s[4][32];
+        // one stream's threads hold half of a row's scores at a time, and read the first half twice
+        constexpr int PART = STREAMS == 1 ? 2 : 4, PARTS = 4 / PART;
+        uint32_t s[PART][32];
+        auto read_scores = [&](int part, bool last) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
-        tmem_ld_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_read + t);
-        // ---- what is not seen
-        __syncwarp();
+          for (int c = 0; c < PART; ++c) tmem_ld_32x32(s_at + 32 * (part * PART + c), s[c]);
+          tmem_ld_wait();
+          if (last) {
+            tc_fence_before_sync();
+            if constexpr (STREAMS == 1) {
+              all_rows_here();
+              if (i + 1 < mine) own_scores(j + 1);
+            } else {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(s_read + t);
+            }
+          }
+        };
         const int base = (first + j) * kTileKeys;
-        if (!__all_sync(0xffffffffu, (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && base + kTileKeys <= limit)) {
+        bool all_seen = false;
+        auto hide_unseen = [&](int part) {
+          if (all_seen) return;
           const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int left = limit - base - 32 * c;                               // keys of the 32 that the row may see
-            const uint32_t word = words[c] & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+          for (int c = 0; c < PART; ++c) {
+            const uint32_t of = PART == 4 ? words[c] : s_seen[j % kTileSeen * 4 + part * PART + c];
+            const int left = limit - base - 32 * (part * PART + c);               // keys of the 32 that the row may see
+            const uint32_t word = of & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
 #pragma unroll
             for (int n = 0; n < 32; ++n) s[c][n] = (word >> n) & 1 ? s[c][n] : 0xff800000u;
           }
-        }
+        };
         // ---- maximum
         float m0 = ninf, m1 = ninf, m2 = ninf, m3 = ninf;
+#pragma unroll 1
+        for (int part = 0; part < PARTS; ++part) {
+          read_scores(part, PARTS == 1);
+          if (part == 0) {
+            __syncwarp();
+            all_seen = __all_sync(0xffffffffu, (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && base + kTileKeys <= limit);
+          }
+          hide_unseen(part);
 #pragma unroll
-        for (int n = 0; n < 32; n += 2) {
-          m0 = max3(m0, __uint_as_float(s[0][n]), __uint_as_float(s[0][n + 1]));
-          m1 = max3(m1, __uint_as_float(s[1][n]), __uint_as_float(s[1][n + 1]));
-          m2 = max3(m2, __uint_as_float(s[2][n]), __uint_as_float(s[2][n + 1]));
-          m3 = max3(m3, __uint_as_float(s[3][n]), __uint_as_float(s[3][n + 1]));
+          for (int n = 0; n < 32; n += 2) {
+            float& m = PART == 1 && (n & 2) ? m1 : m0;
+            m = max3(m, __uint_as_float(s[0][n]), __uint_as_float(s[0][n + 1]));
+            if constexpr (PART > 1) m1 = max3(m1, __uint_as_float(s[1][n]), __uint_as_float(s[1][n + 1]));
+            if constexpr (PART == 4) {
+              m2 = max3(m2, __uint_as_float(s[2][n]), __uint_as_float(s[2][n + 1]));
+              m3 = max3(m3, __uint_as_float(s[3][n]), __uint_as_float(s[3][n + 1]));
+            }
+          }
         }
         const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * scale;
         // the probabilities' columns are free, and the output may be scaled, once the last product has ended
@@ -488,31 +536,48 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
         my_turn();
         const float nm = top == ninf ? 0.0f : -top;
         const f32x2 scale2 = pack2(scale, scale), nm2 = pack2(nm, nm);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            float x, y;
-            unpack2(fma2(pack2(__uint_as_float(s[c][2 * n]), __uint_as_float(s[c][2 * n + 1])), scale2, nm2), x, y);
-            const f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
-            if (n & 1) sum1 = add2(sum1, e); else sum0 = add2(sum0, e);
-            w[n] = pair_to_sixteen<E>(e);
+#pragma unroll 1
+        for (int part = PARTS - 1; part >= 0; --part) {
+          if (part < PARTS - 1) {
+            read_scores(part, part == 0);
+            hide_unseen(part);
           }
-          tmem_st_32x16(p_at + 16 * c, w);
+#pragma unroll
+          for (int c = 0; c < PART; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+              float x, y;
+              unpack2(fma2(pack2(__uint_as_float(s[c][2 * n]), __uint_as_float(s[c][2 * n + 1])), scale2, nm2), x, y);
+              const f32x2 e = pack2(exp2_approx(x), exp2_approx(y));
+              if (n & 1) sum1 = add2(sum1, e); else sum0 = add2(sum0, e);
+              w[n] = pair_to_sixteen<E>(e);
+            }
+            tmem_st_32x16(p_at + 16 * (part * PART + c), w);
+          }
         }
         your_turn();
         tmem_st_wait();
       } else {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_read + t);
+        if constexpr (STREAMS == 1) {
+          all_rows_here();
+          if (i + 1 < mine) own_scores(j + 1);
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_read + t);
+        }
         if (i > 0 && ok) ok = mbar_wait_warp(o_done + t, (i - 1) & 1, polls);
         my_turn();
         your_turn();
       }
       tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + t);
+      if constexpr (STREAMS == 1) {
+        all_rows_here();
+        own_output(j);
+      } else {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + t);
+      }
     }
     // ---- the stream's part: maximum, sum and output, as they are
     if (mine > 0) ok = ok && mbar_wait_warp(o_done + t, (mine - 1) & 1, polls);
@@ -528,10 +593,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   const bool gave_up = __syncthreads_or(!ok) != 0;
   tc_fence_after_sync();
   const uint32_t tmem = *s_tmem;
-  if (gave_up && tid == 12 * 32) atomicExch(p.status, kStatusTileAttentionTimeout);
+  if (gave_up && tid == kIssue * 32) atomicExch(p.status, kStatusTileAttentionTimeout);
   float* const part = reinterpret_cast<float*>(smem + L.k);                       // [stream][row][64], over the slots, 16-byte chunks swizzled by row
   const bool many = p.splits > 1, direct = halves && !many;                       // a row's result is in one place
-  if (warp < 8) {
+  if (warp < kLoad) {
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, at = row0 + t * kTileRows + r;
     const int mine = halves ? count : (count + 1 - t) / 2;
     const float inv = direct ? inverse_sum(s_sum[t * kTileRows + r]) : 0.0f;
@@ -570,13 +635,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (gave_up && (warp == 12 || warp == 13)) {                                    // products that nobody waited for end before their memory is given back
+  if (gave_up && warp >= kIssue && warp < kIssue + STREAMS) {                                    // products that nobody waited for end before their memory is given back
     if (elect_one()) umma_commit(stopped);
     __syncwarp();
     mbar_wait(stopped, 0);
     __syncwarp();
   }
-  if (warp == 12) tmem_dealloc(tmem, kTileTmemCols);
+  if (warp == kIssue) tmem_dealloc(tmem, 256 * STREAMS);
   if (many) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   // The rows are shared out over the blocks of the cluster: first what each part counts in a row and where the row goes, then four values a
   // thread.
@@ -607,7 +672,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_attention_kernel(const _
       s_offset[tid] = ((static_cast<long long>(seq.first_row) + at / p.group) * p.heads + kvh * p.group + at % p.group) * 64;
     }
     __syncthreads();
-    for (int e = tid; e < mine * 16; e += kTileThreads) {
+    for (int e = tid; e < mine * 16; e += kThreads) {
       const int i = e >> 4, r = from + i, c = e & 15;
       float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 2

@@ -257,8 +257,8 @@ template <int BITS, typename E, int STREAMS> int launch_tile(arcq::AttendParams&
 
 // Up to 128 rows: blocks of one stream, two on an SM, where there is a second for it and the keys are few, so that one block's set-up, loads and
 // join run beside the other's products; or where there is one tile of keys.  384 key heads, 40 rows: 128 keys 13.4 us against two streams'
-// 21.4, 384 keys 24.2 against 29.6, 700 keys 39.3 against 40.5, 900 keys 48.9 against 47.4; 140 key heads, 48 rows: 128 keys 7.0 against 7.9,
-// 250 keys 9.2 against 9.1, 500 keys 13.1 against 11.2.
+// 21.5, 384 keys 23.8 against 29.7, 577 keys 33.7 against 37.0, 900 keys 47.1 against 47.3, 1500 keys 65.1 against 62.2; 140 key heads, 48 rows:
+// 128 keys 7.0 against 7.9, 250 keys 9.0 against 9.2, 500 keys 12.9 against 11.1, 900 keys 20.8 against 15.7.
 bool one_stream_is_ahead(const arcq::AttendParams& p) {
   const int key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys;
   return key_tiles <= 1 || (key_tiles <= 6 && static_cast<long long>(p.batch) * p.kv_heads > arcq_host::sm_count());

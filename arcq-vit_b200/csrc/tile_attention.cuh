@@ -1,8 +1,8 @@
 // Attention of many queries a key head on the fifth-generation tensor cores: pieces of prompts over a cache, texts over an encoder's states.
 // Same operator as split_attention.cuh; keys and values are staged in shared memory (packed ones rebuilt in fp16 there, once a block).
 //
-// A block takes up to 256 rows, (query, head) pairs that share a key head, in two streams of 128 with scores and output of their own in tensor
-// memory, a softmax thread a row:
+// A block takes up to 256 rows, (query, head) pairs that share a key head, in two streams of 128 (or one, see below) with scores and output of
+// their own in tensor memory, a softmax thread a row:
 //   more than 128 rows   the streams are the two halves of the rows; both use every tile of 128 keys
 //   up to 128 rows       both streams have the same rows, one takes the even tiles of keys, the other the odd ones
 // so that one stream's exponentials run while the other's products do.  The keys of a row tile are also split over the blocks of a
@@ -11,8 +11,11 @@
 // Running maximum: a row's exponents are taken against a maximum that is renewed only when a score passes it by 2^8 (then the output in
 // tensor memory is scaled): probabilities reach 256 instead of 1 at most, and sums and products are as exact either way.
 //
-// Warps: 0-3 softmax of stream 0, 4-7 of stream 1 (a tensor-memory lane quarter each), 8-11 keys and values, 12 and 13 products of the
-// streams; 14 and 15 only keep step (registers are handed over by groups of four warps).
+// Warps: softmax, four a stream (a tensor-memory lane quarter each), then four for keys and values, then one a stream for its products; with two
+// streams two more only keep step (registers are handed over by groups of four warps).
+//
+// One stream: up to 128 rows over few keys in 16 bits.  Such blocks take half of an SM, so that two run side by side: a block's set-up, first loads
+// and join, together as long as its products, run beside the other block's (which kernel when: one_stream_is_ahead, with times).
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -26,7 +29,7 @@ namespace arcq {
 
 constexpr int kStatusTileAttentionTimeout = 0x502;
 constexpr int kTileRows = 128, kTileKeys = 128;
-__host__ __device__ constexpr int tile_threads(int streams) { return 256 * streams; }
+__host__ __device__ constexpr int tile_threads(int streams) { return streams == 1 ? 288 : 512; }
 // tiles of keys, and of values, in shared memory: 16 bits have no tables there, and one stream's blocks share an SM
 __host__ __device__ constexpr int tile_slots(bool packed, int streams) { return streams == 1 ? 2 : packed ? 3 : 5; }
 constexpr int kTileSeen = 8;
@@ -76,7 +79,7 @@ __device__ __forceinline__ float4 lds128_cluster(uint32_t addr) {
 template <int BITS, typename E, int STREAMS>
 __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_attention_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kThreads = tile_threads(STREAMS), kBlockRows = STREAMS * kTileRows;
-  constexpr int kLoad = 4 * STREAMS, kIssue = STREAMS == 1 ? 0 : kLoad + 4;      // first warps
+  constexpr int kLoad = 4 * STREAMS, kIssue = kLoad + 4;                         // first warps
   constexpr bool PACKED = BITS != 16;
   constexpr int SLOTS = tile_slots(PACKED, STREAMS);
   extern __shared__ uint8_t tile_smem_raw[];
@@ -109,7 +112,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
     pdl_launch_dependents();
     return;
   }
-  if (tid == (kIssue + 1) * 32) {
+  if (tid == (kIssue + STREAMS - 1) * 32) {
     const int users = halves ? STREAMS : 1;                                             // streams that read a tile of keys
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
@@ -124,6 +127,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
     mbar_fence_init();
   }
   if (warp == kIssue) {
+    __syncwarp();
     tmem_alloc(s_tmem, 256 * STREAMS);
     tmem_relinquish();
     tc_fence_before_sync();
@@ -150,40 +154,18 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
   // tile j of the block is tile i of stream t: halves: j = i for both; else j = 2 i + t
   bool ok = true;
 
-  // A tile's products, for a whole warp; q, k and v: descriptors of the queries and of the slot
-  const uint32_t idesc_s = tile_idesc<E>(kTileRows, kTileKeys);
-  const uint32_t idesc_o = tile_idesc<E>(kTileRows, 64) | (1u << 16);             // B with its rows (keys) along K
-  auto desc_lo = [&](uint32_t off) { return ((smem_u32(smem + off) & 0x3FFFFu) >> 4) | (1u << 16); };
-  auto issue_scores = [&](uint32_t tmem, int t, uint32_t q, uint32_t k, int slot) {
-    tc_fence_after_sync();
-    if (elect_one() && ok) {
-      umma_f16_x4(tmem + tile_s_col(t), q, k + slot * (kTileBytes >> 4), idesc_s);
-      umma_commit(s_full + t);
-      umma_commit(k_free + slot);
-    }
-    __syncwarp();
-  };
-  auto issue_output = [&](uint32_t tmem, int t, uint32_t v, int slot, bool fresh) {
-    tc_fence_after_sync();
-    if (elect_one() && ok) {
-#pragma unroll
-      for (int k = 0; k < kTileKeys; k += 16)
-        umma_f16_tmem_a_lo(tmem + tile_o_col(t), tmem + tile_p_col(t) + (k >> 1), v + slot * (kTileBytes >> 4) + 8 * k, idesc_o, !fresh || k > 0 ? 1u : 0u);
-      umma_commit(o_done + t);
-      umma_commit(v_free + slot);
-    }
-    __syncwarp();
-  };
-
-  if (STREAMS > 1 && warp >= kIssue) {
+  if (warp >= kIssue) {
     // ------------------------------------------------------------------ products: a warp a stream
-    fewer_registers<kTileIssueRegs>();
+    if constexpr (STREAMS > 1) fewer_registers<kTileIssueRegs>();
     fill_tables(tid - 128);
     set_up();
     const uint32_t tmem = *s_tmem;
     const int t = warp - kIssue;
     const int mine = t >= STREAMS ? 0 : halves ? count : (count + 1 - t) / 2;
     if (t < STREAMS && mine > 0) {
+      const uint32_t idesc_s = tile_idesc<E>(kTileRows, kTileKeys);
+      const uint32_t idesc_o = tile_idesc<E>(kTileRows, 64) | (1u << 16);         // B with its rows (keys) along K
+      auto desc_lo = [&](uint32_t off) { return ((smem_u32(smem + off) & 0x3FFFFu) >> 4) | (1u << 16); };
       const uint32_t q = desc_lo(L.q + (halves ? t : 0) * kTileBytes), k0 = desc_lo(L.k), v0 = desc_lo(L.v);
       auto at = [&](int i) { return halves ? i : 2 * i + t; };
       for (int i = 0; i <= mine; ++i) {
@@ -191,12 +173,27 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
           const int j = at(i), slot = j % SLOTS;
           ok = ok && (i > 0 || mbar_wait(q_full + (halves ? t : 0), 0, polls)) && mbar_wait(k_full + slot, (j / SLOTS) & 1, polls) &&
                (i == 0 || mbar_wait(s_read + t, (i - 1) & 1, polls));
-          issue_scores(tmem, t, q, k0, slot);
+          tc_fence_after_sync();
+          if (elect_one() && ok) {
+            umma_f16_x4(tmem + tile_s_col(t), q, k0 + slot * (kTileBytes >> 4), idesc_s);
+            umma_commit(s_full + t);
+            umma_commit(k_free + slot);
+          }
+          __syncwarp();
         }
         if (i > 0) {
           const int j = at(i - 1), slot = j % SLOTS;
           ok = ok && mbar_wait(v_full + slot, (j / SLOTS) & 1, polls) && mbar_wait(p_full + t, (i - 1) & 1, polls);
-          issue_output(tmem, t, v0, slot, i == 1);
+          tc_fence_after_sync();
+          if (elect_one() && ok) {
+#pragma unroll
+            for (int k = 0; k < kTileKeys; k += 16)
+              umma_f16_tmem_a_lo(tmem + tile_o_col(t), tmem + tile_p_col(t) + (k >> 1), v0 + slot * (kTileBytes >> 4) + 8 * k, idesc_o,
+                                 i > 1 || k > 0 ? 1u : 0u);
+            umma_commit(o_done + t);
+            umma_commit(v_free + slot);
+          }
+          __syncwarp();
         }
       }
     }
@@ -417,24 +414,11 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (STREAMS > 1 && lane == 0) mbar_arrive(q_full + (halves ? t : 0));
+      if (lane == 0) mbar_arrive(q_full + (halves ? t : 0));
     }
     asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory");
     const float scale = s_max[halves ? t * kTileRows + r : r];
     const uint32_t tmem = *s_tmem;
-    // One stream issues its products itself, behind barriers of its warps.
-    auto own_scores = [&](int j) {
-      if (warp != 0) return;
-      ok = ok && mbar_wait_warp(k_full + j % SLOTS, (j / SLOTS) & 1, polls);
-      issue_scores(tmem, 0, desc_lo(L.q), desc_lo(L.k), j % SLOTS);
-    };
-    auto own_output = [&](int j) {
-      if (warp != 0) return;
-      ok = ok && mbar_wait_warp(v_full + j % SLOTS, (j / SLOTS) & 1, polls);
-      issue_output(tmem, 0, desc_lo(L.v), j % SLOTS, j == 0);
-    };
-    auto all_rows_here = [] { asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory"); };
-    if (STREAMS == 1 && count > 0) own_scores(0);
     asm volatile("bar.sync 1, %0;" ::"n"(128 * STREAMS) : "memory");           // all have read theirs: s_max is free again
     const int mine = halves ? count : (count + 1 - t) / 2;
     const float ninf = __int_as_float(0xff800000);
@@ -456,8 +440,8 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
       tc_fence_after_sync();
       if (rows_here && ok) {
         const uint4 seen = lds128(smem_u32(s_seen + j % kTileSeen * 4));
-        // one stream's threads hold half of a row's scores at a time, and read the first half twice
-        constexpr int PART = STREAMS == 1 ? 2 : 4, PARTS = 4 / PART;
+        // One stream's threads, with 96 registers, hold a quarter of a row's scores at a time and read three of the quarters twice.
+        constexpr int PART = STREAMS == 1 ? 1 : 4, PARTS = 4 / PART;
         uint32_t s[PART][32];
         auto read_scores = [&](int part, bool last) {
 #pragma unroll
@@ -465,13 +449,8 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
           tmem_ld_wait();
           if (last) {
             tc_fence_before_sync();
-            if constexpr (STREAMS == 1) {
-              all_rows_here();
-              if (i + 1 < mine) own_scores(j + 1);
-            } else {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(s_read + t);
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read + t);
           }
         };
         const int base = (first + j) * kTileKeys;
@@ -502,8 +481,8 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
           for (int n = 0; n < 32; n += 2) {
             float& m = PART == 1 && (n & 2) ? m1 : m0;
             m = max3(m, __uint_as_float(s[0][n]), __uint_as_float(s[0][n + 1]));
-            if constexpr (PART > 1) m1 = max3(m1, __uint_as_float(s[1][n]), __uint_as_float(s[1][n + 1]));
             if constexpr (PART == 4) {
+              m1 = max3(m1, __uint_as_float(s[1][n]), __uint_as_float(s[1][n + 1]));
               m2 = max3(m2, __uint_as_float(s[2][n]), __uint_as_float(s[2][n + 1]));
               m3 = max3(m3, __uint_as_float(s[3][n]), __uint_as_float(s[3][n + 1]));
             }
@@ -559,25 +538,15 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
         your_turn();
         tmem_st_wait();
       } else {
-        if constexpr (STREAMS == 1) {
-          all_rows_here();
-          if (i + 1 < mine) own_scores(j + 1);
-        } else {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_read + t);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read + t);
         if (i > 0 && ok) ok = mbar_wait_warp(o_done + t, (i - 1) & 1, polls);
         my_turn();
         your_turn();
       }
       tc_fence_before_sync();
-      if constexpr (STREAMS == 1) {
-        all_rows_here();
-        own_output(j);
-      } else {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + t);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + t);
     }
     // ---- the stream's part: maximum, sum and output, as they are
     if (mine > 0) ok = ok && mbar_wait_warp(o_done + t, (mine - 1) & 1, polls);

@@ -675,6 +675,30 @@ def test_waits_of_the_tile_kernel_that_run_out(pkg, cuda_device, bits, B, n, S, 
     assert torch.equal(run(), want) and pkg.ops.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,S", [(33, 128), (40, 129), (128, 768), (77, 769), (100, 385)])
+def test_blocks_of_one_stream_and_of_two(pkg, cuda_device, dtype, n, S):
+    """More key heads than multiprocessors, up to 128 rows: states on both sides of where one kernel takes over, and pieces over pages."""
+    _cross_check(pkg, cuda_device, dtype, 160, n, S, 1, 1, "mask", seed=41)
+    _cross_check(pkg, cuda_device, dtype, 80, n // 2, S, 4, 2, "lengths", seed=42)
+    lengths = [max(1, S - (31 * i) % (S + 20)) for i in range(160)]
+    _paged_check(pkg, cuda_device, 16, dtype, 1, 1, 64, lengths, [min(n, 1 + (13 * i) % (n + 3)) for i in range(160)], seed=43)
+
+
+@pytest.mark.parametrize("polls", [0, 1, 3])
+@pytest.mark.parametrize("B,n,S", [(1, 40, 100), (200, 40, 700)])
+def test_waits_of_one_stream_that_run_out(pkg, cuda_device, polls, B, n, S):
+    gen = torch.Generator().manual_seed(33)
+    q, k = (torch.randn(B, t, 1, 64, generator=gen).half().to(cuda_device) for t in (n, S))
+    want = pkg.ops.cross_attention(q, k, k)
+    for _ in range(3):
+        with pkg._cabi.option("ARCQ_POLL_LIMIT", polls):
+            got = pkg.ops.cross_attention(q, k, k)
+        status = pkg.ops.device_status()
+        assert status == 0x502 or (polls > 0 and status == 0 and torch.equal(got, want))
+    assert torch.equal(pkg.ops.cross_attention(q, k, k), want) and pkg.ops.device_status() == 0
+
+
 def test_registers_and_workspaces_that_are_too_few(pkg, cuda_device):
     import ctypes
     import threading

@@ -33,6 +33,7 @@ __host__ __device__ constexpr int tile_threads(int streams) { return streams == 
 // tiles of keys, and of values, in shared memory: 16 bits have no tables there, and one stream's blocks share an SM
 __host__ __device__ constexpr int tile_slots(bool packed, int streams) { return streams == 1 ? 2 : packed ? 3 : 5; }
 constexpr int kTileSeen = 8;
+constexpr int kTileRanked = 64;                                    // sequences that are put in order at most
 // two streams' warps share out their registers
 constexpr int kTileLaunchRegs = 128, kTileSoftmaxRegs = 184, kTileLoadRegs = 88, kTileIssueRegs = 56;
 static_assert(2 * kTileSoftmaxRegs + kTileLoadRegs + kTileIssueRegs <= 4 * kTileLaunchRegs, "registers beyond the launch's never come");
@@ -76,7 +77,7 @@ __device__ __forceinline__ float4 lds128_cluster(uint32_t addr) {
   return v;
 }
 
-template <int BITS, typename E, int STREAMS>
+template <int BITS, typename E, int STREAMS, bool RANKED>
 __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_attention_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kThreads = tile_threads(STREAMS), kBlockRows = STREAMS * kTileRows;
   constexpr int kLoad = 4 * STREAMS, kIssue = kLoad + 4;                         // first warps
@@ -99,10 +100,33 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
   const uint32_t polls = p.poll_limit;
 
   const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int tile = p.tiles - 1 - unit / (p.kv_heads * p.batch);                   // long rows of causal keys first
-  const int kvh = unit % p.kv_heads, b = unit / p.kv_heads % p.batch;
+  const int kvh = unit % p.kv_heads;
+  int tile = p.tiles - 1 - unit / (p.kv_heads * p.batch), b = unit / p.kv_heads % p.batch;      // long rows of causal keys first
 
   pdl_wait();
+  if constexpr (RANKED) {
+    // The sequences with most work first, by the keys that their streams go through: blocks beyond the first round start as others end, and the
+    // last to start should be short (when: launch_tile; a kernel of its own, since the choice alone takes 1 % of the others' time).
+    __shared__ uint32_t s_work[kTileRanked];
+    __shared__ int s_b;
+    uint32_t work = 0;
+    if (tid < p.batch) {
+      const AttendSequence s = attend_sequence(p, tid);
+      const long long rows = static_cast<long long>(s.queries) * p.group;
+      work = rows == 0 ? 0u : static_cast<uint32_t>(s.keys) * (rows > kTileRows ? 2u : 1u);
+      s_work[tid] = work;
+    }
+    __syncthreads();
+    const int rank = unit / (p.kv_heads * p.tiles);
+    if (tid < p.batch) {
+      int before = 0;
+      for (int i = 0; i < p.batch; ++i) before += s_work[i] > work || (s_work[i] == work && i < tid) ? 1 : 0;
+      if (before == rank) s_b = tid;
+    }
+    __syncthreads();
+    b = s_b;
+    tile = p.tiles - 1 - unit / p.kv_heads % p.tiles;
+  }
   const AttendSequence seq = attend_sequence(p, b);
   const int all_rows = seq.queries * p.group;
   const bool halves = STREAMS == 1 || all_rows > kTileRows;                       // the streams are halves of the rows; or there is one

@@ -67,7 +67,7 @@ def test_attention_that_is_refused(lib, pkg):
     assert _paged(lib, c, rows=3) == BAD_SHAPE and _paged(lib, c, batch=-1) == BAD_SHAPE and _paged(lib, c, width=1 << 31) == TOO_LARGE
     assert _paged(lib, c, lengths=None) == BAD_ARG and _paged(lib, c, table=None) == BAD_ARG and _paged(lib, c, q=None) == BAD_ARG
     assert _paged(lib, c, q=(1 << 20) + 8) == ALIGN and _paged(lib, c, qs=(256, 60)) == ALIGN and _paged(lib, c, out=(1 << 20) + 2) == ALIGN
-    for s in (0.0, -0.125, float("inf"), float("nan")):
+    for s in (0.0, -0.125, float("inf"), float("nan"), 3e38):
         assert _paged(lib, c, scale=s) == BAD_ARG and _cross(lib, scale=s) == BAD_ARG
     assert _paged(lib, _cache(pkg, bits=16, dtype=2)) == BAD_ARG
     assert _paged(lib, c, batch=0, rows=0) == 0 and _paged(lib, c, rows=0, starts=1 << 20) == 0

@@ -685,6 +685,16 @@ def test_blocks_of_one_stream_and_of_two(pkg, cuda_device, dtype, n, S):
     _paged_check(pkg, cuda_device, 16, dtype, 1, 1, 64, lengths, [min(n, 1 + (13 * i) % (n + 3)) for i in range(160)], seed=43)
 
 
+@pytest.mark.parametrize("bits,dtype", [(4, torch.float16), (16, torch.bfloat16)])
+@pytest.mark.parametrize("B,heads,kv_heads", [(2, 100, 100), (24, 14, 7), (64, 6, 3), (65, 6, 3)])
+def test_sequences_in_the_order_of_their_work(pkg, cuda_device, bits, dtype, B, heads, kv_heads):
+    """A few rounds of blocks, sequences of equal and of different work, some without queries or keys."""
+    lengths = [0 if i % 13 == 5 else 150 + 90 * (i * 5 % 7) for i in range(B)]
+    _paged_check(pkg, cuda_device, bits, dtype, heads, kv_heads, 64, lengths, [0 if i % 11 == 3 else 1 + 37 * (i * 3 % 5) for i in range(B)], seed=51)
+    if bits == 16:
+        _cross_check(pkg, cuda_device, dtype, B, 70, 400, heads, kv_heads, "lengths", seed=52)
+
+
 @pytest.mark.parametrize("polls", [0, 1, 3])
 @pytest.mark.parametrize("B,n,S", [(1, 40, 100), (200, 40, 700)])
 def test_waits_of_one_stream_that_run_out(pkg, cuda_device, polls, B, n, S):

@@ -147,20 +147,60 @@ void split_shape(arcq::AttendParams& p) {
   p.tiles = static_cast<int>((rows + arcq::kSplitRows - 1) / arcq::kSplitRows);
   p.part_rows = static_cast<int>(rows < arcq::kSplitRows ? rows : arcq::kSplitRows);
 }
-bool few_rows(const arcq::AttendParams& p) { return static_cast<long long>(p.max_new) * p.group <= 2 * arcq::kSplitRows; }
-
-// Up to 8 rows a key head the split kernel is always ahead (12 heads, 8 rows, 4 bits: over 300 tokens 8.3 us against the tile kernel's 9.3, over 16 000
-// 20.6 against 33.7).  For 9 to 32 rows it is where keys times key heads are many.  In 4 bits, 16 rows: 96 000 of them 16.0 us against 16.9, 192 000
-// 28.8 against 33.9; below, 48 000 21.2 against 18.0; 32 rows: 384 000 32.7 against 33.0, 768 000 55 against 64.  In 16 bits, where the tile kernel
-// has no codes to look up: 192 000 34.0 against 30.1, 360 000 41.1 against 44.8.
-template <int BITS> bool split_is_ahead(const arcq::AttendParams& p) {
-  constexpr long long kMany = BITS == 16 ? 5 << 16 : 2 << 16;
-  return few_rows(p) && (static_cast<long long>(p.max_new) * p.group <= 8 || static_cast<long long>(p.batch) * p.kv_heads * p.max_keys > kMany);
-}
+// rows of a key head that the split kernel may have; a workspace is asked for up to them
+bool few_rows(const arcq::AttendParams& p) { return static_cast<long long>(p.max_new) * p.group <= 4 * arcq::kSplitRows; }
 
 // Over up to so many keys units are not cut between blocks, which spares the second kernel: 12 heads, 1 token, 4 bits, 512 keys 9.4 us against 11.2,
 // 1024 keys 11.5 against 13.0, 1536 keys 13.4 against 12.5; 50 sequences of up to 1024 keys 16.6 against 16.2.
 constexpr int kWholeUnitKeys = 1152;
+
+// About how long calls over up to kWholeUnitKeys keys take (us; fitted over 60 to 1500 key heads, 1 to 64 rows, 10 to 500 keys; off by a fifth).
+// Split kernel, units cut between a block's warps: every warp has as much to do, and the block joins parts.  Units whole in a warp: nothing is
+// joined, but a warp has whole units to do, at up to twice the pace where few warps have any.  The latter is ahead where units are many or
+// short: 600 key heads, 16 rows, 16 bits, 64 keys 8.3 against 14.2, 500 keys 24.9 against 30.9; 204 key heads, 1 row, 500 keys 17.7 against 10.6.
+struct SplitTimes {
+  double cut, whole;
+};
+template <int BITS> SplitTimes split_times(const arcq::AttendParams& p) {
+  const double rows = static_cast<double>(p.max_new) * p.group, warps = static_cast<double>(arcq_host::sm_count()) * arcq::kSplitWarps;
+  const double units = static_cast<double>(p.batch) * p.kv_heads * ceil(rows / arcq::kSplitRows), steps = p.max_keys / arcq::SplitStep<BITS>::kKeys + 1;
+  const double set_up = BITS == 16 ? 4.7 : 8.0, a_block = units / arcq_host::sm_count();
+  const double join = BITS == 16 ? (rows <= 8 ? 1.2 + 0.05 * rows * a_block : 4.0 + 1.75 * a_block) : (rows <= 8 ? 2.4 : 4.0 + 0.5 * a_block);
+  const double share = fmax(units * steps / warps, 0.4), busy = fmin(units / warps, 1.0);
+  const double cut_step = BITS != 16 && rows > 8 ? 2.2 : 1.25, whole_step = BITS == 16 ? 0.45 * (1.0 + busy) : 1.0 + 1.3 * busy;
+  return {set_up + join + share * cut_step, set_up + ceil(units / warps) * steps * whole_step};
+}
+// Up to 128 rows: blocks of one stream, two on an SM, where there is a second for it and the keys are few, so that one block's set-up, loads and
+// join run beside the other's products; or where there is one tile of keys.  384 key heads, 40 rows: 128 keys 13.4 us against two streams'
+// 21.5, 384 keys 23.8 against 29.7, 577 keys 33.7 against 37.0, 900 keys 47.1 against 47.3, 1500 keys 65.1 against 62.2; 140 key heads, 48 rows:
+// 128 keys 7.0 against 7.9, 250 keys 9.0 against 9.2, 500 keys 12.9 against 11.1, 900 keys 20.8 against 15.7.
+bool one_stream_is_ahead(const arcq::AttendParams& p) {
+  const int key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys;
+  return key_tiles <= 1 || (key_tiles <= 6 && static_cast<long long>(p.batch) * p.kv_heads > arcq_host::sm_count());
+}
+
+// The tile kernel likewise, for up to 128 rows
+template <int BITS> double tile_time(const arcq::AttendParams& p) {
+  const double units = static_cast<double>(p.batch) * p.kv_heads, sms = arcq_host::sm_count(), tiles = fmax(ceil(p.max_keys / static_cast<double>(arcq::kTileKeys)), 1.0);
+  const double splits = fmax(fmin(fmin(floor(sms / units), 8.0), tiles), 1.0);    // blocks of a cluster
+  const double one = 5.8 + 2.2 * (tiles - 1.0), two = 7.4 + 0.85 * (ceil(tiles / splits) - 1.0) + (splits > 1.0 ? 1.0 : 0.0);
+  return 0.5 + (BITS == 16 && one_stream_is_ahead(p) ? ceil(units / (2.0 * sms)) * one : ceil(units / sms) * two);
+}
+// Up to 8 rows a key head the split kernel is always ahead (12 heads, 8 rows, 4 bits: over 300 tokens 8.3 us against the tile kernel's 9.3, over 16 000
+// 20.6 against 33.7); above, over short contexts, by the times (1500 key heads, 16 rows, 30 keys: 16 bits 7.4
+// against 35.5, 4 bits 9.0 against 79; 204 key heads, 250 keys: 16 bits 13.1 against 9.9).  Over long ones, 9 to 32 rows, it is where keys times key heads
+// are many.  In 4 bits, 16 rows: 192 000 of them 28.8 against 33.9; below, 48 000 21.2 against 18.0; 32 rows: 384 000 32.7 against 33.0, 768 000
+// 55 against 64.  In 16 bits, where the tile kernel has no codes to look up: 192 000 34.0 against 30.1, 360 000 41.1 against 44.8.
+template <int BITS> bool split_is_ahead(const arcq::AttendParams& p) {
+  constexpr long long kMany = BITS == 16 ? 5 << 16 : 2 << 16;
+  const long long rows = static_cast<long long>(p.max_new) * p.group;
+  if (rows <= 8 || !few_rows(p)) return few_rows(p);
+  if (p.max_keys <= kWholeUnitKeys) {
+    const SplitTimes t = split_times<BITS>(p);
+    return fmin(t.cut, t.whole) < tile_time<BITS>(p);
+  }
+  return rows <= 2 * arcq::kSplitRows && static_cast<long long>(p.batch) * p.kv_heads * p.max_keys > kMany;
+}
 
 template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
@@ -187,7 +227,8 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
     return fail(ARCQ_E_BAD_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)arcq::split_workspace(p, sms));
   const long long units = arcq::split_units(p), unit_steps = p.max_keys / arcq::SplitStep<BITS>::kKeys + 1, steps = units * unit_steps;
   if (static_cast<double>(units) * unit_steps > 1073741823.0) return fail(ARCQ_E_TOO_LARGE, "too many queries and keys for one call");
-  p.whole_units = p.max_keys <= kWholeUnitKeys;
+  const SplitTimes times = split_times<BITS>(p);
+  p.whole_units = p.max_keys > kWholeUnitKeys ? 0 : times.whole < times.cut ? 2 : 1;
   cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
   if (e == cudaSuccess && !p.whole_units) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
@@ -261,15 +302,6 @@ template <int BITS, typename E, int STREAMS> int launch_tile(arcq::AttendParams&
   if (units * splits > 0x7fffffffLL) return fail(ARCQ_E_TOO_LARGE, "too many queries for one call");
   const cudaError_t e = launch(in_order ? ranked : k, dim3(static_cast<unsigned>(units * splits)), threads, smem, splits, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
-}
-
-// Up to 128 rows: blocks of one stream, two on an SM, where there is a second for it and the keys are few, so that one block's set-up, loads and
-// join run beside the other's products; or where there is one tile of keys.  384 key heads, 40 rows: 128 keys 13.4 us against two streams'
-// 21.5, 384 keys 23.8 against 29.7, 577 keys 33.7 against 37.0, 900 keys 47.1 against 47.3, 1500 keys 65.1 against 62.2; 140 key heads, 48 rows:
-// 128 keys 7.0 against 7.9, 250 keys 9.0 against 9.2, 500 keys 12.9 against 11.1, 900 keys 20.8 against 15.7.
-bool one_stream_is_ahead(const arcq::AttendParams& p) {
-  const int key_tiles = (p.max_keys + arcq::kTileKeys - 1) / arcq::kTileKeys;
-  return key_tiles <= 1 || (key_tiles <= 6 && static_cast<long long>(p.batch) * p.kv_heads > arcq_host::sm_count());
 }
 
 template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {

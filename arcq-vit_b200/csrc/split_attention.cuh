@@ -8,7 +8,8 @@
 // lengths are: long sequences are spread over the GPU as evenly as many short ones.  A warp keeps the running maximum and sum and the
 // 16 x 64 accumulator in registers; it writes a unit that lies in its piece whole, and of one that does not (at most the first and the last)
 // its part.  Parts of a block's warps are added up in the block, those of several blocks by the join kernel behind it, both in the order of the
-// keys.  With short contexts the line is cut at the units' ends and there is no second kernel.
+// keys.  With short contexts the line is cut between blocks at the units' ends and there is no second kernel; where units are many or short it
+// is cut so between warps too, and nothing is joined.
 //
 // Each warp has a ring of steps in shared memory of its own, filled by asynchronous copies two steps ahead (no barriers).  Packed rows are
 // copied as they are, and two codes become two levels in fp16 on the way into the tensor instructions with one read: their byte (or 4 or 6 bits) is
@@ -62,7 +63,7 @@ struct AttendParams {
   int heads, kv_heads, group, tiles, splits, batch;
   void* workspace;                      // split_attention_kernel
   int part_rows;                        // of a part: 16, or all rows that there can be
-  int whole_units;                      // each block has whole units
+  int whole_units;                      // 1: each block has whole units, 2: each warp
   uint32_t poll_limit;                  // tile_attention.cuh
   int* status;
 };
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   using Step = SplitStep<BITS>;
   constexpr int KEYS = Step::kKeys, NT = KEYS / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_scan[kSplitWarps], s_ends[2];
+  __shared__ int s_scan[kSplitWarps], s_ends[kSplitWarps + 1];
   __shared__ int2 s_found[kSplitWarps];
   __shared__ struct {
     int at, b, kvh, tile, rows, steps, first_row;
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     static_cast<SplitHeader*>(p.workspace)->piece = piece;
   }
   if (from >= to) return;
-  const int per = (to - from + kSplitWarps - 1) / kSplitWarps, start = min(from + warp * per, to), end = min(start + per, to);
+  const int per = (to - from + kSplitWarps - 1) / kSplitWarps;
+  int start = min(from + warp * per, to), end = min(start + per, to);
   // parts of this block's warps; the units they are of, by the warp that has the first: 0 .. (begun there), kSplitWarps (before the block's piece)
   float* const parts = p.part_rows <= kSplitSharedRows ? reinterpret_cast<float*>(smem + split_parts<BITS>() - (PACKED ? smem_u32(smem) : 0))
                                                        : split_part(p, 2ll * gridDim.x + 2ll * kSplitWarps * blockIdx.x);
@@ -479,9 +481,20 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   if (tid <= kSplitWarps) s_groups[tid].rows = 0;
   line.find(kSplitWarps, [&](int w) { return from + w * per; }, s_found);
   __syncthreads();
+  int at = start;
+  SplitUnit u;
+  if (start < to) u = line.locate(p, start, s_found + warp, at);
+  if (p.whole_units == 2) {                                                        // the units that begin in the warp's piece
+    if (at < start) {
+      at += u.steps;
+      if (at < to) u = split_next<Units>(p, u.b, u.kvh, u.tile);
+    }
+    start = at;
+    if (lane == 0) s_ends[warp] = at;
+    __syncthreads();
+    end = warp + 1 < kSplitWarps ? s_ends[warp + 1] : to;
+  }
   if (start < end) {
-  int at;
-  SplitUnit u = line.locate(p, start, s_found + warp, at);
 
   const uint32_t ring = split_ring<BITS>(smem_u32(smem), warp);
   // ---- copies, two steps ahead of the computation, in halves of sixteen keys (16 bits: whole steps).  A run is what lies side by side: the rest

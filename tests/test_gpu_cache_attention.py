@@ -685,6 +685,15 @@ def test_blocks_of_one_stream_and_of_two(pkg, cuda_device, dtype, n, S):
     _paged_check(pkg, cuda_device, 16, dtype, 1, 1, 64, lengths, [min(n, 1 + (13 * i) % (n + 3)) for i in range(160)], seed=43)
 
 
+@pytest.mark.parametrize("bits,dtype", [(4, torch.float16), (3, torch.bfloat16), (16, torch.float16), (16, torch.bfloat16)])
+@pytest.mark.parametrize("B,kv_heads,new", [(50, 12, 16), (50, 12, 1), (300, 6, 8), (340, 6, 17), (120, 5, 33), (40, 12, 64), (1900, 1, 3)])
+@pytest.mark.parametrize("longest", [1, 130])
+def test_many_short_units(pkg, cuda_device, bits, dtype, B, kv_heads, new, longest):
+    """Units that warps have whole, more and fewer than warps, of different lengths, some without queries or keys."""
+    lengths = [(longest - (7 * i) % (longest + 1)) for i in range(B)]
+    _paged_check(pkg, cuda_device, bits, dtype, kv_heads, kv_heads, 16, lengths, [0 if i % 9 == 4 else 1 + (5 * i) % new for i in range(B)], seed=61)
+
+
 @pytest.mark.parametrize("bits,dtype", [(4, torch.float16), (16, torch.bfloat16)])
 @pytest.mark.parametrize("B,heads,kv_heads", [(2, 100, 100), (24, 14, 7), (64, 6, 3), (65, 6, 3)])
 def test_sequences_in_the_order_of_their_work(pkg, cuda_device, bits, dtype, B, heads, kv_heads):

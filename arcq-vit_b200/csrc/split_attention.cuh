@@ -24,7 +24,7 @@
 // that lie side by side.
 //
 // Bound by instructions: some 700 a step and warp (32 keys, 16 rows or fewer), three warps a scheduler, 0.83 issued a cycle.  1 token over 64
-// contexts of up to 4096, 12 heads over 4 key heads, 4 bits: 30 us, 24 % of the copy bandwidth (47 MB); over two of 65 521 in 3 bits, 12 heads: 53 us.
+// contexts of up to 4096, 12 heads over 4 key heads, 4 bits: 29 us, 25 % of the copy bandwidth (47 MB); over two of 65 521 in 3 bits, 12 heads: 51 us.
 // Few steps: set-up and latency, 1 token over 333: 8.5 us.
 #pragma once
 #include <cuda_fp16.h>

@@ -718,6 +718,41 @@ def test_waits_of_one_stream_that_run_out(pkg, cuda_device, polls, B, n, S):
     assert torch.equal(pkg.ops.cross_attention(q, k, k), want) and pkg.ops.device_status() == 0
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+def test_a_threads_first_calls_are_captured(pkg, cuda_device, bits):
+    """Nothing has been set up in the thread: every kernel's first launch there goes into a graph, on a stream of its own."""
+    import threading
+    gen = torch.Generator().manual_seed(71)
+    c = _filled(pkg, gen, 40, 2, 64, bits, torch.float16, cuda_device)
+    args = {n: c.get(n) for n in ("k_stats", "v_stats", "codebooks")}
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    table, lengths = torch.arange(40, **i32).reshape(2, 20), torch.tensor([1280, 77], **i32)
+    qs = {n: torch.randn(2 * n, 4, 64, generator=gen).half().to(cuda_device) for n in (1, 30, 200)}
+    states = torch.randn(2, 90, 4, 64, generator=gen).half().to(cuda_device)
+
+    def run():
+        outs = [pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, lengths, None, n, **args) for n, q in qs.items()]
+        return outs + [pkg.ops.cross_attention(q.reshape(2, n, 4, 64), states, states) for n, q in qs.items()]
+    results = []
+
+    def capture():
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, capture_error_mode="thread_local"):
+                outs = run()
+            g.replay()
+            torch.cuda.synchronize()
+            results.append((g, outs))
+        except Exception as e:                                          # noqa: BLE001  (shown by the test's own thread)
+            results.append(e)
+    torch.cuda.synchronize()
+    t = threading.Thread(target=capture)
+    t.start()
+    t.join()
+    assert isinstance(results[0], tuple), results[0]
+    assert all(torch.equal(a, b) for a, b in zip(results[0][1], run())) and pkg.ops.device_status() == 0
+
+
 def test_registers_and_workspaces_that_are_too_few(pkg, cuda_device):
     import ctypes
     import threading

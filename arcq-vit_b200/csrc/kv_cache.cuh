@@ -8,7 +8,8 @@
 //   center        mean - scale * code_sum / 64
 //   value         center + scale * level
 // Center and scale are rounded to fp16: 2^-11 of a value, against quantization steps of 0.1 (4 bits) to 0.6 scale, for 36 instead of 40
-// bytes a row; a center or scale beyond fp16's range is held at its end.
+// bytes a row; a center or scale beyond fp16's range is held at its end.  A group with a NaN or an infinity has a NaN for both (the mean is not
+// finite, so the scale is NaN, and with it the center): all of its 64 values are read back as NaN.
 // A slot is page * page_size + place in it; tokens whose slot is negative or beyond the cache are neither written nor read (zeros).
 #pragma once
 #include <cuda_fp16.h>
@@ -45,7 +46,8 @@ __device__ __forceinline__ long long kv_row(long long slot, int head, int heads,
   return ((page * heads + head) << page_shift) + (slot & ((1ll << page_shift) - 1));
 }
 
-__device__ __forceinline__ __half kv_half(float v) { return __float2half_rn(fminf(fmaxf(v, -65504.0f), 65504.0f)); }
+// held to fp16's range; NaN stays NaN (fmaxf would drop it)
+__device__ __forceinline__ __half kv_half(float v) { return __float2half_rn(v == v ? fminf(fmaxf(v, -65504.0f), 65504.0f) : v); }
 
 // 8 codes of BITS bits, one per nibble
 template <int BITS> __device__ __forceinline__ uint32_t spread_codes(uint32_t x) {

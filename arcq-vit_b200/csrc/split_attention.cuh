@@ -756,8 +756,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       // multiplies all three sums by cancels in the end.
       float v_log = 0.0f;
       if constexpr (PACKED) {
-        const uint32_t own = (seen >> lane) & 1 ? lds32(src + 2 * Step::kRows + Step::kStats + lane * 4) >> 16 : 0u;
-        v_log = static_cast<float>(static_cast<int>(__reduce_max_sync(0xffffffffu, own) >> 10) - 15);
+        const uint32_t own = (seen >> lane) & 1 ? (lds32(src + 2 * Step::kRows + Step::kStats + lane * 4) >> 26) & 31u : 0u;       // without the sign, which a NaN may have
+        v_log = static_cast<float>(static_cast<int>(__reduce_max_sync(0xffffffffu, own)) - 15);
       }
       float m[2] = {ninf, ninf};
 #pragma unroll

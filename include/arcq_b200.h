@@ -404,7 +404,8 @@ int arcq_dense_weight_gemm_prefetch(const void* xhat, const void* w16, const flo
  *   bits 16      row = 64 values of `dtype` (fp16 or bf16); stats and codebooks are not used
  *   bits 2, 3, 4 row = 8 * bits bytes: the codes of one quantizer group, as arcq_act_quant packs them, bit for bit;
  *                stats fp16 [pages, heads, page_size, 2] = (mean - scale * code_sum / 64, scale) rounded to fp16 (and held to its
- *                range); codebooks fp32 [2, 2^bits], keys' and values'.  A value is stats[0] + stats[1] * codebook[code].
+ *                range); codebooks fp32 [2, 2^bits], keys' and values'.  A value is stats[0] + stats[1] * codebook[code].  A group with a
+ *                NaN or an infinity in it has NaN statistics: all 64 values are NaN.
  * page_size: a power of two, 16 or more.  Buffers contiguous, 16-byte aligned.
  */
 typedef struct arcq_kv_cache {

@@ -1,0 +1,102 @@
+"""What the values in a cache may be: NaN and infinities, magnitudes far apart, and roundings that have to cancel."""
+import pytest
+import torch
+
+from test_gpu_cache_attention import U, _cached, _empty_cache, _levels
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+
+
+def _pages_args(c):
+    return {n: c.get(n) for n in ("k_stats", "v_stats", "codebooks")}
+
+
+# ---------------------------------------------------------------- NaN and infinities
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [2, 3, 4])
+@pytest.mark.parametrize("tokens", [40, 1300])                      # eight lanes a group, and a lane
+def test_groups_that_are_not_finite_are_read_back_as_nan(pkg, cuda_device, bits, dtype, tokens):
+    gen = torch.Generator().manual_seed(tokens + bits)
+    pages = -(-tokens // 16)
+    x = [torch.randn(tokens, 2, 64, generator=gen).to(dtype).to(cuda_device) for _ in range(2)]
+    hit = [torch.zeros(tokens, 2, dtype=torch.bool, device=cuda_device) for _ in range(2)]
+    bad = [t.clone() for t in x]
+    for which, token, head, at in ((0, 3, 0, {5: NAN}), (0, 17, 1, {63: INF}), (0, tokens - 1, 0, {0: -INF}), (1, 3, 1, {9: INF, 10: -INF}),
+                                   (1, 4, 0, dict.fromkeys(range(64), INF)), (1, 21, 0, dict.fromkeys(range(64), NAN)), (1, 22, 1, {31: -INF, 32: NAN})):
+        for i, value in at.items():
+            bad[which][token, head, i] = value
+        hit[which][token, head] = True
+    slots = torch.randperm(pages * 16, generator=gen)[:tokens].to(cuda_device)
+    got = []
+    for k, v in (x, bad):
+        c, th = _empty_cache(pages, 2, 16, bits, dtype, cuda_device)
+        pkg.ops.kv_cache_write(k, v, slots, thresholds=th, **c)
+        got.append(pkg.ops.kv_cache_read(slots, out_dtype=torch.float32, **c))
+    for clean, y, h in zip(*got, hit):
+        assert bool(torch.isnan(y[h]).all()), y[h][~torch.isnan(y[h])]
+        assert torch.equal(y[~h], clean[~h])
+
+
+def _plain(q, k, v, seen):
+    """One head in 64 bits: q [n, 64], k, v [S, 64], seen [n, S] -> [n, 64]; values that are not seen do not count."""
+    s = (0.125 * q.double() @ k.double().t()).masked_fill(~seen, -INF)
+    w = torch.softmax(s, -1)
+    return torch.stack([w[i][seen[i]] @ v.double()[seen[i]] for i in range(q.shape[0])])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [2, 3, 4, 16])
+@pytest.mark.parametrize("new", [1, 2, 130])                         # few rows, and the tile kernel
+@pytest.mark.parametrize("which,value", [("k", NAN), ("k", INF), ("v", NAN), ("v", INF), ("v", -INF)])
+def test_what_is_not_finite_and_seen_shows(pkg, cuda_device, bits, dtype, new, which, value):
+    """NaN and infinities where the formula has them, and nowhere else: not with another key head and not in another sequence."""
+    gen = torch.Generator().manual_seed(new)
+    H, Hk, page, L, at = 4, 2, 16, 150, 20                             # every query sees token 20
+    pages = 20
+    x = {n: (0.5 * torch.randn(pages * page, Hk, 64, generator=gen)).to(dtype).to(cuda_device) for n in "kv"}
+    table = torch.randperm(pages, generator=gen).to(torch.int32).reshape(2, 10)
+    slot = int(table[0, at // page]) * page + at % page
+    q = (0.5 * torch.randn(2 * new, H, 64, generator=gen)).to(dtype).to(cuda_device)
+    lengths = torch.full((2,), L, dtype=torch.int32, device=cuda_device)
+    outs = []
+    for planted in (False, True):
+        if planted:
+            x[which][slot, 0, 7] = value
+        c, th = _empty_cache(pages, Hk, page, bits, dtype, cuda_device)
+        pkg.ops.kv_cache_write(x["k"], x["v"], torch.arange(pages * page, device=cuda_device), thresholds=th, **c)
+        outs.append(pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table.to(cuda_device), lengths, None, new, **_pages_args(c)))
+    clean, got = outs
+    assert torch.equal(got[new:], clean[new:]) and torch.equal(got[:new, 2:], clean[:new, 2:])
+    j = torch.arange(L)
+    rows = torch.stack([table[0][j // page].long(), j % page], 1).to(cuda_device)
+    k, v = (_cached(pkg, c, n, rows)[0][:, 0] for n in "kv")
+    seen = (j[None] <= (L - new + torch.arange(new))[:, None]).to(cuda_device)
+    for h in range(2):
+        want = _plain(q[:new, h], k, v, seen)
+        assert not bool(torch.isfinite(want).all()) or (bits, which, value) == (16, "k", INF)      # a score of -inf has no weight
+        y = got[:new, h].double()
+        assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y[torch.isinf(want)], want[torch.isinf(want)])
+        fine = torch.isfinite(want)
+        # scores below 8 * 64 / 8 * 2^-10 off, roundings of weights and outputs: far below a tenth of values of 0.5
+        assert bool(((y - want)[fine].abs() <= 0.05).all())
+    assert pkg.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4, 16])
+@pytest.mark.parametrize("new", [2, 9, 130])
+def test_a_later_key_that_is_nan_has_no_effect_on_earlier_queries(pkg, cuda_device, bits, new):
+    gen = torch.Generator().manual_seed(5)
+    x = [torch.randn(160, 1, 64, generator=gen).half().to(cuda_device) for _ in range(2)]
+    q = torch.randn(new, 2, 64, generator=gen).half().to(cuda_device)
+    table = torch.arange(10, dtype=torch.int32, device=cuda_device)[None]
+    length = torch.tensor([150], dtype=torch.int32, device=cuda_device)
+    outs = []
+    for planted in (False, True):
+        if planted:
+            x[0][149, 0, 3] = NAN
+        c, th = _empty_cache(10, 1, 16, bits, torch.float16, cuda_device)
+        pkg.ops.kv_cache_write(x[0], x[1], torch.arange(160, device=cuda_device), thresholds=th, **c)
+        outs.append(pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, length, None, new, **_pages_args(c)))
+    assert torch.equal(outs[1][:-1], outs[0][:-1]) and bool(torch.isnan(outs[1][-1]).all())

@@ -210,10 +210,14 @@ template <int BITS> __host__ __device__ constexpr uint32_t split_parts() {
 }
 // A level in fp16, rounded up in a share of the copies that is the position between its neighbours: the copies of lanes 4g + c, low and high,
 // serve different keys (values) or parts of a head (keys), over which the roundings then average out.
-__device__ __forceinline__ __half dithered_level(float x, int eighth) {
+// `sixteenths` of the way from one neighbour to the next is where rounding up begins.  Low and high of c = 0 .. 3 have 7 and 9, 5 and 11, 3 and 13, 1 and
+// 15: a pair is off to neither side on average, and the first keys of a context, which have c = 0, are rounded almost to the nearest.  Error against
+// 64 bits in 4 bits and fp16, relative to the output, over 1, 8, 32 and 333 keys:
+// 2.8, 3.3, 3.2, 2.4e-4 (the output's rounding alone: 2.1e-4); with shares rising from 1 for c = 0 to 15 for c = 3 6.1, 5.6, 3.4, 2.3e-4.
+__device__ __forceinline__ __half dithered_level(float x, int sixteenths) {
   const __half down = __float2half_rd(x), up = __float2half_ru(x);
   const float a = __half2float(down), b = __half2float(up);
-  return (x - a) * 16.0f > (b - a) * (2 * eighth + 1) ? up : down;
+  return (x - a) * 16.0f > (b - a) * sixteenths ? up : down;
 }
 // Entry i of the table: codes i & (levels - 1) and i >> BITS.
 template <int BITS> __device__ __forceinline__ void fill_split_table(const float* codebooks, int tid, int threads) {
@@ -224,7 +228,7 @@ template <int BITS> __device__ __forceinline__ void fill_split_table(const float
     uint32_t w[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const __half2 h = __halves2half2(dithered_level(lo, 2 * c), dithered_level(hi, 2 * c + 1));
+      const __half2 h = __halves2half2(dithered_level(lo, 7 - 2 * c), dithered_level(hi, 9 + 2 * c));
       w[c] = *reinterpret_cast<const uint32_t*>(&h);
     }
 #pragma unroll

@@ -129,3 +129,40 @@ def test_roundings_of_levels_have_no_direction(pkg, cuda_device, bits, keys):
         total += float(((got - v.mean(0)) / unit).sum())
         count += got.numel()
     assert abs(total / count) <= (1 / 16 if keys < 4 else 0.0) + 4 * 0.29 / 20
+
+
+# ---------------------------------------------------------------- values of very different sizes
+@pytest.mark.parametrize("bits", [2, 3, 4])
+@pytest.mark.parametrize("new", [1, 2])
+@pytest.mark.parametrize("L,at", [(20, 0), (32, 31), (32, 5), (77, 76), (77, 33)])
+def test_a_large_value_that_hardly_counts_costs_the_others_nothing(pkg, cuda_device, bits, new, L, at):
+    """Few rows: one value ten million times the others, with a weight of e^-60 or not seen at all (the last token, by the query before it).
+
+    Keys of the others are 0 as good as exactly, so they weigh alike, 1 / n each.  The bound: a level's rounding (`_cached`), a weight times scale
+    rounded to fp16 (2^-11, or 2^-25 of the largest of the call's steps, exponents a step has up to 2^6 apart and a maximum's lag of 2^8 on
+    the safe side: n 2^-18 of it), scores 2^-12, sums n 2^-23, and the output's rounding, subnormal below 2^-14."""
+    gen = torch.Generator().manual_seed(L + at)
+    sign = torch.where(torch.rand(64, generator=gen) < 0.5, -1.0, 1.0)
+    k = torch.zeros(128, 1, 64)
+    k[at] = -8 * sign
+    v = 0.003 * torch.randn(128, 1, 64, generator=gen)
+    v[at] = 2.5e4 * torch.randn(64, generator=gen).clamp(-2, 2)
+    k, v = k.half().to(cuda_device), v.half().to(cuda_device)
+    c, th = _empty_cache(8, 1, 16, bits, torch.float16, cuda_device)
+    pkg.ops.kv_cache_write(k, v, torch.arange(128, device=cuda_device), thresholds=th, **c)
+    q = (2 * sign).expand(new, 1, 64).half().contiguous().to(cuda_device)
+    table = torch.arange(8, dtype=torch.int32, device=cuda_device)[None]
+    got = pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, torch.tensor([L], dtype=torch.int32, device=cuda_device), None, new, **_pages_args(c))
+    j = torch.arange(L)
+    rows = torch.stack([j // 16, j % 16], 1).to(cuda_device)
+    (kk, _), (vv, ev) = ((a[:, 0], b[:, 0]) for a, b in (_cached(pkg, c, n, rows) for n in "kv"))
+    scale = c["v_stats"][:, 0, :, 1].reshape(-1)[:L].double()
+    for i in range(new):
+        seen = (j <= L - new + i).to(cuda_device)
+        w = torch.softmax((0.125 * q[i, 0].double() @ kk.t()).masked_fill(~seen, -INF), -1)
+        assert float(w[at]) < 1e-20
+        want = w @ vv
+        off = w @ ev + (2.0 ** -11 + 2.0 ** -12 + L * 2.0 ** -23) * (w @ vv.abs())
+        off = off + L * 2.0 ** -18 * (w * scale).max() * c["codebooks"][1].abs().max() + U[torch.float16] * want.abs() + 2.0 ** -25
+        err = (got[i, 0].double() - want).abs()
+        assert bool((err <= 1.05 * off).all()), (i, float((err / off).max()))

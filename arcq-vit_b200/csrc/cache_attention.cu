@@ -306,6 +306,8 @@ template <int BITS, typename E, int STREAMS> int launch_tile(arcq::AttendParams&
 
 template <int BITS, typename E> int launch_attention(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   if (split_is_ahead<BITS>(p)) return launch_split<BITS, E>(p, workspace_bytes, st);
+  // no blocks for rows that q has not got (the split kernel's grid goes by the steps, its workspace by what the caller said)
+  if (p.starts != nullptr && p.max_new > p.q_rows) p.max_new = static_cast<int>(p.q_rows);
   if constexpr (BITS == 16)
     if (static_cast<long long>(p.max_new) * p.group <= arcq::kTileRows && one_stream_is_ahead(p)) return launch_tile<BITS, E, 1>(p, st);
   return launch_tile<BITS, E, 2>(p, st);
@@ -331,6 +333,8 @@ int check_query(const void* q, int dtype, const void* out, int64_t heads, int64_
   if (!aligned(q, 16) || !aligned(out, 16)) return fail(ARCQ_E_ALIGN, "queries and out must be 16-byte aligned");
   return ARCQ_OK;
 }
+// Rows of a key head, and those of its last block, are counted in 32 bits.
+bool too_many_rows(int64_t max_new, int64_t group) { return max_new * group > 0x7fffffffLL - 256; }
 bool strides_ok(const int64_t* s, int n) {
   for (int i = 0; i < n; ++i)
     if (s[i] % 8 != 0) return false;
@@ -421,6 +425,7 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
   if (batch == 0 || q_rows == 0 || max_new == 0) return ARCQ_OK;
   if (lengths == nullptr || (page_table == nullptr && table_width > 0) || q_strides == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (const int rc = check_query(q, q_dtype, out, heads, cache->heads, scale)) return rc;
+  if (too_many_rows(max_new, heads / cache->heads)) return fail(ARCQ_E_TOO_LARGE, "%lld new tokens a sequence are too many", (long long)max_new);
   const int64_t q_sizes[] = {q_rows, heads};
   if (overlaps(out, q_rows * heads * 128, q, 2, q_sizes, q_strides)) return fail(ARCQ_E_BAD_ARG, "out lies over the queries");
   if (cache->bits == 16 && q_dtype != cache->dtype) return fail(ARCQ_E_BAD_ARG, "queries must have the type of the pages");
@@ -469,6 +474,7 @@ int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype,
   if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || (states > 0 && (k == nullptr || v == nullptr)))
     return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (const int rc = check_query(q, dtype, out, heads, kv_heads, scale)) return rc;
+  if (too_many_rows(queries, heads / kv_heads)) return fail(ARCQ_E_TOO_LARGE, "%lld queries a sequence are too many", (long long)queries);
   const int64_t q_sizes[] = {batch, queries, heads}, kv_sizes[] = {batch, states, kv_heads}, bytes = batch * queries * heads * 128;
   if (overlaps(out, bytes, q, 3, q_sizes, q_strides) || overlaps(out, bytes, k, 3, kv_sizes, k_strides) || overlaps(out, bytes, v, 3, kv_sizes, v_strides))
     return fail(ARCQ_E_BAD_ARG, "out lies over the queries, keys or values");

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
     tile = p.tiles - 1 - unit / p.kv_heads % p.tiles;
   }
   const AttendSequence seq = attend_sequence(p, b);
-  const int all_rows = seq.queries * p.group;
+  const int all_rows = seq.queries * p.group;                                     // the host sees to it that rows, and those of the last block, fit
   const bool halves = STREAMS == 1 || all_rows > kTileRows;                       // the streams are halves of the rows; or there is one
   const int row0 = tile * kBlockRows, rows = min(all_rows - row0, kBlockRows);
   // Tiles of rows that are not there: the whole cluster leaves.

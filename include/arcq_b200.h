@@ -433,7 +433,8 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
  * Attention of the newest tokens of each sequence over its cached keys and values (the new tokens' own among them):
  *   q     [q_rows, heads, 64] fp16 or bf16 (the pages' type in 16 bits), strides of a token and a head in values, multiples of 8;
  *         the queries of sequence b are rows starts[b] .. starts[b+1] - 1 (starts int32 [batch + 1]), or, with starts NULL, max_new rows
- *         each (q_rows = batch * max_new).  max_new bounds the queries of a sequence; what is beyond is left out.
+ *         each (q_rows = batch * max_new).  max_new bounds the queries of a sequence; what is beyond is left out.  max_new * heads / cache.heads is
+ *         2^31 - 257 at most.
  *   page_table int32 [batch, table_width]: page of tokens 0 .. page_size - 1 of the sequence, and so on.  Keys on a page that does
  *         not exist (negative, or not below cache.pages) are not seen.
  *   lengths int32 [batch]: tokens of the sequence in the cache, at most table_width * page_size

@@ -333,6 +333,8 @@ int check_query(const void* q, int dtype, const void* out, int64_t heads, int64_
   if (!aligned(q, 16) || !aligned(out, 16)) return fail(ARCQ_E_ALIGN, "queries and out must be 16-byte aligned");
   return ARCQ_OK;
 }
+// Keys are counted in 32 bits, rounded up to whole tiles.
+constexpr long long kMostKeys = 0x7fffffffLL - (arcq::kTileKeys - 1);
 // Rows of a key head, and those of its last block, are counted in 32 bits.
 bool too_many_rows(int64_t max_new, int64_t group) { return max_new * group > 0x7fffffffLL - 256; }
 bool strides_ok(const int64_t* s, int n) {
@@ -421,7 +423,7 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
   if (batch < 0 || table_width < 0 || max_new < 0 || q_rows < 0 || q_rows > 0x7fffffffLL || batch > 0x7fffffffLL || max_new > 0x7fffffffLL)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld table=%lld new=%lld rows=%lld", (long long)batch, (long long)table_width, (long long)max_new, (long long)q_rows);
   if (starts == nullptr && batch * max_new != q_rows) return fail(ARCQ_E_BAD_SHAPE, "%lld queries for %lld sequences of %lld", (long long)q_rows, (long long)batch, (long long)max_new);
-  if (table_width > 0x7fffffffLL || table_width * cache->page_size > 0x7fffffffLL - 64) return fail(ARCQ_E_TOO_LARGE, "contexts of more than 2^31 tokens");
+  if (table_width > 0x7fffffffLL || table_width * cache->page_size > kMostKeys) return fail(ARCQ_E_TOO_LARGE, "contexts of more than 2^31 tokens");
   if (batch == 0 || q_rows == 0 || max_new == 0) return ARCQ_OK;
   if (lengths == nullptr || (page_table == nullptr && table_width > 0) || q_strides == nullptr) return fail(ARCQ_E_BAD_ARG, "null pointer argument");
   if (const int rc = check_query(q, q_dtype, out, heads, cache->heads, scale)) return rc;
@@ -468,7 +470,7 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,
                          const uint8_t* mask, int64_t mask_stride, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || queries > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > 0x7fffffffLL - 64)
+  if (batch < 0 || queries < 0 || states < 0 || batch > 0x7fffffffLL || queries > 0x7fffffffLL || batch * queries > 0x7fffffffLL || states > kMostKeys)
     return fail(ARCQ_E_BAD_SHAPE, "bad shape: batch=%lld queries=%lld states=%lld", (long long)batch, (long long)queries, (long long)states);
   if (batch == 0 || queries == 0) return ARCQ_OK;
   if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || (states > 0 && (k == nullptr || v == nullptr)))

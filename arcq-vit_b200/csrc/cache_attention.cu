@@ -354,6 +354,18 @@ bool overlaps(const void* out, int64_t bytes, const void* t, int n, const int64_
   return a < b + 2 * (hi + 1) && b + 2 * lo < a + bytes;
 }
 
+// Whether `out`, `bytes` long, lies over any of the `size` bytes at t.
+bool lies_over(const void* out, int64_t bytes, const void* t, __int128 size) {
+  const __int128 a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(t);
+  return t != nullptr && a < b + size && b < a + bytes;
+}
+bool over_cache(const void* out, int64_t bytes, const arcq_kv_cache* c) {
+  const __int128 rows = static_cast<__int128>(c->pages) * c->heads * c->page_size, row = c->bits == 16 ? 128 : 8 * c->bits;
+  if (lies_over(out, bytes, c->k_pages, rows * row) || lies_over(out, bytes, c->v_pages, rows * row)) return true;
+  return c->bits != 16 && (lies_over(out, bytes, c->k_stats, rows * 4) || lies_over(out, bytes, c->v_stats, rows * 4) ||
+                           lies_over(out, bytes, c->codebooks, 8ll << c->bits));
+}
+
 }  // namespace
 
 extern "C" {
@@ -430,6 +442,10 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
   if (too_many_rows(max_new, heads / cache->heads)) return fail(ARCQ_E_TOO_LARGE, "%lld new tokens a sequence are too many", (long long)max_new);
   const int64_t q_sizes[] = {q_rows, heads};
   if (overlaps(out, q_rows * heads * 128, q, 2, q_sizes, q_strides)) return fail(ARCQ_E_BAD_ARG, "out lies over the queries");
+  if (over_cache(out, q_rows * heads * 128, cache)) return fail(ARCQ_E_BAD_ARG, "out lies over the cache");
+  if (lies_over(out, q_rows * heads * 128, page_table, 4 * batch * table_width) || lies_over(out, q_rows * heads * 128, lengths, 4 * batch) ||
+      lies_over(out, q_rows * heads * 128, starts, 4 * (batch + 1)))
+    return fail(ARCQ_E_BAD_ARG, "out lies over the page table, the lengths or the starts");
   if (cache->bits == 16 && q_dtype != cache->dtype) return fail(ARCQ_E_BAD_ARG, "queries must have the type of the pages");
   if (!strides_ok(q_strides, 2)) return fail(ARCQ_E_ALIGN, "strides of the queries must be multiples of 8 values");
   arcq::AttendParams p = {};
@@ -480,6 +496,8 @@ int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype,
   const int64_t q_sizes[] = {batch, queries, heads}, kv_sizes[] = {batch, states, kv_heads}, bytes = batch * queries * heads * 128;
   if (overlaps(out, bytes, q, 3, q_sizes, q_strides) || overlaps(out, bytes, k, 3, kv_sizes, k_strides) || overlaps(out, bytes, v, 3, kv_sizes, v_strides))
     return fail(ARCQ_E_BAD_ARG, "out lies over the queries, keys or values");
+  if (lies_over(out, bytes, lengths, 4 * batch) || (mask_stride >= 0 && lies_over(out, bytes, mask, static_cast<__int128>(batch - 1) * mask_stride + states)))
+    return fail(ARCQ_E_BAD_ARG, "out lies over the lengths or the mask");
   if (lengths != nullptr && mask != nullptr) return fail(ARCQ_E_BAD_ARG, "lengths or a mask, not both");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(ARCQ_E_ALIGN, "keys and values must be 16-byte aligned");
   if (!strides_ok(q_strides, 3) || !strides_ok(k_strides, 3) || !strides_ok(v_strides, 3)) return fail(ARCQ_E_ALIGN, "strides must be multiples of 8 values");

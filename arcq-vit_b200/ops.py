@@ -453,7 +453,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     are.  All three stay on the device: a captured call takes new lengths on every replay.  Causal: the last token of a sequence sees all of
     it, the one before one less.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
 
-    Returns [tokens, heads, 64] (``out`` where given, which does not lie over ``q``): zeros for a token that sees nothing.  Rows of no sequence are
+    Returns [tokens, heads, 64] (``out`` where given, which lies over none of the inputs): zeros for a token that sees nothing.  Rows of no sequence are
     not written."""
     got = _cabi.host().paged_attention(q, page_table, lengths, starts, max_new, causal, scale, out, k_pages, v_pages, k_stats, v_stats, codebooks)
     if got is not None:
@@ -486,7 +486,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths=N
     bf16 (views of a projection's output are read where they are).  ``lengths`` int32 [batch]: the first of the states are seen; or ``mask`` bool
     [batch, states]: those that are True; or neither.  ``scale`` is 1/8 by default.  Heads share key heads in equal groups.
 
-    Returns [batch, queries, heads, 64] (``out`` where given, which does not lie over the others): zeros where nothing is seen."""
+    Returns [batch, queries, heads, 64] (``out`` where given, which lies over none of the inputs): zeros where nothing is seen."""
     got = _cabi.host().cross_attention(q, k, v, lengths, mask, scale, out)
     if got is not None:
         return got

@@ -439,7 +439,7 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
  *         not exist (negative, or not below cache.pages) are not seen.
  *   lengths int32 [batch]: tokens of the sequence in the cache, at most table_width * page_size
  *   causal 1: query i of n sees the first lengths[b] - n + i + 1 tokens; 0: all of them
- *   out   [q_rows, heads, 64] of q's type, not over q: softmax(scale q k^T) v, zeros for a query that sees nothing; rows of no sequence stay as they are.
+ *   out   [q_rows, heads, 64] of q's type, over none of the inputs: softmax(scale q k^T) v, zeros for a query that sees nothing; rows of no sequence stay as they are.
  * heads is a multiple of cache.heads: query head h reads key head h / (heads / cache.heads).  Packed keys and values are rebuilt in
  * fp16, one half-precision fma each, so |center| + 3 scale has to stay within fp16's range; products accumulate in fp32, probabilities are rounded
  * to 16 bits for the second one.  In calls with few queries a level is rounded to fp16 up or down instead, in turn over the keys, and center and
@@ -455,7 +455,7 @@ int arcq_paged_attention(const arcq_kv_cache* cache, const void* q, int q_dtype,
 /*
  * Attention of queries [batch, queries, heads, 64] to an encoder's states, keys and values [batch, states, kv_heads, 64], all fp16 or all
  * bf16; strides of a sequence, a token and a head in values, multiples of 8.  lengths int32 [batch] (the first of the states are seen)
- * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64], not over q, k or v, a workspace for max_new = queries; otherwise as above.
+ * or mask [batch, states] bytes (0: not seen; rows mask_stride apart), or neither.  out [batch, queries, heads, 64], over none of the inputs, a workspace for max_new = queries; otherwise as above.
  */
 int arcq_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t queries, int64_t states, int64_t heads,
                          int64_t kv_heads, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* lengths,

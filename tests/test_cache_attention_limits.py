@@ -20,3 +20,21 @@ def test_keys_that_pass_32_bits_in_whole_tiles(lib, pkg):  # noqa: F811
         assert _paged(lib, _cache(pkg, page_size=page), width=width) == TOO_LARGE, (page, width)
     for states in (2 ** 31 - 127, 2 ** 31 - 65, 2 ** 31 - 1):
         assert _cross(lib, states=states, ks=(0, 0, 64), vs=(0, 0, 64)) == BAD_SHAPE, states
+
+
+def test_outputs_over_the_cache_or_the_tables_are_refused(lib, pkg):  # noqa: F811
+    at = 1 << 24
+    size = 4 * 2 * 16                                                    # rows of the cache
+    ends = dict(k_pages=32 * size, v_pages=32 * size, k_stats=4 * size, v_stats=4 * size, codebooks=4 * 2 * 16)
+    for name, size_of in ends.items():
+        for out in (at, at + size_of - 16, at - 2 * 4 * 128 + 16):
+            assert _paged(lib, _cache(pkg, **{name: at}), out=out) == BAD_ARG and b"over the cache" in lib.arcq_last_error_string(), (name, out - at)
+    for name in ("k_pages", "v_pages"):
+        for out in (at, at + 128 * size - 16):
+            assert _paged(lib, _cache(pkg, bits=16, dtype=1, **{name: at}), out=out) == BAD_ARG and b"over the cache" in lib.arcq_last_error_string()
+    for name in ("table", "lengths", "starts"):
+        assert _paged(lib, _cache(pkg), **{name: at}, out=at) == BAD_ARG and b"out lies over the page table" in lib.arcq_last_error_string()
+    for name in ("lengths", "mask"):
+        assert _cross(lib, **{name: at + 4}, out=at) == BAD_ARG and b"out lies over the lengths" in lib.arcq_last_error_string()
+    # a cache of more bytes than 64 bits count
+    assert _paged(lib, _cache(pkg, pages=MANY, heads=65535, page_size=1 << 20), heads=65535, out=1 << 40, qs=(65535 * 64, 64)) == BAD_ARG

@@ -33,3 +33,38 @@ def test_a_bound_far_above_the_new_tokens(pkg, cuda_device, bits):
     with pytest.raises(RuntimeError, match="too many"):
         run([0, 200], 2 ** 30 - 128, 1)
     assert pkg.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("heads", [1, 20])                           # 4 and 80 rows a key head: both kernels
+@pytest.mark.parametrize("starts,valid,zero", [
+    # rows of a sequence that are as a call with it alone gives them (sequence, from, to), rows that are zero; the rest is not written
+    ([0, 2, 4], [(0, 0, 2), (1, 2, 4)], []),
+    ([0, 2, 10 ** 9], [(0, 0, 2)], [2, 3]),                          # the first 2 of a thousand million: they come before the context's 20 keys
+    ([3, 2, 4], [(1, 2, 4)], []),                                    # backwards: no queries
+    ([-5, 1, 2], [(1, 1, 2)], []),                                   # before the first row: no queries
+    ([-2 ** 31, 2 ** 31 - 1, 2], [], []),
+    ([2 ** 31 - 1, 4, 4], [], []),
+    ([4, 9, 9], [], []),                                             # behind the last row
+    ([1, 1, 4], [(1, 1, 4)], []),
+    ([2, 4, 0], [(0, 2, 4)], [])])
+def test_starts_that_are_not_in_order(pkg, cuda_device, bits, heads, starts, valid, zero):
+    gen = torch.Generator().manual_seed(4)
+    c = _filled(pkg, gen, 4, 1, 16, bits, torch.float16, cuda_device)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    table, lengths = torch.arange(4, **i32).reshape(2, 2), torch.tensor([20, 31], **i32)
+    q = torch.randn(4, heads, 64, generator=gen).half().to(cuda_device)
+    guarded = torch.full((4 + 64, heads, 64), 5.0, device=cuda_device).half()          # rows around out
+    out = guarded[32:36]
+    pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, lengths, torch.tensor(starts, **i32), 4, out=out, **_args(c))
+    want = torch.full_like(guarded, 5.0)
+    for b, lo, hi in valid:
+        want[32 + lo:32 + hi] = pkg.ops.paged_attention(q[lo:hi], c["k_pages"], c["v_pages"], table[b:b + 1], lengths[b:b + 1], None, hi - lo, **_args(c))
+    for row in zero:
+        want[32 + row] = 0
+    # keys may be split otherwise: two roundings of weights and outputs below 4; what is not written or zero is so exactly
+    off = torch.zeros(4 + 64, 1, 1, device=cuda_device)
+    for _, lo, hi in valid:
+        off[32 + lo:32 + hi] = 4 * 4 * 2.0 ** -11
+    assert bool(((guarded.float() - want.float()).abs() <= off).all())
+    assert pkg.ops.device_status() == 0

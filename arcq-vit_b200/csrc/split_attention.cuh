@@ -134,7 +134,7 @@ __device__ __forceinline__ float bf16_top(const uint32_t* w, int n) {
 }
 __device__ __forceinline__ float bf16_to_half(uint32_t* w, int n, float top) {
   const int e = (__float_as_int(top) >> 23) - 127;
-  const int up = top > 0.0f && e < 128 ? min(max(13 - e, -100), 100) : 0;
+  const int up = top > 0.0f && e < 128 ? min(13 - e, 126) : 0;                     // -114 at least; f and the factor are normal numbers
   const float f = __int_as_float((up + 127) << 23);
 #pragma unroll
   for (int j = 0; j < n; ++j) w[j] = pair_to_sixteen<__half>(mul2(sixteen_to_pair<__nv_bfloat16>(w[j]), pack2(f, f)));

@@ -166,3 +166,22 @@ def test_a_large_value_that_hardly_counts_costs_the_others_nothing(pkg, cuda_dev
         off = off + L * 2.0 ** -18 * (w * scale).max() * c["codebooks"][1].abs().max() + U[torch.float16] * want.abs() + 2.0 ** -25
         err = (got[i, 0].double() - want).abs()
         assert bool((err <= 1.05 * off).all()), (i, float((err / off).max()))
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_queries_of_bf16_at_the_ends_of_their_range(pkg, cuda_device, new):
+    """Over packed keys a row of queries is scaled into fp16's range by a power of two; 2^120 needs more than 2^-100, and 2^-100 more than 2^100."""
+    gen = torch.Generator().manual_seed(1)
+    c, th = _empty_cache(8, 2, 32, 4, torch.bfloat16, cuda_device)
+    x = [torch.randn(256, 2, 64, generator=gen).bfloat16().to(cuda_device) for _ in range(2)]
+    pkg.ops.kv_cache_write(x[0], x[1], torch.arange(256, device=cuda_device), thresholds=th, **c)
+    table = torch.arange(8, dtype=torch.int32, device=cuda_device)[None]
+    length = torch.tensor([250], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(new, 4, 64, generator=gen).bfloat16().to(cuda_device)
+
+    def run(e):
+        return pkg.ops.paged_attention(q * 2.0 ** e, c["k_pages"], c["v_pages"], table, length, None, new, scale=0.125 * 2.0 ** -e, **_pages_args(c))
+    want = run(0)
+    assert bool(torch.isfinite(want).all())
+    for e in (-100, 100, 120):
+        assert torch.equal(run(e), want), e

@@ -303,7 +303,7 @@ const at::Tensor* plain_tensor(PyObject* o, at::ScalarType t, const c10::Device&
 bool read_kv_cache(PyObject* const* args, arcq_kv_cache* c) {
   const at::Tensor *k = tensor_of(args[0]), *v = tensor_of(args[1]);
   if (k == nullptr || v == nullptr || !k->is_cuda() || k->dim() != 4 || !k->is_contiguous() || !v->is_contiguous() || v->sizes() != k->sizes() ||
-      v->scalar_type() != k->scalar_type() || v->device() != k->device())
+      v->scalar_type() != k->scalar_type() || v->device() != k->device() || wants_gradient({k, v}))
     return false;
   c->pages = k->size(0);
   c->heads = k->size(1);
@@ -323,7 +323,8 @@ bool read_kv_cache(PyObject* const* args, arcq_kv_cache* c) {
   c->bits = static_cast<int>(row / 8);
   const at::Tensor *ks = plain_tensor(args[2], at::kHalf, k->device()), *vs = plain_tensor(args[3], at::kHalf, k->device()),
                    *cb = plain_tensor(args[4], at::kFloat, k->device());
-  if (ks == nullptr || vs == nullptr || cb == nullptr || cb->dim() != 2 || cb->size(0) != 2 || cb->size(1) != 1 << c->bits) return false;
+  if (ks == nullptr || vs == nullptr || cb == nullptr || cb->dim() != 2 || cb->size(0) != 2 || cb->size(1) != 1 << c->bits || wants_gradient({ks, vs, cb}))
+    return false;
   for (const at::Tensor* t : {ks, vs})
     if (t->dim() != 4 || t->size(0) != c->pages || t->size(1) != c->heads || t->size(2) != c->page_size || t->size(3) != 2) return false;
   c->k_stats = ks->mutable_data_ptr();
@@ -339,7 +340,7 @@ const at::Tensor* slots_tensor(PyObject* o, const c10::Device& dev) {
 bool read_out(PyObject* o, const at::Tensor& q, at::Tensor* out) {
   if (o == Py_None) return true;
   const at::Tensor* t = plain_tensor(o, q.scalar_type(), q.device());
-  if (t == nullptr || t->sizes() != q.sizes() || !aligned16(t->const_data_ptr())) return false;
+  if (t == nullptr || t->sizes() != q.sizes() || !aligned16(t->const_data_ptr()) || wants_gradient({t})) return false;
   *out = *t;
   return true;
 }
@@ -367,7 +368,7 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* th = nullptr;
   if (c.bits != 16) {
     th = plain_tensor(args[3], at::kFloat, dev);
-    if (th == nullptr || th->dim() != 2 || th->size(0) != 2 || th->size(1) != (1 << c.bits) - 1) Py_RETURN_NONE;
+    if (th == nullptr || th->dim() != 2 || th->size(0) != 2 || th->size(1) != (1 << c.bits) - 1 || wants_gradient({th})) Py_RETURN_NONE;
   }
   without_gil([&] {
     const c10::cuda::CUDAGuard guard(dev);

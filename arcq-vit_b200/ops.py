@@ -296,7 +296,7 @@ def attention(qkv: torch.Tensor, batch: int, tokens: int, heads: int, thresholds
 
 # ---------------------------------------------------------------- key/value cache, attention over it and to an encoder's states
 def _no_gradient(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or with detached tensors")
 
 
@@ -340,6 +340,7 @@ def _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks, device=None):
     """The C view of a cache, and the tensors that it holds besides the pages."""
     if not isinstance(k_pages, torch.Tensor) or not k_pages.is_cuda or k_pages.dim() != 4:
         raise RuntimeError("k_pages must be a CUDA tensor [pages, heads, page_size, row]")
+    _no_gradient(k_pages, v_pages, k_stats, v_stats, codebooks)
     device = k_pages.device if device is None else device
     pages, heads, size, row = k_pages.shape
     c = _cabi.KvCache(pages=pages, heads=heads, page_size=size)
@@ -385,7 +386,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_page
     lib = _cabi.load()
     k = _heads_of_64(k, "k", 3, None, tuple(_DT))
     v = _heads_of_64(v, "v", 3, k.device, (k.dtype,))
-    _no_gradient(k, v)
+    _no_gradient(k, v, thresholds)
     c, _held = _kv_cache(k_pages, v_pages, k_stats, v_stats, codebooks, k.device)
     if v.shape != k.shape or k.shape[1] != c.heads:
         raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match a cache of {c.heads} heads")
@@ -437,6 +438,7 @@ def _workspace(size: int, device) -> torch.Tensor:
 def _attention_out(out, q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _no_gradient(out)
     _plain(out, "out", q.dtype, q.device, q.shape)
     if out.data_ptr() % 16:
         raise RuntimeError("out must be 16-byte aligned")

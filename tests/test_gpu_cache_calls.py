@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_cache_attention import _filled
+from test_gpu_cache_attention import _empty_cache, _filled
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,35 @@ def test_starts_that_are_not_in_order(pkg, cuda_device, bits, heads, starts, val
         off[32 + lo:32 + hi] = 4 * 4 * 2.0 ** -11
     assert bool(((guarded.float() - want.float()).abs() <= off).all())
     assert pkg.ops.device_status() == 0
+
+
+def test_what_asks_for_gradients_is_refused(pkg, cuda_device):
+    """The cache's own tensors and out, like queries, keys and values: there is no backward pass, and none is left out in silence."""
+    dev, ops = cuda_device, pkg.ops
+    i32 = dict(dtype=torch.int32, device=dev)
+    table, lengths, slots = torch.zeros(2, 2, **i32), torch.ones(2, **i32), torch.arange(3, device=dev)
+    q, k = torch.randn(2, 4, 64, device=dev).half(), torch.randn(3, 2, 64, device=dev).half()
+
+    def calls(c, th, out=None):
+        args = _args(c)
+        return [lambda: ops.paged_attention(q, c["k_pages"], c["v_pages"], table, lengths, out=out, **args),
+                lambda: ops.kv_cache_write(k, k, slots, thresholds=th, **c), lambda: ops.kv_cache_read(slots, **c)]
+    for bits, names in ((16, ["k_pages", "v_pages"]), (4, ["k_stats", "v_stats", "codebooks"])):
+        c, th = _empty_cache(4, 2, 16, bits, torch.float16, dev)
+        for name in names:
+            asks = {**c, name: c[name].clone().requires_grad_()}
+            for f in calls(asks, th):
+                with pytest.raises(RuntimeError, match="backward"):
+                    f()
+            with torch.no_grad():
+                for f in calls(asks, th):
+                    f()
+    with pytest.raises(RuntimeError, match="backward"):
+        calls(c, th.clone().requires_grad_())[1]()
+    with pytest.raises(RuntimeError, match="backward"):
+        calls(c, th, torch.empty_like(q).requires_grad_())[0]()
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.cross_attention(q[None], k[None], k[None], out=torch.empty_like(q[None]).requires_grad_())
+    for f in calls(c, th, torch.empty_like(q)):
+        f()
+    assert ops.device_status() == 0

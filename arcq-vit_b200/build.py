@@ -70,11 +70,13 @@ def _host_command():
 
 
 def _compile(unit: Path, force: bool, verbose: bool) -> Path:
-    """The unit's object, compiled anew where a file that went into it (nvcc's list beside it) is newer."""
+    """The unit's object, compiled anew where a file that went into it (nvcc's list beside it) is newer, or where the list is of another
+    place: objects of a tree that was copied say nothing about the copy's files."""
     obj, used = unit.with_suffix(".o"), unit.with_suffix(".d")
     names = used.read_text().replace("\\\n", " ").split(":", 1)[-1].split() if used.exists() else []
     files = [Path(n) for n in names]
-    if force or not files or not all(f.exists() for f in files) or _older(obj, files):
+    here = all(f.exists() for f in files) and any(f.samefile(unit) for f in files)
+    if force or not here or _older(obj, files):
         _run([_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-c", "-MD", "-MF", str(used), "-o", str(obj), str(unit)], verbose)
     return obj
 

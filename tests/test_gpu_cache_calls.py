@@ -100,3 +100,52 @@ def test_what_asks_for_gradients_is_refused(pkg, cuda_device):
     for f in calls(c, th, torch.empty_like(q)):
         f()
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [2, 4])
+@pytest.mark.parametrize("tokens", [40, 1500])                       # both write kernels
+@pytest.mark.parametrize("new", [1, 100])                            # both attentions
+def test_codebooks_that_have_just_been_written(pkg, cuda_device, bits, tokens, new):
+    """Fitted right before the first write, one kernel between: eagerly and captured, with other levels each time, behind other work."""
+    gen = torch.Generator().manual_seed(bits + tokens)
+    pages = -(-tokens // 16)
+    c, th = _empty_cache(pages, 2, 16, bits, torch.float16, cuda_device)
+    base_cb, base_th = c["codebooks"].clone(), th.clone()
+    k, v = (torch.randn(tokens, 2, 64, generator=gen).half().to(cuda_device) for _ in range(2))
+    q = torch.randn(new, 4, 64, generator=gen).half().to(cuda_device)
+    slots = torch.arange(tokens, device=cuda_device)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda_device)[None]
+    length = torch.tensor([tokens], dtype=torch.int32, device=cuda_device)
+    factor, other = torch.ones((), device=cuda_device), torch.zeros(1 << 22, device=cuda_device)
+
+    def fit_and_use():
+        other.add_(1.0)
+        th.copy_(base_th * factor)
+        c["codebooks"].copy_(base_cb * factor)
+        other[:4].add_(1.0)                                            # the kernel between
+        pkg.ops.kv_cache_write(k, v, slots, thresholds=th, **c)
+        read = pkg.ops.kv_cache_read(slots, **c)
+        y = pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, length, None, new, **_args(c))
+        return (*read, y)
+
+    def one_by_one(f):
+        c2, _ = _empty_cache(pages, 2, 16, bits, torch.float16, cuda_device)
+        c2["codebooks"], th2 = base_cb * f, base_th * f
+        torch.cuda.synchronize()
+        pkg.ops.kv_cache_write(k, v, slots, thresholds=th2, **c2)
+        read = pkg.ops.kv_cache_read(slots, **c2)
+        return (*read, pkg.ops.paged_attention(q, c2["k_pages"], c2["v_pages"], table, length, None, new, **_args(c2)))
+    factors = [1.0, 0.5, 1.5, 0.75] * 3
+    want = {f: one_by_one(f) for f in set(factors)}
+    assert not torch.equal(want[0.5][0], want[1.5][0])
+    for f in factors:
+        factor.fill_(f)
+        assert all(torch.equal(a, b) for a, b in zip(fit_and_use(), want[f])), f
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = fit_and_use()
+    for f in factors:
+        factor.fill_(f)
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[f])), f
+    assert pkg.ops.device_status() == 0

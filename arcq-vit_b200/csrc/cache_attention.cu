@@ -204,7 +204,6 @@ template <int BITS> bool split_is_ahead(const arcq::AttendParams& p) {
 
 template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t workspace_bytes, cudaStream_t st) {
   auto k = arcq::split_attention_kernel<BITS, E>;
-  auto join = arcq::join_attention_kernel<arcq::SplitUnits<arcq::SplitStep<BITS>::kKeys>>;
   constexpr size_t smem = arcq::split_parts<BITS>() + arcq::kSplitSharedParts + 128;
   static_assert(smem + arcq::kSplitBase <= 227 * 1024, "");
   static thread_local int done_dev = -1;
@@ -230,7 +229,7 @@ template <int BITS, typename E> int launch_split(arcq::AttendParams& p, int64_t 
   const SplitTimes times = split_times<BITS>(p);
   p.whole_units = p.max_keys > kWholeUnitKeys ? 0 : times.whole < times.cut ? 2 : 1;
   cudaError_t e = launch(k, dim3(static_cast<unsigned>(steps < sms ? steps : sms)), arcq::kSplitThreads, smem, 1, st, p);
-  if (e == cudaSuccess && !p.whole_units) e = launch(join, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
+  if (e == cudaSuccess && !p.whole_units) e = launch(arcq::join_attention_kernel, dim3(static_cast<unsigned>(units)), arcq::kJoinThreads, 0, 1, st, p);
   return e == cudaSuccess ? ARCQ_OK : arcq_host::cuda_fail(e, "attention launch");
 }
 

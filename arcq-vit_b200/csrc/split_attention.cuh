@@ -244,45 +244,44 @@ template <int BITS, int I> __device__ __forceinline__ uint32_t table_address(uin
 }
 
 // ---------------------------------------------------------------- units and their line
-// U: how many rows a unit has and how many steps it takes
-template <int KEYS> struct SplitUnits {
-  static constexpr int kRows = kSplitRows;
-  static __device__ __forceinline__ int steps(int, int keys) { return max((keys + KEYS - 1) / KEYS, 1); }      // without keys a step, in which nothing is seen
-};
+// KEYS: of a step
 struct SplitUnit {
   int b, kvh, tile;
   AttendSequence seq;
   int rows, keys, steps;
 };
-template <typename U> __device__ __forceinline__ int split_tiles(const AttendParams& p, const AttendSequence& s) {
-  return static_cast<int>((static_cast<long long>(s.queries) * p.group + U::kRows - 1) / U::kRows);
+__device__ __forceinline__ int split_tiles(const AttendParams& p, const AttendSequence& s) {
+  return static_cast<int>((static_cast<long long>(s.queries) * p.group + kSplitRows - 1) / kSplitRows);
 }
-template <typename U> __device__ __forceinline__ void split_tile(const AttendParams& p, SplitUnit& u) {
-  u.rows = static_cast<int>(min(static_cast<long long>(u.seq.queries) * p.group - static_cast<long long>(u.tile) * U::kRows, static_cast<long long>(U::kRows)));
+__device__ __forceinline__ int split_rows(const AttendParams& p, const AttendSequence& s, int tile) {
+  return static_cast<int>(min(static_cast<long long>(s.queries) * p.group - static_cast<long long>(tile) * kSplitRows, static_cast<long long>(kSplitRows)));
+}
+template <int KEYS> __device__ __forceinline__ void split_tile(const AttendParams& p, SplitUnit& u) {
+  u.rows = split_rows(p, u.seq, u.tile);
   u.keys = u.seq.keys;
-  if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * U::kRows + u.rows - 1) / p.group + 1, 0));
-  u.steps = U::steps(u.rows, u.keys);
+  if (p.causal) u.keys = min(u.keys, max(u.seq.keys - u.seq.all_queries + (u.tile * kSplitRows + u.rows - 1) / p.group + 1, 0));
+  u.steps = max((u.keys + KEYS - 1) / KEYS, 1);                                    // without keys a step, in which nothing is seen
 }
 // steps of all units of a sequence and key head
-template <typename U> __device__ __forceinline__ int split_head_steps(const AttendParams& p, const AttendSequence& seq) {
+template <int KEYS> __device__ __forceinline__ int split_head_steps(const AttendParams& p, const AttendSequence& seq) {
   SplitUnit u;
   u.seq = seq;
-  const int tiles = split_tiles<U>(p, u.seq);
+  const int tiles = split_tiles(p, u.seq);
   int n = 0;
   for (u.tile = 0; u.tile < tiles; ++u.tile) {
-    split_tile<U>(p, u);
+    split_tile<KEYS>(p, u);
     n += u.steps;
   }
   return n;
 }
 // The unit after (b, kvh, tile); behind the last one: b = batch.  What a kernel keeps of a unit while it works on it is little.
-template <typename U> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
+template <int KEYS> __device__ __forceinline__ SplitUnit split_next(const AttendParams& p, int b, int kvh, int tile) {
   SplitUnit u;
   u.b = b;
   u.kvh = kvh;
   u.tile = tile + 1;
   u.seq = attend_sequence(p, b);
-  if (u.tile >= split_tiles<U>(p, u.seq)) {
+  if (u.tile >= split_tiles(p, u.seq)) {
     u.tile = 0;
     if (++u.kvh == p.kv_heads) {
       u.kvh = 0;
@@ -293,27 +292,27 @@ template <typename U> __device__ __forceinline__ SplitUnit split_next(const Atte
       if (u.b >= p.batch) return u;
     }
   }
-  split_tile<U>(p, u);
+  split_tile<KEYS>(p, u);
   return u;
 }
 // The line: each of a block's threads has a share of the sequences, `mine` steps, with `before` steps before them.  Where all sequences are alike
 // `mine` is a sequence's.  (The host keeps the line below 2^30 steps.)
-template <typename U, int THREADS> struct SplitLine {
+template <int KEYS> struct SplitLine {
   int share, total, mine, before;
   bool alike;
   // whole block; of_warps: shared memory for a number a warp
   __device__ __forceinline__ SplitLine(const AttendParams& p, int* of_warps) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     alike = p.lengths == nullptr && p.starts == nullptr;
-    share = (p.batch + THREADS - 1) / THREADS;
+    share = (p.batch + kSplitThreads - 1) / kSplitThreads;
     if (alike) {
-      mine = split_head_steps<U>(p, attend_sequence(p, 0)) * p.kv_heads;
+      mine = split_head_steps<KEYS>(p, attend_sequence(p, 0)) * p.kv_heads;
       total = mine * p.batch;
       before = 0;
       return;
     }
     mine = 0;
-    for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_head_steps<U>(p, attend_sequence(p, b)) * p.kv_heads;
+    for (int b = tid * share; b < min((tid + 1) * share, p.batch); ++b) mine += split_head_steps<KEYS>(p, attend_sequence(p, b)) * p.kv_heads;
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -325,7 +324,7 @@ template <typename U, int THREADS> struct SplitLine {
     total = 0;
     before = sum - mine;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
+    for (int w = 0; w < kSplitWarps; ++w) {
       const int n = of_warps[w];
       if (w < warp) before += n;
       total += n;
@@ -353,7 +352,7 @@ template <typename U, int THREADS> struct SplitLine {
       at = found->y;
       for (;; ++u.b) {
         u.seq = attend_sequence(p, u.b);
-        of_head = split_head_steps<U>(p, u.seq);
+        of_head = split_head_steps<KEYS>(p, u.seq);
         if (at + of_head * p.kv_heads > x) break;
         at += of_head * p.kv_heads;
       }
@@ -361,7 +360,7 @@ template <typename U, int THREADS> struct SplitLine {
     u.kvh = (x - at) / max(of_head, 1);
     at += u.kvh * of_head;
     for (u.tile = 0;; ++u.tile) {
-      split_tile<U>(p, u);
+      split_tile<KEYS>(p, u);
       if (at + u.steps > x) break;
       at += u.steps;
     }
@@ -452,8 +451,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   if constexpr (PACKED) fill_split_table<BITS>(p.codebooks, tid, kSplitThreads);
   pdl_wait();
 
-  using Units = SplitUnits<KEYS>;
-  const SplitLine<Units, kSplitThreads> line(p, s_scan);
+  const SplitLine<KEYS> line(p, s_scan);
   // ---- the block's piece of the line, and the warp's
   const int piece = max(static_cast<int>((static_cast<unsigned>(line.total) + gridDim.x - 1) / gridDim.x), 1);
   int from = static_cast<int>(min(static_cast<long long>(blockIdx.x) * piece, static_cast<long long>(line.total))), to = min(piece, line.total - from) + from;
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
   if (p.whole_units == 2) {                                                        // the units that begin in the warp's piece
     if (at < start) {
       at += u.steps;
-      if (at < to) u = split_next<Units>(p, u.b, u.kvh, u.tile);
+      if (at < to) u = split_next<KEYS>(p, u.b, u.kvh, u.tile);
     }
     start = at;
     if (lane == 0) s_ends[warp] = at;
@@ -592,7 +590,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       f_slot = f_slot + 1 == kSplitStages ? 0 : f_slot + 1;
       if (--f_left > 0) {
         if (++f_step == f.steps) {
-          const SplitUnit n = split_next<Units>(p, f.b, f.kvh, f.tile);
+          const SplitUnit n = split_next<KEYS>(p, f.b, f.kvh, f.tile);
           f = {n.b, n.kvh, n.tile, n.keys, n.steps};
           f_step = run = 0;
           look_up(0);
@@ -969,7 +967,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
     }
     at += u.steps;
     if (step < steps) {
-      u = split_next<Units>(p, u.b, u.kvh, u.tile);
+      u = split_next<KEYS>(p, u.b, u.kvh, u.tile);
       load_queries();
     }
   }
@@ -1000,26 +998,23 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
 
 // Adds up the blocks' parts of the units that lie in more than one block's piece: a block a unit, four values of a row a thread.
 constexpr int kJoinThreads = 256;
-template <typename U> __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
+static __global__ void __launch_bounds__(kJoinThreads) join_attention_kernel(const __grid_constant__ AttendParams p) {
   pdl_launch_dependents();
   const long long unit = blockIdx.x;
-  SplitUnit u;
-  u.tile = static_cast<int>(unit % p.tiles);
-  u.kvh = static_cast<int>(unit / p.tiles % p.kv_heads);
-  u.b = static_cast<int>(unit / p.tiles / p.kv_heads);
+  const int tile = static_cast<int>(unit % p.tiles), kvh = static_cast<int>(unit / p.tiles % p.kv_heads), b = static_cast<int>(unit / p.tiles / p.kv_heads);
   pdl_wait();
   const SplitRecord rec = split_records(p)[unit];                                  // not written where there is no such tile
   const int piece = static_cast<SplitHeader*>(p.workspace)->piece;
-  u.seq = attend_sequence(p, u.b);
-  if (u.tile >= split_tiles<U>(p, u.seq) || rec.whole) return;
-  split_tile<U>(p, u);
+  const AttendSequence seq = attend_sequence(p, b);
+  if (tile >= split_tiles(p, seq) || rec.whole) return;
+  const int rows = split_rows(p, seq, tile);
   const int first = rec.start / piece, last = (rec.start + rec.steps - 1) / piece;
-  for (int e = threadIdx.x; e < u.rows * 16; e += kJoinThreads) {
+  for (int e = threadIdx.x; e < rows * 16; e += kJoinThreads) {
     const int row = e >> 4, column = e & 15;
     float top, sum;
     const float4 o = add_parts(last - first + 1, row, column, top, sum,
                                [&](int q) { return split_part(p, 2ll * (first + q) + (rec.start >= (first + q) * piece ? 1 : 0)); });
-    write_four(p, u.seq.first_row, u.kvh, u.tile * U::kRows + row, column, o, inverse_sum(sum));
+    write_four(p, seq.first_row, kvh, tile * kSplitRows + row, column, o, inverse_sum(sum));
   }
 }
 

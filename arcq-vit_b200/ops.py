@@ -377,8 +377,8 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_page
     in fp16 or bf16, or [pages, heads, page_size, 8 * bits] uint8 with bits 2, 3 or 4.  Packed, a head's 64 values are one quantizer
     group: the codes are those of ``quantize_activation``, and ``k_stats`` / ``v_stats`` [pages, heads, page_size, 2] fp16 hold
     (mean - scale * code_sum / 64, scale); a head with a NaN or an infinity in it becomes NaN as a whole.  ``codebooks`` [2, 2^bits] and
-    ``thresholds`` [2, 2^bits - 1], fp32: the keys' and the values'.  Like all that belongs to a layer they are read while the kernel before
-    may still run, here and by the cache's other operators: what has just been fitted needs any other operation between it and the call.
+    ``thresholds`` [2, 2^bits - 1], fp32: the keys' and the values'; they may have been fitted right before the call.
+    (``kv_cache_read`` and ``paged_attention`` read codebooks while the operation before them may still run: change them before a write.)
 
     ``slots`` int64 [tokens]: page * page_size + place in the page.  Tokens with a negative slot, or one beyond the cache, are left out.
     As with ``index_put_``, of tokens with the same slot any may be found there afterwards, or parts of several."""

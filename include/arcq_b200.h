@@ -407,8 +407,8 @@ int arcq_dense_weight_gemm_prefetch(const void* xhat, const void* w16, const flo
  *                range); codebooks fp32 [2, 2^bits], keys' and values'.  A value is stats[0] + stats[1] * codebook[code].  A group with a
  *                NaN or an infinity in it has NaN statistics: all 64 values are NaN.
  * page_size: a power of two, 16 or more.  Buffers contiguous, 16-byte aligned.
- * codebooks and thresholds are a layer's: read early (see "Order on the stream"), by reads of the cache too.  Where they have only just been
- * fitted, the kernel that wrote them may not be the last one before the call.  Pages, statistics and all else are read in order.
+ * arcq_kv_cache_write takes codebooks and thresholds that the kernel just before it has fitted.  Reading the cache and attention over it read
+ * codebooks early (see "Order on the stream"): the kernel just before such a call may be a write, but not what writes the codebooks.
  */
 typedef struct arcq_kv_cache {
   void *k_pages, *v_pages;

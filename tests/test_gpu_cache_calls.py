@@ -105,8 +105,10 @@ def test_what_asks_for_gradients_is_refused(pkg, cuda_device):
 @pytest.mark.parametrize("bits", [2, 4])
 @pytest.mark.parametrize("tokens", [40, 1500])                       # both write kernels
 @pytest.mark.parametrize("new", [1, 100])                            # both attentions
-def test_codebooks_that_have_just_been_written(pkg, cuda_device, bits, tokens, new):
-    """Fitted right before the first write, one kernel between: eagerly and captured, with other levels each time, behind other work."""
+@pytest.mark.parametrize("last", ["another kernel", "codebooks", "thresholds"])
+def test_codebooks_that_have_just_been_written(pkg, cuda_device, bits, tokens, new, last):
+    """Fitted right before the first write, by the kernel before it or the one before that: eagerly and captured, with other levels each time,
+    behind other work."""
     gen = torch.Generator().manual_seed(bits + tokens)
     pages = -(-tokens // 16)
     c, th = _empty_cache(pages, 2, 16, bits, torch.float16, cuda_device)
@@ -120,9 +122,14 @@ def test_codebooks_that_have_just_been_written(pkg, cuda_device, bits, tokens, n
 
     def fit_and_use():
         other.add_(1.0)
-        th.copy_(base_th * factor)
-        c["codebooks"].copy_(base_cb * factor)
-        other[:4].add_(1.0)                                            # the kernel between
+        if last == "thresholds":
+            torch.mul(base_cb, factor, out=c["codebooks"])
+            torch.mul(base_th, factor, out=th)
+        else:
+            torch.mul(base_th, factor, out=th)
+            torch.mul(base_cb, factor, out=c["codebooks"])
+        if last == "another kernel":
+            other[:4].add_(1.0)
         pkg.ops.kv_cache_write(k, v, slots, thresholds=th, **c)
         read = pkg.ops.kv_cache_read(slots, **c)
         y = pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, length, None, new, **_args(c))

@@ -680,7 +680,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
       seen_after = copy_step();
       cp_async_wait<2>();
       __syncwarp();
-      const uint32_t src = ring + slot * Step::kBytes, seen = seen_now;
+      const uint32_t src = ring + slot * Step::kBytes;
+      uint32_t seen = seen_now;
       slot = slot + 1 == kSplitStages ? 0 : slot + 1;
       const int base = key_base + step * KEYS;
       const bool all = seen == (KEYS == 32 ? 0xffffffffu : 0xffffu);
@@ -752,6 +753,18 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
             const int key = PACKED ? 8 * c + key_in_eight(n, j & 1) : 8 * n + 2 * c + (j & 1);
             if (((seen >> key) & 1) == 0 || base + key >= limit[j >> 1]) s[n][j] = ninf;
           }
+        if constexpr (PACKED) {
+          // Values that are NaN, and only some of the rows see them: 0 * NaN would show in the others.  They are left out from here on, and the
+          // sums of the rows that see one are NaN instead.
+          const uint32_t own = lds32(src + 2 * Step::kRows + Step::kStats + lane * 4);
+          const uint32_t bad = seen & __ballot_sync(0xffffffffu, (own & 0x7C00u) == 0x7C00u || (own & 0x7C000000u) == 0x7C000000u);
+          if (bad != 0) {
+            seen &= ~bad;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (base + __ffs(bad) - 1 < limit[h]) sum[h] = __int_as_float(0x7fffffff);
+          }
+        }
       }
       // Packed: the values' scales go into the probabilities, sum p (scale * level + center) = sum (p scale) level + sum p center.  A row's
       // exponents are taken against the largest of a key's score plus its scale (log2, rounded down), so that p * scale stays in fp16's range;
@@ -824,7 +837,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) split_attention_kernel(const
         const uint32_t stats = src + 2 * Step::kRows + Step::kStats + c * 32;
         const uint4 v0 = lds128(stats), v1 = lds128(stats + 16);
         vst[0] = v0.x; vst[1] = v0.y; vst[2] = v0.z; vst[3] = v0.w; vst[4] = v1.x; vst[5] = v1.y; vst[6] = v1.z; vst[7] = v1.w;
-        if (!all) {
+        if (seen != 0xffffffffu) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) vst[j] = (seen >> (8 * c + j)) & 1 ? vst[j] : 0u;
         }

@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
   uint64_t *const q_full = bars + 20, *const s_full = bars + 22, *const s_read = bars + 24, *const p_full = bars + 26, *const o_done = bars + 28;   // [stream]
   uint64_t* const stopped = bars + 30;
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 31);
+  int* const s_first_bad = reinterpret_cast<int*>(s_tmem + 1);                    // packed: the first key whose values are NaN
   uint32_t* const s_seen = reinterpret_cast<uint32_t*>(smem + L.seen);            // [tile % kTileSeen][warp]: written before the tile's keys are handed over
   float* const s_max = reinterpret_cast<float*>(smem + L.max);                    // [stream][row]
   float* const s_sum = reinterpret_cast<float*>(smem + L.sum);
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
       mbar_init(k_full + i, 4); mbar_init(v_full + i, 4);
       mbar_init(k_free + i, users); mbar_init(v_free + i, users);
     }
+    *s_first_bad = 0x7fffffff;
     for (int t = 0; t < STREAMS; ++t) {
       mbar_init(s_read + t, 4); mbar_init(p_full + t, 4);
       mbar_init(s_full + t, 1); mbar_init(o_done + t, 1);
@@ -396,7 +398,13 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
         write_keys(k_smem + slot * kTileBytes + row, k);
         hand_over(k_full + slot);
         wait_free(v_free, j);
-        write_values(v_smem + slot * kTileBytes + row, v);
+        // Values that are NaN are left out of the products, where 0 * NaN would show in rows that do not see them; those that do get it below.
+        Row used = v;
+        if ((v.stats & 0x7C00u) == 0x7C00u || (v.stats & 0x7C000000u) == 0x7C000000u) {
+          used.stats = 0;
+          atomicMin(s_first_bad, (first + j) * kTileKeys + 32 * w + lane);
+        }
+        write_values(v_smem + slot * kTileBytes + row, used);
         hand_over(v_full + slot);
       }
     }
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(tile_threads(STREAMS), 3 - STREAMS) tile_atten
     float x, y;
     unpack2(add2(sum0, sum1), x, y);
     s_max[t * kTileRows + r] = top;
-    s_sum[t * kTileRows + r] = x + y;
+    s_sum[t * kTileRows + r] = PACKED && *s_first_bad < limit ? __int_as_float(0x7fffffff) : x + y;
   }
   // ---------------------------------------------------------------------- join and write
   // All copies into the key and value slots have landed (their products have ended) or nobody waits for them any more.

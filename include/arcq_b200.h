@@ -445,8 +445,8 @@ int arcq_kv_cache_read(const arcq_kv_cache* cache, const int64_t* slots, int64_t
  * heads is a multiple of cache.heads: query head h reads key head h / (heads / cache.heads).  Packed keys and values are rebuilt in
  * fp16, one half-precision fma each, so |center| + 3 scale has to stay within fp16's range; products accumulate in fp32, probabilities are rounded
  * to 16 bits for the second one.  In calls with few queries a level is rounded to fp16 up or down instead, in turn over the keys, and center and
- * scale come in fp32.  NaN and infinities in keys and values that none of a sequence's queries sees have no effect; in values that only its later
- * queries see they may show in the earlier ones'.
+ * scale come in fp32.  NaN and infinities in keys and values have no effect on queries that do not see them, but for values in 16-bit pages that
+ * later queries of the same sequence see: they may show in the earlier ones'.
  *   workspace  arcq_attention_workspace bytes of the call's own until it has run, 16-byte aligned (NULL where that is 0)
  */
 int64_t arcq_attention_workspace(int64_t batch, int64_t max_new, int64_t heads, int64_t kv_heads);

@@ -185,3 +185,32 @@ def test_queries_of_bf16_at_the_ends_of_their_range(pkg, cuda_device, new):
     assert bool(torch.isfinite(want).all())
     for e in (-100, 100, 120):
         assert torch.equal(run(e), want), e
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4])
+@pytest.mark.parametrize("new", [2, 9, 40, 130, 300])
+@pytest.mark.parametrize("at", [-1, -2, "half"])
+@pytest.mark.parametrize("both", [False, True])
+def test_a_later_value_that_is_nan_has_no_effect_on_earlier_queries(pkg, cuda_device, bits, new, at, both):
+    """Packed pages: the queries that see a value with a NaN are NaN, the others are what they are without it."""
+    at = 349 - (new // 2 if at == "half" else -at - 1)
+    gen = torch.Generator().manual_seed(5)
+    x = [torch.randn(352, 1, 64, generator=gen).half().to(cuda_device) for _ in range(2)]
+    q = torch.randn(new, 2, 64, generator=gen).half().to(cuda_device)
+    table = torch.arange(22, dtype=torch.int32, device=cuda_device)[None]
+    length = torch.tensor([350], dtype=torch.int32, device=cuda_device)
+    outs = []
+    for planted in (False, True):
+        if planted:
+            x[1][at, 0, 3] = INF
+            if both:
+                x[1][349, 0, 9] = NAN
+        c, th = _empty_cache(22, 1, 16, bits, torch.float16, cuda_device)
+        pkg.ops.kv_cache_write(x[0], x[1], torch.arange(352, device=cuda_device), thresholds=th, **c)
+        outs.append(pkg.ops.paged_attention(q, c["k_pages"], c["v_pages"], table, length, None, new, **_pages_args(c)))
+    sees = torch.arange(new) >= at - (350 - new)
+    assert bool(torch.isnan(outs[1][sees.to(cuda_device)]).all())
+    earlier = (~sees).to(cuda_device)
+    # the few-row kernel's exponents may be taken against another maximum: two roundings of weights and outputs below 4
+    assert bool(((outs[1][earlier].double() - outs[0][earlier].double()).abs() <= 4 * 4 * 2.0 ** -11).all())
+    assert pkg.ops.device_status() == 0

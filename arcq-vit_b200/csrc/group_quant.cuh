@@ -57,15 +57,18 @@ struct GroupQuantParams {            // the same in every thread of the block
   f32x2 nz;                          // two -0 (see mul2_rn)
 };
 
-// Fills the tables; threads 0 to 15 come with a threshold (+inf from L - 1 on) and a level each.  `sync_and(bool)` is a barrier over exactly
-// the `nthreads` calling threads (numbered `tid`) that returns the conjunction of its arguments.  Ends with a barrier: the tables are complete
-// on return.
-template <int L, bool CODES, typename SyncAnd>
-__device__ __forceinline__ GroupQuantParams group_quant_tables_of(GroupQuantTables* t, float threshold, float level, int tid, int nthreads,
-                                                                  SyncAnd sync_and) {
+struct LoadConstant {
+  __device__ __forceinline__ float operator()(const float* at) const { return __ldg(at); }
+};
+// Fills the tables; `sync_and(bool)` is a barrier over exactly the `nthreads` calling threads (numbered `tid`) that
+// returns the conjunction of its arguments.  Ends with a barrier: the tables are complete on return.
+template <int L, bool CODES, typename SyncAnd, typename Load = LoadConstant>
+__device__ __forceinline__ GroupQuantParams group_quant_tables(GroupQuantTables* t, const float* __restrict__ thresholds,
+                                                               const float* __restrict__ codebook, int tid, int nthreads,
+                                                               SyncAnd sync_and, Load load = Load()) {
   if (tid < 16) {
-    t->th[tid] = threshold;
-    t->cb[tid] = level;
+    t->th[tid] = tid < L - 1 ? load(thresholds + tid) : __int_as_float(0x7f800000);
+    t->cb[tid] = tid < L ? load(codebook + tid) : 0.0f;
   }
   if (tid == 0) t->nz = -0.0f;
   sync_and(true);
@@ -99,14 +102,6 @@ __device__ __forceinline__ GroupQuantParams group_quant_tables_of(GroupQuantTabl
   p.nz = pack2(t->nz, t->nz);
   sync_and(true);
   return p;
-}
-
-template <int L, bool CODES, typename SyncAnd>
-__device__ __forceinline__ GroupQuantParams group_quant_tables(GroupQuantTables* t, const float* __restrict__ thresholds,
-                                                               const float* __restrict__ codebook, int tid, int nthreads,
-                                                               SyncAnd sync_and) {
-  return group_quant_tables_of<L, CODES>(t, tid < L - 1 ? __ldg(thresholds + tid) : __int_as_float(0x7f800000), tid < L ? __ldg(codebook + tid) : 0.0f,
-                                         tid, nthreads, sync_and);
 }
 
 // The exact code of one value: IEEE quotient, search in the sorted thresholds.

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
 // Many tokens, 16-bit values: a lane a group (group_quant.cuh), 32 groups a warp and step, the next step's rows on their way meanwhile.  Eight
 // lanes copy a row, so a row may lie anywhere; codes and statistics leave from registers, a full 32-byte sector of codes a row in 4 bits.
 // Bound by the quantizer's issue slots like the kernels that it shares them with: 16 384 tokens of 12 heads in 4 bits (50 MB in, 14 MB out)
-// 24 us, 61 with the octets of kv_write_kernel.
+// 24.8 us, 61 with the octets of kv_write_kernel.
 constexpr int kWriteWarps = 4, kWriteThreads = kWriteWarps * 32;
 constexpr uint32_t kWriteTables = kWriteWarps * 2 * 4096;
 constexpr uint32_t kWriteSmem = 1024 + kWriteTables + (sizeof(GroupQuantTables) + 15) / 16 * 16;
@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(kWriteThreads, 4) kv_write_tile_kernel(const _
   int buf = 0;
   constexpr int L = 1 << BITS;
   auto make_tables = [&] {
-    const float th = tid < L - 1 ? load_settled(kv.thresholds + tid) : __int_as_float(0x7f800000), cb = tid < L ? load_settled(kv.levels + tid) : 0.0f;
-    return group_quant_tables_of<L, true>(tables, th, cb, tid, kWriteThreads, [](bool b) { return __syncthreads_and(b) != 0; });
+    return group_quant_tables<L, true>(tables, kv.thresholds, kv.levels, tid, kWriteThreads, [](bool b) { return __syncthreads_and(b) != 0; },
+                                       [](const float* at) { return load_settled(at); });
   };
   GroupQuantParams gp = make_tables();
   pdl_wait();
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kWriteThreads, 4) kv_write_tile_kernel(const _
   }
 }
 
-// 16 bits: a copy, 16 bytes a thread
+// 16 bits: a copy, 16 bytes a thread.  16 384 tokens of 12 heads (50 MB in and out each) 20.2 us, 15.4 at the copy bandwidth.
 __global__ void __launch_bounds__(256) kv_write_copy_kernel(const __grid_constant__ KvCacheParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -267,8 +267,9 @@ template <typename O> __device__ __forceinline__ void store_sixteen(O* out, cons
 }
 
 // Sixteen values a thread, a sector of the output in 16 bits.  BITS 16: pages of type T.  Levels come from a table of 16 in shared memory (as many
-// banks, so no conflicts).  16 384 tokens of 12 heads in 4 bits (14 MB in, 50 MB out) 12.6 us, 16.5 with eight values a thread, where the addresses
-// cost twice as much; 40 009 tokens of 3 heads in 3 bits, all over the cache, 10.2 us, 11.4.
+// banks, so no conflicts).  16 384 tokens of 12 heads in 4 bits (14 MB in, 50 MB out) one after the other 12.6 us, 16.5 with eight values a thread,
+// where the addresses cost twice as much; all over the cache 14.0 us, in 16 bits (50 MB in) 19.1; 40 009 tokens of 3 heads in 3 bits, all over the
+// cache, 9.2 us.
 template <typename T, int BITS, typename O>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvCacheParams p) {
   pdl_launch_dependents();

@@ -250,7 +250,11 @@ template <typename Kernel> int clusters_at_a_time(Kernel k, int size, int thread
   cudaGetLastError();
   return 0;
 }
-constexpr double kTileSetUp = 7.0;         // of a block, in tiles of keys: 13 us against 1.75 us
+// What a round of blocks counts besides its tiles of keys, in tiles (1.7 us for both streams): more than a block's set-up, which is some 4 by tile_time,
+// since blocks of a further round start unevenly.  Over 27 calls of 1 to 24 sequences and 64 to 2048 queries it hardly matters (2, 4, 7 and 10 within
+// 0.1 % of one another in all); 13 sequences of 256 over 2000, 12 heads, 4 bits: 75.4 us with 2 and 4, 73.7 with 7 and 10; 13 x 256 over 2309 in 16 bits
+// 75.6 and 76.7.
+constexpr double kTileSetUp = 7.0;
 
 // Blocks of a row tile, 1 to 8: the cluster size for which the rounds of blocks over the SMs take the fewest tiles of keys, a block's set-up and
 // the joining of results counted as tiles.

@@ -18,14 +18,17 @@
 //   q . k_j = scale_j (q . level_j) + center_j sum(q),    sum_j p_j v_j = sum_j (p_j scale_j) level_j + sum_j p_j center_j
 // Rounded to fp16 a level is off by the same amount wherever its code stands, which would add up over a long context; its copies are rounded up or
 // down in the share of its position between the two, and lanes serve different keys, so that it averages out (error against 64 bits over 65 521
-// keys of 3 bits, relative to the output: 3.9e-4 with all copies rounded alike, 2.0e-4 so, which is the output's own rounding).  p_j scale_j is
+// keys of 3 bits, relative to the output: 3.9e-4 with all copies rounded alike, 2.1e-4 so, which is the output's own rounding).  p_j scale_j is
 // rounded to fp16 as p_j is without scales.  Pairs of keys' values are a byte as it is stored; of values, which have to be paired along the
 // keys, the codes of two keys are interleaved.  The order of a head's values in a product is free, and so is that of keys: each lane takes values
 // that lie side by side.
 //
-// Bound by instructions: some 700 a step and warp (32 keys, 16 rows or fewer), three warps a scheduler, 0.83 issued a cycle.  1 token over 64
-// contexts of up to 4096, 12 heads over 4 key heads, 4 bits: 29 us, 25 % of the copy bandwidth (47 MB); over two of 65 521 in 3 bits, 12 heads: 51 us.
-// Few steps: set-up and latency, 1 token over 333: 8.5 us.
+// 1 token over 64 contexts of up to 4096, 12 heads over 4 key heads, 4 bits: 29.3 us, 25 % of the copy bandwidth (47 MB); over two of 65 521 in 3
+// bits, 12 heads: 52.7 us.  Two things take that time, in about equal parts for the first: launches, set-up and the join, during which little is
+// issued (0.42 a scheduler and cycle over the whole call), and 660 instructions a step and warp (32 keys, 16 rows or fewer; counted over the call, by
+// pipe 214 integer, 240 fp32, 103 loads and stores).  Table reads, their addresses, row reads and the interleaving of values are a quarter of
+// them; of the fp32 pipe's, scores, exponents and scales account for some 90.
+// Few steps: set-up and latency, 1 token over 333: 9.0 us.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>

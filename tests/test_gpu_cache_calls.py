@@ -156,3 +156,21 @@ def test_codebooks_that_have_just_been_written(pkg, cuda_device, bits, tokens, n
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want[f])), f
     assert pkg.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4])
+def test_a_cache_with_codebooks_fitted_to_the_first_prompt(pkg, cuda_device, bits):
+    """As a layer's are fitted: what is read back is the quantizer's reconstruction but for center and scale in fp16."""
+    gen = torch.Generator().manual_seed(bits)
+    k, v = ((torch.randn(300, 2, 64, generator=gen) + 0.3).half().to(cuda_device) for _ in range(2))
+    fits = [pkg.codebook.calibrate_codebook(t.reshape(-1, 64), bits=bits) for t in (k, v)]
+    codebooks, thresholds = (torch.stack(t) for t in zip(*fits))
+    c, _ = _empty_cache(20, 2, 16, bits, torch.float16, cuda_device)
+    c["codebooks"] = codebooks
+    slots = torch.arange(300, device=cuda_device)
+    pkg.ops.kv_cache_write(k, v, slots, thresholds=thresholds, **c)
+    for i, (x, got) in enumerate(zip((k, v), pkg.ops.kv_cache_read(slots, out_dtype=torch.float32, **c))):
+        want = pkg.ops.quantize_activation_dequant(x.reshape(300, 128), thresholds[i], codebooks[i], bits, 64).reshape(x.shape).double()
+        st = c["kv"[i] + "_stats"][:19].permute(0, 2, 1, 3).reshape(304, 2, 2)[:300].double()
+        off = 2.0 ** -11 * (st[..., :1].abs() + (want - st[..., :1]).abs()) * 1.01 + 2.0 ** -20 * want.abs() + 2.0 ** -24
+        assert bool(((got.double() - want).abs() <= off).all())
